@@ -10,6 +10,8 @@ from .capi import (  # noqa: F401
     MODES,
     SafetensorsFile,
     Weights,
+    attention,
+    attention_paged,
     weights_free,
     declared_symbols,
     device_weights,
@@ -34,7 +36,10 @@ from .capi import (  # noqa: F401
     linear_raw,
     load,
     pack_act_f16,
+    qkv_rope,
+    qkv_rope_paged,
     quantize_f32,
+    rms_norm,
     swiglu_pack_f16,
     workspace_bytes,
 )

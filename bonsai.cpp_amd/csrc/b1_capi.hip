@@ -443,6 +443,244 @@ int bonsai_b1_norm_mod_pack_f16(const float *x, int64_t ldx, int H, int rows, co
                : BONSAI_B1_ERR_HIP;
 }
 
+// ---- the operators around a block's linears ----
+
+// A 16-byte aligned pointer to rows of `cols` values whose stride keeps them
+// so (`unit` values are 16 bytes); NULL is not.
+static bool rows_ok(const void *p, int64_t ld, int64_t cols, int unit) {
+    return p && !(reinterpret_cast<uintptr_t>(p) & 15u) && ld >= cols && ld % unit == 0;
+}
+
+static int rms_norm_args(const float *x, int64_t ldx, const float *add, int64_t lda, int H, int rows,
+                         const float *weight, float eps, const float *h, int64_t ldh) {
+    if (H <= 0 || H % BONSAI_B1_BLOCK_SIZE || rows < 0 || !(eps >= 0.f)) return BONSAI_B1_ERR_ARG;
+    if (rows > 0 && !rows_ok(x, ldx, H, 4)) return BONSAI_B1_ERR_ARG;
+    if (add && !rows_ok(add, lda, H, 4)) return BONSAI_B1_ERR_ARG;
+    if (h && !rows_ok(h, ldh, H, 4)) return BONSAI_B1_ERR_ARG;
+    // in place: a row's values are read before they are written
+    if (h && ((h == x && ldh != ldx) || (h == add && ldh != lda))) return BONSAI_B1_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(weight) & 15u) return BONSAI_B1_ERR_ARG;
+    return BONSAI_B1_OK;
+}
+
+int bonsai_b1_rms_norm_f32(const float *x, int64_t ldx, const float *add, int64_t ld_add, int H, int rows,
+                           const float *weight, float eps, float *h, int64_t ldh, float *y, int64_t ldy,
+                           hipStream_t stream) {
+    const int st = rms_norm_args(x, ldx, add, ld_add, H, rows, weight, eps, h, ldh);
+    if (st != BONSAI_B1_OK) return st;
+    if (rows > 0 && !rows_ok(y, ldy, H, 4)) return BONSAI_B1_ERR_ARG;
+    if (!current_device(nullptr)) return BONSAI_B1_ERR_DEVICE;
+    if (rows == 0) return BONSAI_B1_OK;
+    return b1::launch_rms_norm(x, ldx, add, ld_add, H, rows, weight, eps, h, ldh, y, ldy, nullptr, stream) ==
+                   hipSuccess
+               ? BONSAI_B1_OK
+               : BONSAI_B1_ERR_HIP;
+}
+
+int bonsai_b1_rms_norm_pack_f16(const float *x, int64_t ldx, const float *add, int64_t ld_add, int H, int rows,
+                                const float *weight, float eps, float *h, int64_t ldh, void *packed,
+                                hipStream_t stream) {
+    const int st = rms_norm_args(x, ldx, add, ld_add, H, rows, weight, eps, h, ldh);
+    if (st != BONSAI_B1_OK) return st;
+    if (rows > 0 && !rows_ok(packed, H, H, 8)) return BONSAI_B1_ERR_ARG;
+    if (!current_device(nullptr)) return BONSAI_B1_ERR_DEVICE;
+    if (rows == 0) return BONSAI_B1_OK;
+    return b1::launch_rms_norm(x, ldx, add, ld_add, H, rows, weight, eps, h, ldh, nullptr, 0, packed, stream) ==
+                   hipSuccess
+               ? BONSAI_B1_OK
+               : BONSAI_B1_ERR_HIP;
+}
+
+// Head layout and counts shared by the q/k/v and attention entries.  A
+// call's rows (tokens x heads) stay below 2^28, which keeps every index of a
+// row or work item in 32 bits and every grid within the launch limit.
+static bool heads_ok(int tokens, int heads, int kv_heads, int head_dim, int dtype) {
+    if (tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return false;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return false;
+    if (dtype != BONSAI_B1_F16 && dtype != BONSAI_B1_BF16) return false;
+    return (int64_t)tokens * heads < (1 << 28) && heads < (1 << 20) && tokens < (1 << 24);
+}
+
+static bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < ((int64_t)1 << 40); }
+
+static bool pages_ok(const bonsai_b1_kv_pages *p, int n_seqs, int kv_heads, int head_dim) {
+    if (!p->k || !p->v || ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15u))
+        return false;
+    if (p->n_pages <= 0 || p->page_size <= 0 || (p->page_size & (p->page_size - 1))) return false;
+    if (!stride_ok(p->page_stride) || !stride_ok(p->head_stride) || !stride_ok(p->row_stride)) return false;
+    // rows and heads apart from one another
+    if (p->row_stride < head_dim && p->page_size > 1) return false;
+    if (p->head_stride < head_dim && kv_heads > 1) return false;
+    if (p->page_stride < head_dim && p->n_pages > 1) return false;
+    if (p->max_pages <= 0 || p->ld_pages < p->max_pages || n_seqs <= 0 || !p->pages || !p->kv_len) return false;
+    if ((reinterpret_cast<uintptr_t>(p->pages) | reinterpret_cast<uintptr_t>(p->kv_len)) & 3u) return false;
+    return (int64_t)p->max_pages * p->page_size < (1 << 30);
+}
+
+static void set_pages(b1::KvSeqs *s, const bonsai_b1_kv_pages *p) {
+    s->pages = p->pages;
+    s->ld_pages = p->ld_pages;
+    s->max_pages = p->max_pages;
+    s->n_pages = p->n_pages;
+    s->page_shift = __builtin_ctz((unsigned)p->page_size);
+    s->kv_len = p->kv_len;
+}
+
+int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *g, hipStream_t stream) {
+    if (!g || !heads_ok(g->tokens, g->heads, g->kv_heads, g->head_dim, g->dtype) || !(g->eps >= 0.f))
+        return BONSAI_B1_ERR_ARG;
+    const int64_t nq = (int64_t)g->heads * g->head_dim, nk = (int64_t)g->kv_heads * g->head_dim;
+    if ((reinterpret_cast<uintptr_t>(g->q_weight) | reinterpret_cast<uintptr_t>(g->k_weight)) & 15u)
+        return BONSAI_B1_ERR_ARG;
+    if (g->rope && (g->rope_rows <= 0 || g->rope_dim <= 0 || g->rope_dim % 8 || g->rope_dim > g->head_dim ||
+                    (reinterpret_cast<uintptr_t>(g->rope) & 15u)))
+        return BONSAI_B1_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(g->positions) | reinterpret_cast<uintptr_t>(g->q_start) |
+         reinterpret_cast<uintptr_t>(g->bad)) & 3u)
+        return BONSAI_B1_ERR_ARG;
+    if (g->pages) {
+        if (g->tokens > 0 && !pages_ok(g->pages, g->n_seqs, g->kv_heads, g->head_dim)) return BONSAI_B1_ERR_ARG;
+        if (!g->q_start && g->n_seqs > 1) return BONSAI_B1_ERR_ARG;
+    }
+    if (g->tokens > 0) {
+        if (!rows_ok(g->q, g->ldq, nq, 4) || !rows_ok(g->k, g->ldk, nk, 4) || !rows_ok(g->v, g->ldv, nk, 4))
+            return BONSAI_B1_ERR_ARG;
+        if (!rows_ok(g->q_out, g->ld_q, nq, 8)) return BONSAI_B1_ERR_ARG;
+        if (!g->pages && (!rows_ok(g->k_out, g->ld_kv, nk, 8) || !rows_ok(g->v_out, g->ld_kv, nk, 8)))
+            return BONSAI_B1_ERR_ARG;
+    }
+    if (!current_device(nullptr)) return BONSAI_B1_ERR_DEVICE;
+    if (g->tokens == 0) return BONSAI_B1_OK;
+    b1::QkvArgs a{};
+    a.q = g->q;
+    a.k = g->k;
+    a.v = g->v;
+    a.ldq = g->ldq;
+    a.ldk = g->ldk;
+    a.ldv = g->ldv;
+    a.heads = g->heads;
+    a.kv_heads = g->kv_heads;
+    a.head_dim = g->head_dim;
+    a.tokens = g->tokens;
+    a.bf16 = g->dtype == BONSAI_B1_BF16;
+    a.q_weight = g->q_weight;
+    a.k_weight = g->k_weight;
+    a.eps = g->eps;
+    a.rope = g->rope;
+    a.rope_rows = g->rope_rows;
+    a.rope_dim = g->rope ? g->rope_dim : 0;
+    a.interleaved = g->interleaved != 0;
+    a.positions = g->positions;
+    a.q_out = static_cast<uint16_t *>(g->q_out);
+    a.q_row = g->ld_q;
+    a.bad = g->bad;
+    if (g->pages) {
+        a.k_out = static_cast<uint16_t *>(g->pages->k);
+        a.v_out = static_cast<uint16_t *>(g->pages->v);
+        a.kv_page = g->pages->page_stride;
+        a.kv_head = g->pages->head_stride;
+        a.kv_row = g->pages->row_stride;
+        set_pages(&a.seqs, g->pages);
+        a.seqs.n_seqs = g->n_seqs;
+        a.seqs.tokens = g->tokens;
+        a.seqs.q_start = g->q_start;
+    } else {
+        a.k_out = static_cast<uint16_t *>(g->k_out);
+        a.v_out = static_cast<uint16_t *>(g->v_out);
+        a.kv_head = g->head_dim;
+        a.kv_row = g->ld_kv;
+    }
+    return b1::launch_qkv(a, stream) == hipSuccess ? BONSAI_B1_OK : BONSAI_B1_ERR_HIP;
+}
+
+// Checks an attention call and fills the kernels' arguments.
+static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
+    if (!g || !heads_ok(g->tokens, g->heads, g->kv_heads, g->head_dim, g->dtype)) return BONSAI_B1_ERR_ARG;
+    if (g->n_seqs < 0 || g->n_seqs >= (1 << 24) || g->window < 0 || (g->window > 0 && !g->causal))
+        return BONSAI_B1_ERR_ARG;
+    if (!(g->scale > 0.f) || g->scale > 3.0e38f) return BONSAI_B1_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(g->q_start) | reinterpret_cast<uintptr_t>(g->kv_start) |
+         reinterpret_cast<uintptr_t>(g->bad)) & 3u)
+        return BONSAI_B1_ERR_ARG;
+    if (!g->q_start && g->n_seqs > 1) return BONSAI_B1_ERR_ARG;
+    *a = b1::AttnArgs{};
+    a->seqs.n_seqs = g->n_seqs;
+    a->seqs.tokens = g->tokens;
+    a->seqs.q_start = g->q_start;
+    if (g->tokens == 0 || g->n_seqs == 0) return BONSAI_B1_OK;
+    const int64_t row = (int64_t)g->heads * g->head_dim;
+    if (!rows_ok(g->out, g->ldo, row, 8) || !stride_ok(g->ldo)) return BONSAI_B1_ERR_ARG;
+    if (!rows_ok(g->q, g->q_row, 0, 8) || !stride_ok(g->q_row) || !stride_ok(g->q_head)) return BONSAI_B1_ERR_ARG;
+    if (g->pages) {
+        if (!pages_ok(g->pages, g->n_seqs, g->kv_heads, g->head_dim)) return BONSAI_B1_ERR_ARG;
+        set_pages(&a->seqs, g->pages);
+        a->k = static_cast<const uint16_t *>(g->pages->k);
+        a->v = static_cast<const uint16_t *>(g->pages->v);
+        a->k_page = a->v_page = g->pages->page_stride;
+        a->k_row = a->v_row = g->pages->row_stride;
+        a->k_head = a->v_head = g->pages->head_stride;
+    } else {
+        if (g->kv_tokens < 0 || g->kv_tokens >= (1 << 30) || (!g->kv_start && g->n_seqs > 1))
+            return BONSAI_B1_ERR_ARG;
+        // no keys at all: k and v are not read
+        if (g->kv_tokens > 0 && (!rows_ok(g->k, g->k_row, 0, 8) || !rows_ok(g->v, g->v_row, 0, 8) ||
+                                 !stride_ok(g->k_row) || !stride_ok(g->k_head) || !stride_ok(g->v_row) ||
+                                 !stride_ok(g->v_head)))
+            return BONSAI_B1_ERR_ARG;
+        a->seqs.kv_tokens = g->kv_tokens;
+        a->seqs.kv_start = g->kv_start;
+        a->k = static_cast<const uint16_t *>(g->k);
+        a->v = static_cast<const uint16_t *>(g->v);
+        a->k_row = g->k_row;
+        a->k_head = g->k_head;
+        a->v_row = g->v_row;
+        a->v_head = g->v_head;
+    }
+    a->q = static_cast<const uint16_t *>(g->q);
+    a->q_row = g->q_row;
+    a->q_head = g->q_head;
+    a->heads = g->heads;
+    a->kv_heads = g->kv_heads;
+    a->head_dim = g->head_dim;
+    a->bf16 = g->dtype == BONSAI_B1_BF16;
+    a->causal = g->causal != 0;
+    a->window = g->window;
+    a->scale = g->scale;
+    a->out = static_cast<uint16_t *>(g->out);
+    a->ldo = g->ldo;
+    a->packed = g->packed != 0;
+    a->bad = g->bad;
+    return BONSAI_B1_OK;
+}
+
+size_t bonsai_b1_attention_workspace_bytes(const bonsai_b1_attention_args *args) {
+    b1::AttnArgs a;
+    if (attention_args(args, &a) != BONSAI_B1_OK || a.seqs.tokens == 0 || a.seqs.n_seqs == 0) return 0;
+    DeviceInfo *dev = current_device(nullptr);
+    return dev ? b1::attn_workspace_bytes(a, dev->num_cus) : 0;
+}
+
+int bonsai_b1_attention(const bonsai_b1_attention_args *args, void *workspace, size_t workspace_bytes,
+                        hipStream_t stream) {
+    b1::AttnArgs a;
+    const int st = attention_args(args, &a);
+    if (st != BONSAI_B1_OK) return st;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) return BONSAI_B1_ERR_ARG;
+    DeviceInfo *dev = current_device(nullptr);
+    if (!dev) return BONSAI_B1_ERR_DEVICE;
+    if (a.seqs.tokens == 0 || a.seqs.n_seqs == 0) return BONSAI_B1_OK;
+    WsLease lease;
+    if (!workspace) {
+        workspace_bytes = b1::attn_workspace_bytes(a, dev->num_cus);
+        if (workspace_bytes > 0) {
+            lease.acquire(dev, stream, workspace_bytes);
+            workspace = lease.ptr();
+        }
+    }
+    return b1::launch_attn(a, dev->num_cus, workspace, workspace_bytes, stream) == hipSuccess ? BONSAI_B1_OK
+                                                                                             : BONSAI_B1_ERR_HIP;
+}
+
 int bonsai_b1_quantize_f32(const float *w, int64_t ldw, int in_dim, int out_dim, void *packed, int order,
                            hipStream_t stream) {
     if (in_dim <= 0 || out_dim < 0 || in_dim % BONSAI_B1_BLOCK_SIZE || ldw < in_dim) return BONSAI_B1_ERR_ARG;

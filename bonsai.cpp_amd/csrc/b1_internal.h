@@ -195,6 +195,74 @@ hipError_t launch_gelu_pack(const float *act, int64_t lda, int M, int K, void *p
 hipError_t launch_swiglu_pack(const float *act, int64_t lda, int M, int H, void *packed, int64_t ldp,
                               hipStream_t s);
 
+// RMS norm over rows of h = x (+ add): y = h / sqrt(mean(h^2) + eps) * w, in
+// fp32 (y [rows][ldy]) or as packed fp16 activations (packed, row stride H);
+// h stored when `h` is given (x or add themselves allowed).  H % 32 == 0,
+// rows and vectors 16-byte aligned.
+hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_t lda, int H, int rows,
+                           const float *w, float eps, float *h, int64_t ldh, float *y, int64_t ldy, void *packed,
+                           hipStream_t s);
+
+// Sequences and their keys, as every attention kernel sees them.  Tokens of
+// sequence b are rows q_start[b] .. q_start[b + 1] (NULL: one sequence of
+// all tokens); its keys are rows kv_start[b] .. of k and v, or with `pages`
+// the first kv_len[b] places of its pages.
+struct KvSeqs {
+    int n_seqs, tokens;
+    const int32_t *q_start;
+    int kv_tokens; // contiguous keys
+    const int32_t *kv_start;
+    const int32_t *pages; // [n_seqs][ld_pages], or NULL: contiguous keys
+    int64_t ld_pages;
+    int max_pages, n_pages, page_shift;
+    const int32_t *kv_len;
+};
+
+struct AttnArgs {
+    const uint16_t *q, *k, *v;
+    int64_t q_row, q_head;
+    int64_t k_page, k_row, k_head; // element strides (k_page: paged keys)
+    int64_t v_page, v_row, v_head;
+    KvSeqs seqs;
+    int heads, kv_heads, head_dim, bf16;
+    int causal, window;
+    float scale;
+    uint16_t *out; // rows [tokens][ldo], or packed fp16 activations
+    int64_t ldo;
+    int packed;
+    int32_t *bad; // device counter of bad indexes, or NULL
+    // filled by attn_plan / launch_attn
+    int splits = 1;  // key ranges a row's keys may be split into
+    int target = 0;  // small kernel: work-groups wanted
+    float *part_o = nullptr;   // [splits][tokens * heads][head_dim]
+    float *part_ml = nullptr; // [splits][tokens * heads][2]: maximum (base 2), sum
+};
+
+// Workspace bytes of a call, for a device of num_cus (0: none).
+size_t attn_workspace_bytes(const AttnArgs &a, int num_cus);
+// Runs without a workspace too (ws NULL or too small), its keys unsplit.
+hipError_t launch_attn(const AttnArgs &a, int num_cus, void *ws, size_t ws_bytes, hipStream_t s);
+
+// fp32 q, k, v rows of a linear -> head norm (weights or NULL), rotary
+// embedding (table rows of rope_dim: cos then sin; or NULL), 16 bits; k and
+// v as rows or into the pages of seqs.pages.
+struct QkvArgs {
+    const float *q, *k, *v;
+    int64_t ldq, ldk, ldv;
+    int heads, kv_heads, head_dim, tokens, bf16;
+    const float *q_weight, *k_weight;
+    float eps;
+    const float *rope;
+    int rope_rows, rope_dim, interleaved;
+    const int32_t *positions; // [tokens] or NULL
+    uint16_t *q_out, *k_out, *v_out;
+    int64_t q_row;                    // q_out row stride
+    int64_t kv_page, kv_head, kv_row; // k_out, v_out strides
+    KvSeqs seqs;                      // seqs.pages == NULL: rows
+    int32_t *bad;
+};
+hipError_t launch_qkv(const QkvArgs &a, hipStream_t s);
+
 // Packed B1_0 writer over device fp32 weights [N][ldw]; order 0 = numpy's
 // np.mean summation, 1 = left to right.
 hipError_t launch_quantize(const float *w, int64_t ldw, int K, int N, void *packed, int order, hipStream_t s);

@@ -563,6 +563,149 @@ int bonsai_b1_swiglu_pack_f16_ld(const float *act, int64_t lda, int hidden,
                                  hipStream_t stream);
 
 /*
+ * RMS norm with the residual's addition, the pre-norm of a decoder block:
+ *   h = x + add,  y = h / sqrt(mean(h^2) + eps) * weight
+ * over rows of H, in fp32.  add may be NULL (h = x); h is stored when `h` is
+ * given, which may be x or add themselves (same row stride), and must not
+ * overlap them otherwise.  weight may be NULL (1).  The _pack form writes
+ * the packed fp16 activations of y that bonsai_b1_linear_packed_f16 reads
+ * (row stride H; |y| beyond 65504 becomes +-inf there).  H % 32 == 0;
+ * pointers 16-byte aligned, row strides multiples of 4.
+ */
+int bonsai_b1_rms_norm_f32(const float *x, int64_t ldx, const float *add,
+                           int64_t ld_add, int H, int rows,
+                           const float *weight, float eps, float *h,
+                           int64_t ldh, float *y, int64_t ldy,
+                           hipStream_t stream);
+int bonsai_b1_rms_norm_pack_f16(const float *x, int64_t ldx, const float *add,
+                                int64_t ld_add, int H, int rows,
+                                const float *weight, float eps, float *h,
+                                int64_t ldh, void *packed,
+                                hipStream_t stream);
+
+/* 16-bit types of queries, keys, values and caches. */
+enum { BONSAI_B1_F16 = 0, BONSAI_B1_BF16 = 1 };
+
+/*
+ * A paged cache of keys and values and the sequences that use it.  Place j
+ * of sequence b is row j % page_size of page pages[b * ld_pages +
+ * j / page_size]; kv head h of row r of page p starts at element
+ * p * page_stride + h * head_stride + r * row_stride of k and of v.
+ * page_size: a power of two.  Strides: multiples of 8 elements; k and v
+ * 16-byte aligned.  Sequence b has kv_len[b] keys, its new tokens among
+ * them (they are its last ones).  Table entries behind a sequence's last
+ * page are not read.  max_pages * page_size < 2^30.
+ */
+typedef struct bonsai_b1_kv_pages {
+    void *k, *v;          /* device */
+    int n_pages;          /* pages in k and in v */
+    int page_size;
+    int64_t page_stride, head_stride, row_stride;
+    const int32_t *pages; /* device [n_seqs][ld_pages] */
+    int64_t ld_pages;
+    int max_pages;        /* entries of a table row, <= ld_pages */
+    const int32_t *kv_len; /* device [n_seqs] */
+} bonsai_b1_kv_pages;
+
+/*
+ * Indexes in device memory (starts, lengths, page tables, positions) are
+ * read by the kernels alone.  Each is brought into range before it addresses
+ * anything; a row that depends on one that was not in range comes out NaN,
+ * nothing of it is stored in a cache, and the optional device counter `bad`
+ * grows by at least 1 a call.  Sequences must not overlap; where they do,
+ * the rows they share are unspecified.
+ */
+
+/*
+ * From a linear's fp32 q/k/v columns to what attention reads: RMS norm of
+ * each q and k head (weights of head_dim, NULL: none), rotary embedding by
+ * table (NULL: none), and rounding to 16 bits.  A table row of rope_dim
+ * holds rope_dim / 2 cosines, then as many sines; columns from rope_dim on
+ * are not rotated.  With interleaved = 0 column i < rope_dim / 2 is turned
+ * with column i + rope_dim / 2, else column 2 i with 2 i + 1:
+ *   (a, b) -> (a cos - b sin, b cos + a sin).
+ * positions: the tokens' table rows; NULL: row i for token i, or with
+ * `pages` the token's place in its sequence.  Keys and values go to rows
+ * k_out, v_out (pages NULL; row stride ld_kv), or to their sequences' places
+ * in the cache: token i of sequence b (rows q_start[b] .. q_start[b + 1];
+ * NULL: one sequence) to place kv_len[b] - (its tokens) + i; rows of no
+ * sequence are left as they were.  No two of a call's tokens may have the
+ * same place in memory (pages that two sequences share).
+ * head_dim 64, 128 or 256; fp32 pointers 16-byte aligned, row strides
+ * multiples of 4; 16-bit pointers 16-byte aligned, strides multiples of 8;
+ * rope_dim a multiple of 8, <= head_dim.  The reference computes these as
+ * separate ggml ops on q and k (src/diffuser_graph.cpp:354-406 and
+ * src/b1_0_kernel.h:309-361, interleaved).
+ */
+typedef struct bonsai_b1_qkv_args {
+    const float *q, *k, *v; /* [tokens][ld], heads side by side */
+    int64_t ldq, ldk, ldv;
+    int tokens, heads, kv_heads, head_dim;
+    const float *q_weight, *k_weight; /* [head_dim] or NULL */
+    float eps;
+    const float *rope; /* [rope_rows][rope_dim] or NULL */
+    int rope_rows, rope_dim, interleaved;
+    const int32_t *positions; /* device [tokens] or NULL */
+    int dtype;                /* BONSAI_B1_F16 / _BF16 */
+    void *q_out;              /* [tokens][ld_q] */
+    int64_t ld_q;
+    void *k_out, *v_out; /* [tokens][ld_kv]; unused with pages */
+    int64_t ld_kv;
+    const bonsai_b1_kv_pages *pages; /* or NULL */
+    int n_seqs;                      /* with pages */
+    const int32_t *q_start;          /* device [n_seqs + 1] or NULL; with pages */
+    int32_t *bad;                    /* device counter or NULL */
+} bonsai_b1_qkv_args;
+int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
+
+/*
+ * Attention of packed sequences:
+ *   out[i] = sum_j softmax_j(scale q_i k_j) v_j
+ * over the keys that token i sees.  heads = group * kv_heads: query head h
+ * reads key head h / group.  Sequence b's tokens are rows q_start[b] ..
+ * q_start[b + 1] of q and out (NULL: one sequence of all `tokens`); its keys
+ * are rows kv_start[b] .. of k and v (NULL: all kv_tokens), or, with pages,
+ * its places in the cache.  With n tokens and m keys, causal token i sees
+ * keys 0 .. m - n + i, and with window > 0 (causal only) the last `window`
+ * of those; a token that sees none gets zeros.  Masked and absent keys do
+ * not reach the output, whatever they hold.  Rows of no sequence are left as
+ * they were.
+ * Scores and sums are fp32; softmax weights are rounded to the inputs' type
+ * for the product with v.  out: rows of heads * head_dim in the inputs' type
+ * (packed = 0), or the packed fp16 activations of the next B1_0 linear
+ * (packed = 1: bonsai_b1_pack_act_f16_ld's layout with row stride ldo, so
+ * that `out` may be a column range of wider activations), as the reference's
+ * ggml_flash_attn_ext feeds its output projections
+ * (src/diffuser_graph.cpp:406-441,509-536).
+ * head_dim 64, 128 or 256; pointers 16-byte aligned; strides in elements,
+ * multiples of 8; scale > 0; out apart from the inputs.
+ * workspace: bonsai_b1_attention_workspace_bytes(args) bytes (16-byte
+ * aligned) for calls whose keys are split over work-groups, or NULL for the
+ * library's per-stream workspace.  Without one (a capture never allocates)
+ * the call runs unsplit: the same values up to the order of fp32 sums,
+ * slower for few rows over many keys.
+ */
+typedef struct bonsai_b1_attention_args {
+    const void *q, *k, *v; /* k, v unused with pages */
+    int64_t q_row, q_head; /* strides of tokens and heads */
+    int64_t k_row, k_head, v_row, v_head;
+    int dtype, heads, kv_heads, head_dim;
+    int tokens, kv_tokens, n_seqs;
+    const int32_t *q_start;  /* device [n_seqs + 1] or NULL */
+    const int32_t *kv_start; /* device [n_seqs + 1] or NULL; unused with pages */
+    const bonsai_b1_kv_pages *pages; /* or NULL */
+    int causal, window;
+    float scale;
+    void *out;
+    int64_t ldo;
+    int packed;
+    int32_t *bad; /* device counter or NULL */
+} bonsai_b1_attention_args;
+size_t bonsai_b1_attention_workspace_bytes(const bonsai_b1_attention_args *args);
+int bonsai_b1_attention(const bonsai_b1_attention_args *args, void *workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
+/*
  * The B1_0 writer on the device; replaces quantize_b1_0 of
  * convert_to_b1_0_packed.py:21-43 and of tests/c_ops/test_b1_linear.cpp:
  * 129-163.  w: fp32 [out_dim][ldw] device weights (ldw >= in_dim,
