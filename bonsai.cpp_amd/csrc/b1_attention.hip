@@ -208,11 +208,23 @@ __device__ __forceinline__ int find_tile(const AttnArgs &a, int group, int t, in
     return -1;
 }
 
+// A range-checked resource over `bytes` from p (at most 2^32 - 1): reads at
+// or past its end give zeros and touch no memory.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_buffer(const uint16_t *p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0,
+                                             (int)(uint32_t)min(bytes, (int64_t)0xffffffffu), kBufferFlags);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 template <bool BF, int D, bool PAGED>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(AttnArgs a) {
     constexpr int ST = D / 16, DT = D / 32, CH = D / 8;
-    __shared__ __align__(1024) uint8_t sm[2][2][kKeys * D * 2];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // two tiles of keys and values, as four objects: the compiler then knows
+    // that the copies into one tile do not concern the reads of the other,
+    // and does not wait for them before these
+    __shared__ __align__(1024) uint8_t k0[kKeys * D * 2], k1[kKeys * D * 2], v0[kKeys * D * 2], v1[kKeys * D * 2];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int l31 = lane & 31, h = lane >> 5;
     const int group = a.heads / a.kv_heads;
     if (a.bad && blockIdx.x == 0 && wave == 0) report_seqs(a.seqs, a.bad);
@@ -223,16 +235,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
     item /= a.splits;
     const int kvh = item % a.kv_heads;
     int t;
-    const int b = __builtin_amdgcn_readfirstlane(find_tile(a, group, item / a.kv_heads, t));
+    const int b = uniform(find_tile(a, group, item / a.kv_heads, t));
     if (b < 0) return;
-    const Seq s = seq_of(a.seqs, b);
+    Seq s = seq_of(a.seqs, b);
+    s.q0 = uniform(s.q0), s.nq = uniform(s.nq), s.kv0 = uniform(s.kv0), s.nk = uniform(s.nk);
     // the last tiles of a causal sequence have the most keys: first
-    t = (s.nq * group + kRows - 1) / kRows - 1 - t;
+    t = uniform((s.nq * group + kRows - 1) / kRows - 1 - t);
     const TileKeys tk = tile_keys(a, s, group, t);
     const int per = tiles_a_range(tk, a.splits);
-    const int ranges = max(1, (tk.t1 - tk.t0 + per - 1) / per);
+    const int ranges = uniform(max(1, (tk.t1 - tk.t0 + per - 1) / per));
     if (split >= ranges) return;
-    const int t0 = tk.t0 + split * per, t1 = min(t0 + per, tk.t1);
+    const int t0 = uniform(tk.t0 + split * per), t1 = uniform(min(t0 + per, tk.t1));
 
     // this lane's row; rows past the tile's last repeat it and store nothing
     const int r = tk.r0 + min(wave * 32 + l31, tk.rows - 1);
@@ -245,24 +258,53 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
     int first_lo, first_hi, last_lo, last_hi;
     visible(a, s, (tk.r0 + min(wave * 32, tk.rows - 1)) / group, first_lo, first_hi);
     visible(a, s, (tk.r0 + min(wave * 32 + 31, tk.rows - 1)) / group, last_lo, last_hi);
+    first_lo = uniform(first_lo), first_hi = uniform(first_hi), last_lo = uniform(last_lo), last_hi = uniform(last_hi);
 
     const uint16_t *qrow = a.q + token * a.q_row + head * a.q_head;
     const KeyRows kr = key_rows<PAGED>(a.k, a.k_page, a.k_row, a.k_head, kvh, s);
     const KeyRows vr = key_rows<PAGED>(a.v, a.v_page, a.v_row, a.v_head, kvh, s);
     bool bad = s.bad;
 
-    // a wave's instruction copies 512 / D rows; lane i lands at 16 i, so the
-    // swizzle is in which chunk of the row it reads
-    auto load = [&](int kb, int buf) {
+    // Copies a tile of keys and values.  A wave's instruction copies the
+    // 512 / D rows that lie in 1 KiB; lane i lands at 16 i, so the swizzle is
+    // in which chunk of the row it reads.  Rows past the last key read zeros.
+    // Paged: `page` is the page of key kb + lane, and rows of more than one
+    // page (of fewer than 512 / D keys) take an instruction a page.
+    constexpr int NR = 512 / D;
+    auto load = [&](int kb, int page, uint8_t *ks, uint8_t *vs) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-            const int at = wave * (D / 32) + i;
-            const int row = at * (512 / D) + lane / CH;
-            const int j = min(kb + row, s.nk - 1);
-            const int chunk = (lane % CH) ^ swizzle<D>(row);
-            dma_lds16(kr.base + key_at<PAGED>(a, kr, b, j, bad) + chunk * 8, sm[buf][0] + at * 1024);
-            dma_lds16(vr.base + key_at<PAGED>(a, vr, b, j, bad) + chunk * 8, sm[buf][1] + at * 1024);
+            const int at = wave * (D / 32) + i, row0 = at * NR;
+            const int row = row0 + lane / CH;
+            const int chunk = ((lane % CH) ^ swizzle<D>(row)) * 16;
+            if constexpr (PAGED) {
+                const int size = 1 << a.seqs.page_shift, span = min(size, NR);
+                for (int sub = 0; sub < NR; sub += span) {
+                    const int id = __builtin_amdgcn_readlane(page, row0 + sub);
+                    const int first = (kb + row0 + sub) & -size;         // the page's first key
+                    const int64_t keys = max(0, min(size, s.nk - first)); // keys there
+                    const uint32_t off = (uint32_t)((kb + row) & (size - 1));
+                    if (NR == span || (unsigned)(lane / CH - sub) < (unsigned)span) {
+                        dma_buf_lds16(key_buffer(kr.base + id * kr.page, keys * kr.row * 2), ks + at * 1024,
+                                      off * (uint32_t)(kr.row * 2) + chunk);
+                        dma_buf_lds16(key_buffer(vr.base + id * vr.page, keys * vr.row * 2), vs + at * 1024,
+                                      off * (uint32_t)(vr.row * 2) + chunk);
+                    }
+                }
+            } else {
+                const int64_t keys = s.nk - kb;
+                dma_buf_lds16(key_buffer(kr.base + kb * kr.row, keys * kr.row * 2), ks + at * 1024,
+                              (uint32_t)row * (uint32_t)(kr.row * 2) + chunk);
+                dma_buf_lds16(key_buffer(vr.base + kb * vr.row, keys * vr.row * 2), vs + at * 1024,
+                              (uint32_t)row * (uint32_t)(vr.row * 2) + chunk);
+            }
         }
+    };
+    auto pages = [&](int kb) {
+        if constexpr (PAGED)
+            return page_of(a.seqs, b, min(kb + lane, s.nk - 1), bad);
+        else
+            return 0;
     };
 
     u32x4 qf[ST];
@@ -274,14 +316,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
     float m = kLowest, l = 0.f;
     const float scale2 = a.scale * 1.44269504f; // exp(x) = exp2(x log2 e)
 
-    if (t0 < t1) load(t0 * kKeys, 0);
-    for (int tt = t0; tt < t1; ++tt) {
-        const int kb = tt * kKeys, buf = (tt - t0) & 1;
+    int next = 0; // pages of the tile after the one that is being copied
+    if (t0 < t1) {
+        load(t0 * kKeys, pages(t0 * kKeys), k0, v0);
+        next = pages((t0 + 1) * kKeys);
+    }
+    auto tile = [&](int tt, const uint8_t *ks, const uint8_t *vs, uint8_t *ks2, uint8_t *vs2) {
+        const int kb = tt * kKeys;
         wait_vmcnt<0>();
+        wait_lgkmcnt0();
         lds_barrier();
-        if (tt + 1 < t1) load(kb + kKeys, buf ^ 1);
-        if (!wave_on || kb > last_hi || kb + kKeys - 1 < first_lo) continue;
-        const uint8_t *ks = sm[buf][0], *vs = sm[buf][1];
+        if (tt + 1 < t1) {
+            load(kb + kKeys, next, ks2, vs2);
+            next = pages(kb + 2 * kKeys);
+        }
+        if (!wave_on || kb > last_hi || kb + kKeys - 1 < first_lo) return;
         // scores, transposed: column = row of q, register i of half h = key
         // 8 (i / 4) + 4 h + i % 4
         floatx16 sc[2];
@@ -312,7 +361,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
         mx = halves_max(mx) * scale2;
-        if (__any(mx > m)) {
+        // the maximum is only moved when some row's grew by 2^8: until then
+        // its weights are up to 256, which fp16 and the fp32 sums hold
+        if (__any(mx > m + 8.f)) {
             const float mn = fmaxf(m, mx);
             const float alpha = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
@@ -347,6 +398,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
                     o[dt] = mfma32<BF>(u32x4{x[0], x[1], y[0], y[1]}, pf, o[dt]);
                 }
             }
+    };
+    for (int tt = t0; tt < t1; tt += 2) {
+        tile(tt, k0, v0, k1, v1);
+        if (tt + 1 < t1) tile(tt + 1, k1, v1, k0, v0);
     }
     l = halves_sum(l);
 
@@ -390,8 +445,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
                 *reinterpret_cast<floatx4 *>(po + 32 * i + 8 * g + 4 * h) =
                     floatx4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
         if (h == 0) *reinterpret_cast<float2v *>(a.part_ml + 2 * at) = float2v{m, l};
+        if (h == 0 && split == 0) a.part_n[token * a.heads + head] = ranges;
         return;
     }
+    if (a.splits > 1 && h == 0) a.part_n[token * a.heads + head] = 1;
     uint16_t *orow = a.out + token * a.ldo + head * D;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
@@ -675,8 +732,10 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
                     *reinterpret_cast<floatx4 *>(a.part_o + at * D + c0 + e) =
                         floatx4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
                 if (c0 == 0) *reinterpret_cast<float2v *>(a.part_ml + 2 * at) = float2v{M, L};
+                if (c0 == 0 && range == 0) a.part_n[token * a.heads + head] = plan.ranges;
             }
         } else {
+            if (a.splits > 1 && mine && c0 == 0) a.part_n[token * a.heads + head] = 1;
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] *= inv;
             store_row<BF, D>(a, token, head, c0, acc, mine);
@@ -687,60 +746,71 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
 
 // ---- joining the ranges -----------------------------------------------------
 
-// 16 lanes a row; rows whose keys were not split are there already.
-template <bool BF, int D, bool FEW>
+// P groups of 16 lanes take a row, each every P-th of its ranges; rows whose
+// keys were not split are there already.  Bound by latency: a row's sequence
+// and number of ranges are one read deep, the maxima and sums of all ranges
+// are read at once by the 16 lanes.
+template <bool BF, int D, int P>
 __global__ __launch_bounds__(256) void b1_attn_join_kernel(AttnArgs a) {
-    constexpr int E = D / 16;
-    const int group = a.heads / a.kv_heads;
+    constexpr int E = D / 16, ROWS = 16 / P; // rows a work-group
+    __shared__ __align__(16) float so[16][D + 4];
     const int all = a.seqs.tokens * a.heads;
-    const int unit = FEW ? few_unit(a) : 0;
-    // a wave's rows are 4 heads in a row; each row's sequence by the whole wave
-    const int wave_row = blockIdx.x * 16 + (threadIdx.x >> 6) * 4;
-    int token = 0, ranges = 0;
-    for (int k = 0; k < 4; ++k) {
-        const int row = wave_row + k;
-        if (row >= all) break;
-        const int tk = row / a.heads;
-        const int b = seq_of_token(a.seqs, tk);
-        int n = 0;
-        if (b >= 0) {
-            const Seq s = seq_of(a.seqs, b);
-            if (FEW) {
-                n = few_plan(a, s, unit).ranges;
-            } else {
-                const TileKeys keys = tile_keys(a, s, group, ((tk - s.q0) * group + row % a.heads % group) / kRows);
-                const int per = tiles_a_range(keys, a.splits);
-                n = (keys.t1 - keys.t0 + per - 1) / per;
-            }
+    const int lane16 = threadIdx.x & 15, at16 = threadIdx.x >> 4;
+    const int row = blockIdx.x * ROWS + at16 / P, part = at16 % P, c0 = lane16 * E;
+    int ranges = row < all ? a.part_n[row] : 0; // of a row of no sequence: anything
+    // the sequences of the wave's rows, each by the whole wave
+    const int wave_row = uniform(row);
+    int last = -1, there = 0, mask = 0;
+#pragma unroll
+    for (int k = 0; k < (P < 4 ? 4 / P : 1); ++k) {
+        const int tk = (wave_row + k) / a.heads;
+        if (wave_row + k < all && tk != last) {
+            there = seq_of_token(a.seqs, tk) >= 0;
+            last = tk;
         }
-        if (((threadIdx.x >> 4) & 3) == k) token = tk, ranges = n;
+        mask |= there << k;
     }
-    const int row = wave_row + ((threadIdx.x >> 4) & 3), c0 = (threadIdx.x & 15) * E;
-    const bool mine = row < all && ranges > 1;
-    float o[E];
+    const bool mine = row < all && (mask >> (row - wave_row) & 1) && ranges > 1 && ranges <= a.splits;
+    if (!mine) ranges = 0;
     float M = kLowest, L = 0.f;
+    for (int i = lane16; i < ranges; i += 16) M = fmaxf(M, a.part_ml[2 * ((int64_t)i * all + row)]);
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
+    for (int i = lane16; i < ranges; i += 16) {
+        const float2v ml = *reinterpret_cast<const float2v *>(a.part_ml + 2 * ((int64_t)i * all + row));
+        L += __builtin_amdgcn_exp2f(ml[0] - M) * ml[1];
+    }
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) L += __shfl_xor(L, x);
+    // weights that add up to at most 1 before they meet a sum of values
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
-    if (mine) {
-        for (int i = 0; i < ranges; ++i) M = fmaxf(M, a.part_ml[2 * ((int64_t)i * all + row)]);
-        for (int i = 0; i < ranges; ++i) {
-            const float2v ml = *reinterpret_cast<const float2v *>(a.part_ml + 2 * ((int64_t)i * all + row));
-            L += __builtin_amdgcn_exp2f(ml[0] - M) * ml[1];
-        }
-        // weights that add up to at most 1 before they meet a sum of values
-        const float inv = L == 0.f ? 0.f : 1.0f / L;
-        for (int i = 0; i < ranges; ++i) {
-            const int64_t at = (int64_t)i * all + row;
-            const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - M) * inv;
+#pragma unroll 4
+    for (int i = part; i < ranges; i += P) {
+        const int64_t at = (int64_t)i * all + row;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - M) * inv;
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                const floatx4 v = *reinterpret_cast<const floatx4 *>(a.part_o + at * D + c0 + e);
+        for (int e = 0; e < E; e += 4) {
+            const floatx4 v = *reinterpret_cast<const floatx4 *>(a.part_o + at * D + c0 + e);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[e + k] += f * v[k];
-            }
+            for (int k = 0; k < 4; ++k) o[e + k] += f * v[k];
         }
     }
-    store_row<BF, D>(a, token, row % a.heads, c0, o, mine);
+    if constexpr (P > 1) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<floatx4 *>(&so[at16][c0 + e]) = floatx4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        __syncthreads();
+        if (part == 0) {
+#pragma unroll
+            for (int k = 1; k < P; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += so[at16 + k][c0 + e];
+        }
+    }
+    store_row<BF, D>(a, row / a.heads, row % a.heads, c0, o, mine && part == 0);
 }
 
 // ---- which kernel, how many ranges -------------------------------------------
@@ -798,7 +868,7 @@ size_t round_256(size_t b) { return (b + 255) & ~(size_t)255; }
 size_t part_bytes(const AttnArgs &a, int splits) {
     if (splits <= 1) return 0;
     const size_t rows = (size_t)splits * a.seqs.tokens * a.heads;
-    return round_256(rows * a.head_dim * 4) + rows * 8;
+    return round_256(rows * a.head_dim * 4) + round_256(rows * 8) + (size_t)a.seqs.tokens * a.heads * 4;
 }
 
 template <bool BF, int D>
@@ -818,11 +888,13 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
     if (p.splits > 1) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        const dim3 join(ceil_div((int64_t)a.seqs.tokens * a.heads, 16));
-        if (p.few)
-            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, true>), join, block, 0, s, a);
+        const int64_t rows = (int64_t)a.seqs.tokens * a.heads;
+        if (p.splits <= 4)
+            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 1>), dim3(ceil_div(rows, 16)), block, 0, s, a);
+        else if (p.splits <= 16)
+            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 4>), dim3(ceil_div(rows, 4)), block, 0, s, a);
         else
-            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, false>), join, block, 0, s, a);
+            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 16>), dim3(rows), block, 0, s, a);
     }
     return hipGetLastError();
 }
@@ -841,8 +913,10 @@ hipError_t launch_attn(const AttnArgs &args, int num_cus, void *ws, size_t ws_by
     a.target = p.target;
     if (p.splits > 1) {
         a.part_o = static_cast<float *>(ws);
-        a.part_ml = reinterpret_cast<float *>(
-            static_cast<uint8_t *>(ws) + round_256((size_t)p.splits * a.seqs.tokens * a.heads * a.head_dim * 4));
+        const size_t rows = (size_t)p.splits * a.seqs.tokens * a.heads;
+        uint8_t *at = static_cast<uint8_t *>(ws) + round_256(rows * a.head_dim * 4);
+        a.part_ml = reinterpret_cast<float *>(at);
+        a.part_n = reinterpret_cast<int32_t *>(at + round_256(rows * 8));
     }
     switch (a.head_dim) {
     case 64: return a.bf16 ? launch<true, 64>(a, p, s) : launch<false, 64>(a, p, s);

@@ -514,6 +514,8 @@ static bool pages_ok(const bonsai_b1_kv_pages *p, int n_seqs, int kv_heads, int 
     if (p->page_stride < head_dim && p->n_pages > 1) return false;
     if (p->max_pages <= 0 || p->ld_pages < p->max_pages || n_seqs <= 0 || !p->pages || !p->kv_len) return false;
     if ((reinterpret_cast<uintptr_t>(p->pages) | reinterpret_cast<uintptr_t>(p->kv_len)) & 3u) return false;
+    // 32-bit offsets within a page
+    if (p->page_size >= (1 << 30) || p->row_stride >= ((int64_t)1 << 30) / p->page_size) return false;
     return (int64_t)p->max_pages * p->page_size < (1 << 30);
 }
 
@@ -617,7 +619,7 @@ static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
         a->k = static_cast<const uint16_t *>(g->pages->k);
         a->v = static_cast<const uint16_t *>(g->pages->v);
         a->k_page = a->v_page = g->pages->page_stride;
-        a->k_row = a->v_row = g->pages->row_stride;
+        a->k_row = a->v_row = g->pages->page_size > 1 ? g->pages->row_stride : g->head_dim;
         a->k_head = a->v_head = g->pages->head_stride;
     } else {
         if (g->kv_tokens < 0 || g->kv_tokens >= (1 << 30) || (!g->kv_start && g->n_seqs > 1))
@@ -627,13 +629,18 @@ static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
                                  !stride_ok(g->k_row) || !stride_ok(g->k_head) || !stride_ok(g->v_row) ||
                                  !stride_ok(g->v_head)))
             return BONSAI_B1_ERR_ARG;
+        // rows apart from one another, 64 of them within 32-bit offsets
+        const int64_t most = 1 << 24;
+        if (g->kv_tokens > 1 && (g->k_row < g->head_dim || g->v_row < g->head_dim || g->k_row > most ||
+                                 g->v_row > most))
+            return BONSAI_B1_ERR_ARG;
         a->seqs.kv_tokens = g->kv_tokens;
         a->seqs.kv_start = g->kv_start;
         a->k = static_cast<const uint16_t *>(g->k);
         a->v = static_cast<const uint16_t *>(g->v);
-        a->k_row = g->k_row;
+        a->k_row = g->kv_tokens > 1 ? g->k_row : g->head_dim;
         a->k_head = g->k_head;
-        a->v_row = g->v_row;
+        a->v_row = g->kv_tokens > 1 ? g->v_row : g->head_dim;
         a->v_head = g->v_head;
     }
     a->q = static_cast<const uint16_t *>(g->q);

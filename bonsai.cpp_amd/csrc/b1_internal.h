@@ -236,6 +236,7 @@ struct AttnArgs {
     int target = 0;  // small kernel: work-groups wanted
     float *part_o = nullptr;   // [splits][tokens * heads][head_dim]
     float *part_ml = nullptr; // [splits][tokens * heads][2]: maximum (base 2), sum
+    int32_t *part_n = nullptr; // [tokens * heads]: the row's ranges
 };
 
 // Workspace bytes of a call, for a device of num_cus (0: none).
