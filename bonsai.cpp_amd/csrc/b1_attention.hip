@@ -11,6 +11,8 @@
 
 #include <limits.h>
 
+#include <algorithm>
+
 #include "b1_seqs.h"
 
 namespace b1 {
@@ -145,26 +147,55 @@ __device__ void row_fp32(const AttnArgs &a, const KeyRows &kr, const KeyRows &vr
     l = l == l ? 1.f : l;
 }
 
+// l + the two values of a pair.
+template <bool BF>
+__device__ __forceinline__ float add_pair(uint32_t p, float l) {
+    if constexpr (BF)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u),
+                                               l, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, p), __builtin_bit_cast(half2v, 0x3c003c00u), l,
+                                      false);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // ---- tiles of 128 rows ------------------------------------------------------
 
-constexpr int kRows = 128, kKeys = 64;
-
-// Swizzle of a row's 16-byte chunks in LDS.  A K fragment reads one chunk
-// column of 32 consecutive rows and a V fragment two neighbouring columns of
-// 4 consecutive rows; without it all rows of D >= 128 (256 bytes, one sweep
-// of the banks) share their banks.
+constexpr int kRows = 128;
+// Keys in LDS at a time (a stage), and waves a SIMD, by head dim.
 template <int D>
-__device__ __forceinline__ int swizzle(int row) {
+struct TileShapeOf {
+    static constexpr int keys = D == 64 ? 64 : 32;
+    static constexpr int waves = D == 256 ? 2 : 3;
+};
+// A range of a split tile has at least this many keys, so that its fixed
+// costs (queries, partial sums out and in) stay small beside them.
+constexpr int kLeastKeys = 256;
+
+// Swizzles of a row's 16-byte chunks in LDS (64 banks of 4 bytes: two rows of
+// D = 64, one of 128 a sweep).  A K fragment reads one chunk column of 16
+// consecutive rows in a sweep; a V fragment a block of four chunks of four
+// consecutive rows.  Each swizzle spreads its own pattern over all banks.
+template <int D>
+__device__ __forceinline__ int swizzle_k(int row) {
     if constexpr (D == 64)
         return ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
     else
         return (row & 7) << 1 | ((row >> 3) & 1);
 }
+template <int D>
+__device__ __forceinline__ int swizzle_v(int row) {
+    if constexpr (D == 64)
+        return ((row >> 1) & 1) << 2;
+    else
+        return (row & 3) << 2;
+}
 
-// The rows of tile t (of kRows) and the range of 64-key tiles they see.
+// The rows of tile t of a sequence and the keys [k0, k1) that they see.
 struct TileKeys {
     int r0, rows; // first row, rows there (<= kRows)
-    int t0, t1;   // key tiles
+    int k0, k1;
 };
 __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, int group, int t) {
     TileKeys k;
@@ -173,83 +204,161 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, i
     int lo, hi, x;
     visible(a, s, k.r0 / group, lo, x);
     visible(a, s, (k.r0 + k.rows - 1) / group, x, hi);
-    k.t0 = lo / kKeys;
-    k.t1 = hi < lo ? k.t0 : hi / kKeys + 1;
+    k.k0 = lo;
+    k.k1 = max(hi + 1, lo);
     return k;
 }
-// Key tiles of each of the ranges a row tile's keys are split into: at least
-// four, so that a range's fixed costs stay small beside its keys.
-__device__ __forceinline__ int tiles_a_range(const TileKeys &k, int splits) {
-    return max(4, (k.t1 - k.t0 + splits - 1) / splits);
-}
+__device__ __forceinline__ int seq_tiles(const Seq &s, int group) { return (s.nq * group + kRows - 1) / kRows; }
 
-// The sequence and row tile of work item t, by the whole wave; b = -1: none.
-__device__ __forceinline__ int find_tile(const AttnArgs &a, int group, int t, int &local) {
+// Into how many ranges a sequence's tiles are split: a fixed number, or so
+// that all ranges of all sequences have about the same number of keys and
+// make about a.target work items.
+__device__ __forceinline__ int seq_last_keys(const AttnArgs &a, const Seq &s, int group) {
+    const int n = seq_tiles(s, group);
+    if (n == 0) return 0;
+    const TileKeys k = tile_keys(a, s, group, n - 1);
+    return k.k1 - k.k0;
+}
+__device__ __forceinline__ int tile_unit(const AttnArgs &a, int group) {
+    if (a.splits == 1 || a.target == 0) return 0;
     const int lane = threadIdx.x & 63;
-    int run = 0;
-    for (int b0 = 0; b0 < a.seqs.n_seqs; b0 += 64) {
-        const int b = b0 + lane;
-        int n = 0;
-        if (b < a.seqs.n_seqs) n = (seq_of(a.seqs, b).nq * group + kRows - 1) / kRows;
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
-        const uint64_t past = __ballot(run + incl > t);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            local = t - run - __shfl(incl - n, l);
-            return b0 + l;
-        }
-        run += __shfl(incl, 63);
+    float total = 0.f; // a range's size needs no more
+    for (int b = lane; b < a.seqs.n_seqs; b += 64) {
+        const Seq s = seq_of(a.seqs, b);
+        total += (float)seq_tiles(s, group) * (float)seq_last_keys(a, s, group);
     }
-    return -1;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
+    return max(kLeastKeys, (int)fminf(total * (float)a.kv_heads / (float)a.target, 1.0e9f) + 1);
+}
+__device__ __forceinline__ int seq_splits(const AttnArgs &a, const Seq &s, int group, int unit) {
+    if (a.splits == 1 || a.target == 0) return a.splits;
+    return max(1, min(a.splits, (seq_last_keys(a, s, group) + unit - 1) / unit));
 }
 
-// A range-checked resource over `bytes` from p (at most 2^32 - 1): reads at
-// or past its end give zeros and touch no memory.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_buffer(const uint16_t *p, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0,
-                                             (int)(uint32_t)min(bytes, (int64_t)0xffffffffu), kBufferFlags);
+// A work item: key head, row tile and range of one of the sequences.  The
+// first a.solo items are whole tiles (of the one sequence of such a call);
+// after them each tile is `splits` items in a row, whose partial sums are at
+// part .. part + splits - 1.
+struct TileItem {
+    int b, kvh, t, range, splits, part;
+};
+// Finds item i (or, of whole tiles, the i-th tile behind the solo ones), by
+// the whole wave; b = -1: none.
+__device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int i, bool whole) {
+    TileItem r;
+    const int lane = threadIdx.x & 63;
+    const int unit = tile_unit(a, group);
+    int j = i, tiles0 = 0, items0 = 0, g;
+    r.b = -1;
+    r.splits = 1;
+    r.range = 0;
+    r.part = 0;
+    if (a.solo > 0) { // one sequence
+        r.b = 0;
+        if (!whole && i < a.solo) {
+            g = i;
+        } else {
+            j = whole ? i : i - a.solo;
+            r.splits = a.splits;
+            g = a.solo + (whole ? j : j / r.splits);
+            r.range = whole ? 0 : j % r.splits;
+            r.part = (g - a.solo) * r.splits;
+        }
+        if (g >= seq_tiles(seq_of(a.seqs, 0), group) * a.kv_heads) r.b = -1;
+    } else {
+        for (int b0 = 0; b0 < a.seqs.n_seqs && r.b < 0; b0 += 64) {
+            int n = 0, c = 1;
+            if (b0 + lane < a.seqs.n_seqs) {
+                const Seq s = seq_of(a.seqs, b0 + lane);
+                n = seq_tiles(s, group) * a.kv_heads;
+                c = seq_splits(a, s, group, unit);
+            }
+            int tiles = n, items = n * c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(tiles, o), y = __shfl_up(items, o);
+                if (lane >= o) tiles += x, items += y;
+            }
+            const uint64_t past = __ballot((whole ? tiles0 + tiles : items0 + items) > i);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                r.b = b0 + l;
+                r.splits = __shfl(c, l);
+                const int at = __shfl(items - n * c, l) + items0;
+                j = i - (whole ? __shfl(tiles - n, l) + tiles0 : at);
+                g = whole ? j : j / r.splits;
+                r.range = whole ? 0 : j % r.splits;
+                r.part = at + g * r.splits;
+            }
+            tiles0 += __shfl(tiles, 63);
+            items0 += __shfl(items, 63);
+        }
+    }
+    if (r.b < 0) return r;
+    r.b = uniform(r.b);
+    r.kvh = uniform(g % a.kv_heads);
+    // the last tiles of a causal sequence have the most keys: first
+    r.t = uniform(seq_tiles(seq_of(a.seqs, r.b), group) - 1 - g / a.kv_heads);
+    r.range = uniform(r.range);
+    r.splits = uniform(r.splits);
+    r.part = uniform(r.part);
+    return r;
+}
+// The stages [t0, t1) of a range, and how many ranges the tile has.
+struct TileRange {
+    int t0, t1, ranges;
+};
+template <int D>
+__device__ __forceinline__ TileRange tile_range(const TileKeys &k, int splits, int range) {
+    constexpr int KK = TileShapeOf<D>::keys;
+    const int first = k.k0 / KK, last = (k.k1 + KK - 1) / KK;
+    const int per = max(kLeastKeys / KK, (last - first + splits - 1) / splits);
+    TileRange r;
+    r.ranges = splits == 1 ? 1 : max(1, (last - first + per - 1) / per);
+    r.t0 = first + range * per;
+    r.t1 = r.ranges == 1 ? last : min(r.t0 + per, last);
+    return r;
 }
 
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// A range-checked resource over `bytes` from p (none where it is negative,
+// as for keys past the last): reads at or past its end give zeros and touch
+// no memory.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_buffer(const uint16_t *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, max(0, bytes), kBufferFlags);
+}
 
+// Bound by the matrix units together with the vector instructions of the
+// softmax (a 32 x 32 block of scores is 8 products of 32 cycles at D = 128,
+// as many for the values, and about 80 vector instructions, 16 of them
+// exponentials), and by how well three independent work-groups a CU hide one
+// another's LDS reads, barriers and copies.
 template <bool BF, int D, bool PAGED>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(AttnArgs a) {
-    constexpr int ST = D / 16, DT = D / 32, CH = D / 8;
-    // two tiles of keys and values, as four objects: the compiler then knows
-    // that the copies into one tile do not concern the reads of the other,
+__global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kernel(AttnArgs a) {
+    constexpr int ST = D / 16, DT = D / 32, CH = D / 8, KK = TileShapeOf<D>::keys, KT = KK / 32;
+    // two stages of keys and values, as four objects: the compiler then knows
+    // that the copies into one stage do not concern the reads of the other,
     // and does not wait for them before these
-    __shared__ __align__(1024) uint8_t k0[kKeys * D * 2], k1[kKeys * D * 2], v0[kKeys * D * 2], v1[kKeys * D * 2];
+    __shared__ __align__(1024) uint8_t k0[KK * D * 2], k1[KK * D * 2], v0[KK * D * 2], v1[KK * D * 2];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int l31 = lane & 31, h = lane >> 5;
     const int group = a.heads / a.kv_heads;
     if (a.bad && blockIdx.x == 0 && wave == 0) report_seqs(a.seqs, a.bad);
 
-    // work item: key head, row tile, key range
-    int item = blockIdx.x;
-    const int split = item % a.splits;
-    item /= a.splits;
-    const int kvh = item % a.kv_heads;
-    int t;
-    const int b = uniform(find_tile(a, group, item / a.kv_heads, t));
+    const TileItem it = find_item(a, group, blockIdx.x, false);
+    const int b = it.b, kvh = it.kvh;
     if (b < 0) return;
     Seq s = seq_of(a.seqs, b);
     s.q0 = uniform(s.q0), s.nq = uniform(s.nq), s.kv0 = uniform(s.kv0), s.nk = uniform(s.nk);
-    // the last tiles of a causal sequence have the most keys: first
-    t = uniform((s.nq * group + kRows - 1) / kRows - 1 - t);
-    const TileKeys tk = tile_keys(a, s, group, t);
-    const int per = tiles_a_range(tk, a.splits);
-    const int ranges = uniform(max(1, (tk.t1 - tk.t0 + per - 1) / per));
-    if (split >= ranges) return;
-    const int t0 = uniform(tk.t0 + split * per), t1 = uniform(min(t0 + per, tk.t1));
+    const TileKeys tk = tile_keys(a, s, group, it.t);
+    const TileRange tr = tile_range<D>(tk, it.splits, it.range);
+    const int ranges = uniform(tr.ranges), t0 = uniform(tr.t0), t1 = uniform(tr.t1);
+    if (it.range >= ranges) return;
 
     // this lane's row; rows past the tile's last repeat it and store nothing
-    const int r = tk.r0 + min(wave * 32 + l31, tk.rows - 1);
-    const bool mine = wave * 32 + l31 < tk.rows;
+    const int wrow = wave * 32 + l31;
+    const int r = tk.r0 + min(wrow, tk.rows - 1);
+    const bool mine = wrow < tk.rows;
     const int token = s.q0 + r / group, head = kvh * group + r % group;
     int lo, hi;
     visible(a, s, r / group, lo, hi);
@@ -265,42 +374,39 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
     const KeyRows vr = key_rows<PAGED>(a.v, a.v_page, a.v_row, a.v_head, kvh, s);
     bool bad = s.bad;
 
-    // Copies a tile of keys and values.  A wave's instruction copies the
-    // 512 / D rows that lie in 1 KiB; lane i lands at 16 i, so the swizzle is
-    // in which chunk of the row it reads.  Rows past the last key read zeros.
-    // Paged: `page` is the page of key kb + lane, and rows of more than one
-    // page (of fewer than 512 / D keys) take an instruction a page.
-    constexpr int NR = 512 / D;
-    auto load = [&](int kb, int page, uint8_t *ks, uint8_t *vs) {
+    // Copies a stage.  A wave's instruction copies the NR rows that lie in 1
+    // KiB; lane i lands at 16 i, so the swizzle is in which chunk of the row
+    // it reads.  Rows past the last key read zeros.  Paged: `page` is the
+    // page of key kb + lane, keys and values lie alike, and rows of more than
+    // one page (of fewer than NR keys) take an instruction a page.
+    constexpr int NR = 512 / D, NI = KK * D / 2048;
+    auto load = [&](int kb, int page, uint8_t *ks, uint8_t *vs) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int at = wave * (D / 32) + i, row0 = at * NR;
+        for (int i = 0; i < NI; ++i) {
+            const int at = wave * NI + i, row0 = at * NR;
             const int row = row0 + lane / CH;
-            const int chunk = ((lane % CH) ^ swizzle<D>(row)) * 16;
+            const int ck = ((lane % CH) ^ swizzle_k<D>(row)) * 16, cv = ((lane % CH) ^ swizzle_v<D>(row)) * 16;
             if constexpr (PAGED) {
                 const int size = 1 << a.seqs.page_shift, span = min(size, NR);
+                const int bytes = (int)kr.row * 2;
+                const uint32_t off = (uint32_t)((kb + row) & (size - 1)) * (uint32_t)bytes;
                 for (int sub = 0; sub < NR; sub += span) {
-                    const int id = __builtin_amdgcn_readlane(page, row0 + sub);
-                    const int first = (kb + row0 + sub) & -size;         // the page's first key
-                    const int64_t keys = max(0, min(size, s.nk - first)); // keys there
-                    const uint32_t off = (uint32_t)((kb + row) & (size - 1));
+                    const int64_t at_page = __builtin_amdgcn_readlane(page, row0 + sub) * kr.page;
+                    // keys of the page up to the sequence's last
+                    const int keys = min(size, s.nk - ((kb + row0 + sub) & -size));
                     if (NR == span || (unsigned)(lane / CH - sub) < (unsigned)span) {
-                        dma_buf_lds16(key_buffer(kr.base + id * kr.page, keys * kr.row * 2), ks + at * 1024,
-                                      off * (uint32_t)(kr.row * 2) + chunk);
-                        dma_buf_lds16(key_buffer(vr.base + id * vr.page, keys * vr.row * 2), vs + at * 1024,
-                                      off * (uint32_t)(vr.row * 2) + chunk);
+                        dma_buf_lds16(key_buffer(kr.base + at_page, keys * bytes), ks + at * 1024, off + ck);
+                        dma_buf_lds16(key_buffer(vr.base + at_page, keys * bytes), vs + at * 1024, off + cv);
                     }
                 }
             } else {
-                const int64_t keys = s.nk - kb;
-                dma_buf_lds16(key_buffer(kr.base + kb * kr.row, keys * kr.row * 2), ks + at * 1024,
-                              (uint32_t)row * (uint32_t)(kr.row * 2) + chunk);
-                dma_buf_lds16(key_buffer(vr.base + kb * vr.row, keys * vr.row * 2), vs + at * 1024,
-                              (uint32_t)row * (uint32_t)(vr.row * 2) + chunk);
+                const int keys = min(KK, s.nk - kb), kbytes = (int)kr.row * 2, vbytes = (int)vr.row * 2;
+                dma_buf_lds16(key_buffer(kr.base + kb * kr.row, keys * kbytes), ks + at * 1024, row * kbytes + ck);
+                dma_buf_lds16(key_buffer(vr.base + kb * vr.row, keys * vbytes), vs + at * 1024, row * vbytes + cv);
             }
         }
     };
-    auto pages = [&](int kb) {
+    auto pages = [&](int kb) __attribute__((always_inline)) {
         if constexpr (PAGED)
             return page_of(a.seqs, b, min(kb + lane, s.nk - 1), bad);
         else
@@ -316,39 +422,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
     float m = kLowest, l = 0.f;
     const float scale2 = a.scale * 1.44269504f; // exp(x) = exp2(x log2 e)
 
-    int next = 0; // pages of the tile after the one that is being copied
+    int next = 0; // pages of the stage after the one that is being copied
     if (t0 < t1) {
-        load(t0 * kKeys, pages(t0 * kKeys), k0, v0);
-        next = pages((t0 + 1) * kKeys);
+        load(t0 * KK, pages(t0 * KK), k0, v0);
+        next = pages((t0 + 1) * KK);
     }
-    auto tile = [&](int tt, const uint8_t *ks, const uint8_t *vs, uint8_t *ks2, uint8_t *vs2) {
-        const int kb = tt * kKeys;
+    auto stage = [&](int tt, const uint8_t *ks, const uint8_t *vs, uint8_t *ks2, uint8_t *vs2)
+                     __attribute__((always_inline)) {
+        const int kb = tt * KK;
+        // every wave's copies of this stage are there, and its reads of the
+        // last one done
         wait_vmcnt<0>();
         wait_lgkmcnt0();
         lds_barrier();
         if (tt + 1 < t1) {
-            load(kb + kKeys, next, ks2, vs2);
-            next = pages(kb + 2 * kKeys);
+            load(kb + KK, next, ks2, vs2);
+            next = pages(kb + 2 * KK);
         }
-        if (!wave_on || kb > last_hi || kb + kKeys - 1 < first_lo) return;
+        if (!wave_on || kb > last_hi || kb + KK - 1 < first_lo) return;
         // scores, transposed: column = row of q, register i of half h = key
         // 8 (i / 4) + 4 h + i % 4
-        floatx16 sc[2];
+        floatx16 sc[KT];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < KT; ++kt) {
             sc[kt] = floatx16{};
             const int row = kt * 32 + l31;
 #pragma unroll
             for (int i = 0; i < ST; ++i) {
                 const u32x4 kf = *reinterpret_cast<const u32x4 *>(ks + row * (D * 2) +
-                                                                  (((2 * i + h) ^ swizzle<D>(row)) << 4));
+                                                                  (((2 * i + h) ^ swizzle_k<D>(row)) << 4));
                 sc[kt] = mfma32<BF>(kf, qf[i], sc[kt]);
             }
         }
-        if (kb + kKeys - 1 > first_hi || kb < last_lo) {
+        if (kb + KK - 1 > first_hi || kb < last_lo) {
             const int top = hi - kb - 4 * h, bot = lo - kb - 4 * h;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int c = 32 * kt + 8 * (i / 4) + i % 4;
@@ -357,7 +466,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
         }
         float mx = -kInf;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kt][i]);
         mx = halves_max(mx) * scale2;
@@ -371,37 +480,33 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
+        // weights, rounded to the inputs' type for the product and summed as
+        // rounded; o (transposed) += v (transposed) p, 16 keys a product, in
+        // the order the scores' registers hold them
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int x = 0; x < 2 * KT; ++x) {
+            u32x4 pf;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[kt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kt][i], scale2, -m));
-                l += sc[kt][i];
+            for (int e = 0; e < 4; ++e) {
+                const int i = 8 * (x & 1) + 2 * e;
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x / 2][i], scale2, -m));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x / 2][i + 1], scale2, -m));
+                pf[e] = pack_16<BF>(p0, p1);
+                l = add_pair<BF>(pf[e], l);
             }
-        // o (transposed) += v (transposed) p: 16 keys a step, in the order
-        // the scores' registers hold them
+            const int row = 16 * x + 4 * h + (lane & 15) / 4;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                u32x4 pf;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pf[e] = pack_16<BF>(sc[kt][8 * u + 2 * e], sc[kt][8 * u + 2 * e + 1]);
-                const int row = kt * 32 + 16 * u + 4 * h + (lane & 15) / 4;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-                    auto at = [&](int rw) {
-                        return vs + rw * (D * 2) + ((chunk ^ swizzle<D>(rw)) << 4) + (lane & 1) * 8;
-                    };
-                    const u32x2 x = read_columns(at(row)), y = read_columns(at(row + 8));
-                    o[dt] = mfma32<BF>(u32x4{x[0], x[1], y[0], y[1]}, pf, o[dt]);
-                }
+            for (int dt = 0; dt < DT; ++dt) {
+                const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+                const uint8_t *at = vs + row * (D * 2) + ((chunk ^ swizzle_v<D>(row)) << 4) + (lane & 1) * 8;
+                const u32x2 y = read_columns(at), z = read_columns(at + 8 * (D * 2));
+                o[dt] = mfma32<BF>(u32x4{y[0], y[1], z[0], z[1]}, pf, o[dt]);
             }
+        }
     };
     for (int tt = t0; tt < t1; tt += 2) {
-        tile(tt, k0, v0, k1, v1);
-        if (tt + 1 < t1) tile(tt + 1, k1, v1, k0, v0);
+        stage(tt, k0, v0, k1, v1);
+        if (tt + 1 < t1) stage(tt + 1, k1, v1, k0, v0);
     }
     l = halves_sum(l);
 
@@ -410,65 +515,62 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void b1_attn_tile_kernel(Att
         if (a.bad && threadIdx.x == 0) atomicAdd(a.bad, 1);
     }
     if (!wave_on) return;
+    if (bad) l = __builtin_nanf("");
     float inv = l == 0.f ? 0.f : 1.0f / l;
-    if (bad) {
-        inv = l = __builtin_nanf("");
-    } else {
-        int odd = 0;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) odd |= !finite(o[i][e] * inv);
-        odd |= __shfl_xor(odd, 32);
-        if (odd) {
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] = floatx16{};
-            row_fp32<BF, D, PAGED>(a, kr, vr, b, qrow, max(lo, t0 * kKeys), min(hi + 1, t1 * kKeys), scale2, m, l,
-                                   [&](const uint16_t *v, float p) {
-#pragma unroll
-                                       for (int i = 0; i < DT; ++i)
-#pragma unroll
-                                           for (int e = 0; e < 16; ++e)
-                                               o[i][e] += p * to_f32<BF>(v[32 * i + 8 * (e / 4) + 4 * h + e % 4]);
-                                   });
-            inv = l == 0.f ? 0.f : 1.0f / l;
-        }
-    }
-    if (!mine) return;
-    if (ranges > 1) {
-        const int64_t at = ((int64_t)split * a.seqs.tokens + token) * a.heads + head;
-        float *po = a.part_o + at * D;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
+    // columns 32 i .. of the row: register e of half h = column 8 (e / 4) +
+    // 4 h + e % 4
+    const int64_t part = (int64_t)(it.part + it.range) * kRows + wrow;
+    auto store = [&](int i, floatx16 v) __attribute__((always_inline)) {
+        if (!mine) return;
+        if (ranges > 1) {
+            float *po = a.part_o + part * D + 32 * i + 4 * h;
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<floatx4 *>(po + 32 * i + 8 * g + 4 * h) =
-                    floatx4{o[i][4 * g], o[i][4 * g + 1], o[i][4 * g + 2], o[i][4 * g + 3]};
-        if (h == 0) *reinterpret_cast<float2v *>(a.part_ml + 2 * at) = float2v{m, l};
-        if (h == 0 && split == 0) a.part_n[token * a.heads + head] = ranges;
-        return;
-    }
-    if (a.splits > 1 && h == 0) a.part_n[token * a.heads + head] = 1;
-    uint16_t *orow = a.out + token * a.ldo + head * D;
-#pragma unroll
-    for (int i = 0; i < DT; ++i) {
-        o[i] *= inv;
+                *reinterpret_cast<floatx4 *>(po + 8 * g) = floatx4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+            return;
+        }
+        v *= inv;
+        uint16_t *orow = a.out + token * a.ldo + head * D + 32 * i;
         if (a.packed) {
             // words d .. d + 3 of the block: columns d and d + 16
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 u32x4 w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = pack_f16(o[i][4 * g + e], o[i][4 * g + e + 8]);
-                *reinterpret_cast<u32x4 *>(orow + 32 * i + 16 * g + 8 * h) = w;
+                for (int e = 0; e < 4; ++e) w[e] = pack_f16(v[4 * g + e], v[4 * g + e + 8]);
+                *reinterpret_cast<u32x4 *>(orow + 16 * g + 8 * h) = w;
             }
         } else {
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<u32x2 *>(orow + 32 * i + 8 * g + 4 * h) =
-                    u32x2{pack_16<BF>(o[i][4 * g], o[i][4 * g + 1]), pack_16<BF>(o[i][4 * g + 2], o[i][4 * g + 3])};
+                *reinterpret_cast<u32x2 *>(orow + 8 * g + 4 * h) =
+                    u32x2{pack_16<BF>(v[4 * g], v[4 * g + 1]), pack_16<BF>(v[4 * g + 2], v[4 * g + 3])};
         }
+    };
+    int odd = 0;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) odd |= !finite(o[i][e] * inv);
+    odd |= __shfl_xor(odd, 32);
+    if (odd && !bad) {
+#pragma unroll 1
+        for (int i = 0; i < DT; ++i) {
+            floatx16 v = {};
+            row_fp32<BF, D, PAGED>(a, kr, vr, b, qrow, max(lo, t0 * KK), min(hi + 1, t1 * KK), scale2, m, l,
+                                   [&](const uint16_t *x, float p) {
+#pragma unroll
+                                       for (int e = 0; e < 16; ++e)
+                                           v[e] += p * to_f32<BF>(x[32 * i + 8 * (e / 4) + 4 * h + e % 4]);
+                                   });
+            inv = l == 0.f ? 0.f : 1.0f / l;
+            store(i, v);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) store(i, o[i]);
     }
+    if (ranges > 1 && mine && h == 0) *reinterpret_cast<float2v *>(a.part_ml + 2 * part) = float2v{m, l};
 }
 
 // ---- few rows a sequence ----------------------------------------------------
@@ -658,8 +760,14 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
                     sc[kt][i] = __builtin_amdgcn_exp2f(sc[kt][i] - m);
                     l += sc[kt][i];
                 }
-            const u32x4 pf = {pack_16<BF>(sc[0][0], sc[0][1]), pack_16<BF>(sc[0][2], sc[0][3]),
-                              pack_16<BF>(sc[1][0], sc[1][1]), pack_16<BF>(sc[1][2], sc[1][3])};
+            u32x4 pf, pr;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float p0 = sc[k / 2][2 * (k & 1)], p1 = sc[k / 2][2 * (k & 1) + 1];
+                pf[k] = pack_16<BF>(p0, p1);
+                if (BF) // what the rounding to 8 bits left
+                    pr[k] = pack_16<BF>(p0 - to_f32<BF>((uint16_t)pf[k]), p1 - to_f32<BF>((uint16_t)(pf[k] >> 16)));
+            }
             // matrix row c of product e is column E c + e
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -668,6 +776,7 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) vf[k] = __builtin_amdgcn_perm(vw[2 * k + 1][e / 2], vw[2 * k][e / 2], sel);
                 o[e] = mfma16<BF>(vf, pf, o[e]);
+                if (BF) o[e] = mfma16<BF>(vf, pr, o[e]);
             }
         }
         l += __shfl_xor(l, 16);
@@ -746,17 +855,72 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
 
 // ---- joining the ranges -----------------------------------------------------
 
-// P groups of 16 lanes take a row, each every P-th of its ranges; rows whose
-// keys were not split are there already.  Bound by latency: a row's sequence
-// and number of ranges are one read deep, the maxima and sums of all ranges
-// are read at once by the 16 lanes.
+// The joined sums of a row's ranges, by 16 lanes with E columns each: from
+// `first` on every `step`-th of `ranges`, partial sums `apart` rows apart,
+// with the weights of all ranges.
+template <int E>
+__device__ __forceinline__ void join_ranges(const float *part_o, const float *part_ml, int64_t row, int64_t apart,
+                                            int ranges, int first, int step, int c0, float (&o)[E]) {
+    const int lane16 = threadIdx.x & 15;
+    float M = kLowest, L = 0.f;
+    for (int i = lane16; i < ranges; i += 16) M = fmaxf(M, part_ml[2 * (row + i * apart)]);
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
+    for (int i = lane16; i < ranges; i += 16) {
+        const float2v ml = *reinterpret_cast<const float2v *>(part_ml + 2 * (row + i * apart));
+        L += __builtin_amdgcn_exp2f(ml[0] - M) * ml[1];
+    }
+#pragma unroll
+    for (int x = 8; x >= 1; x >>= 1) L += __shfl_xor(L, x);
+    // weights that add up to at most 1 before they meet a sum of values
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int i = first; i < ranges; i += step) {
+        const int64_t at = row + i * apart;
+        const float f = __builtin_amdgcn_exp2f(part_ml[2 * at] - M) * inv;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const floatx4 v = *reinterpret_cast<const floatx4 *>(part_o + at * (16 * E) + c0 + e);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[e + k] += f * v[k];
+        }
+    }
+}
+
+// Rows of split tiles: a work-group takes 16 rows of one.
+template <bool BF, int D>
+__global__ __launch_bounds__(256) void b1_attn_tile_join_kernel(AttnArgs a) {
+    constexpr int E = D / 16;
+    const int group = a.heads / a.kv_heads;
+    const TileItem it = find_item(a, group, blockIdx.x / (kRows / 16), true);
+    if (it.b < 0) return;
+    const Seq s = seq_of(a.seqs, it.b);
+    const TileKeys tk = tile_keys(a, s, group, it.t);
+    const int ranges = tile_range<D>(tk, it.splits, 0).ranges;
+    const int row = blockIdx.x % (kRows / 16) * 16 + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * E;
+    // (whole work-groups; part sums past the launched items: of sequences
+    // that overlap, which no plan counts)
+    if (ranges <= 1 || row - (int)(threadIdx.x >> 4) >= tk.rows || it.part + ranges > a.items) return;
+    const bool mine = row < tk.rows;
+    const int r = tk.r0 + min(row, tk.rows - 1);
+    float o[E];
+    join_ranges<E>(a.part_o, a.part_ml, (int64_t)it.part * kRows + min(row, tk.rows - 1), kRows, ranges, 0, 1, c0, o);
+    store_row<BF, D>(a, s.q0 + r / group, it.kvh * group + r % group, c0, o, mine);
+}
+
+// Rows of the few-rows kernel: P groups of 16 lanes take a row, each every
+// P-th of its ranges; rows whose keys were not split are there already.
+// Bound by latency: a row's sequence and number of ranges are one read deep,
+// the maxima and sums of all ranges are read at once by the 16 lanes.
 template <bool BF, int D, int P>
-__global__ __launch_bounds__(256) void b1_attn_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void b1_attn_few_join_kernel(AttnArgs a) {
     constexpr int E = D / 16, ROWS = 16 / P; // rows a work-group
     __shared__ __align__(16) float so[16][D + 4];
     const int all = a.seqs.tokens * a.heads;
-    const int lane16 = threadIdx.x & 15, at16 = threadIdx.x >> 4;
-    const int row = blockIdx.x * ROWS + at16 / P, part = at16 % P, c0 = lane16 * E;
+    const int at16 = threadIdx.x >> 4;
+    const int row = blockIdx.x * ROWS + at16 / P, part = at16 % P, c0 = (threadIdx.x & 15) * E;
     int ranges = row < all ? a.part_n[row] : 0; // of a row of no sequence: anything
     // the sequences of the wave's rows, each by the whole wave
     const int wave_row = uniform(row);
@@ -771,33 +935,8 @@ __global__ __launch_bounds__(256) void b1_attn_join_kernel(AttnArgs a) {
         mask |= there << k;
     }
     const bool mine = row < all && (mask >> (row - wave_row) & 1) && ranges > 1 && ranges <= a.splits;
-    if (!mine) ranges = 0;
-    float M = kLowest, L = 0.f;
-    for (int i = lane16; i < ranges; i += 16) M = fmaxf(M, a.part_ml[2 * ((int64_t)i * all + row)]);
-#pragma unroll
-    for (int x = 8; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
-    for (int i = lane16; i < ranges; i += 16) {
-        const float2v ml = *reinterpret_cast<const float2v *>(a.part_ml + 2 * ((int64_t)i * all + row));
-        L += __builtin_amdgcn_exp2f(ml[0] - M) * ml[1];
-    }
-#pragma unroll
-    for (int x = 8; x >= 1; x >>= 1) L += __shfl_xor(L, x);
-    // weights that add up to at most 1 before they meet a sum of values
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
     float o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int i = part; i < ranges; i += P) {
-        const int64_t at = (int64_t)i * all + row;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - M) * inv;
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const floatx4 v = *reinterpret_cast<const floatx4 *>(a.part_o + at * D + c0 + e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[e + k] += f * v[k];
-        }
-    }
+    join_ranges<E>(a.part_o, a.part_ml, mine ? row : 0, all, mine ? ranges : 0, part, P, c0, o);
     if constexpr (P > 1) {
 #pragma unroll
         for (int e = 0; e < E; e += 4)
@@ -817,58 +956,70 @@ __global__ __launch_bounds__(256) void b1_attn_join_kernel(AttnArgs a) {
 
 struct AttnPlan {
     bool few;
-    int splits, target, grid;
+    int splits, target, solo;
+    int64_t grid, tiles; // work-groups; tiles that may be split
 };
 
-int ceil_div(int64_t a, int64_t b) {
-    const int64_t v = (a + b - 1) / b;
-    return v > INT_MAX ? INT_MAX : (int)v;
-}
-
+// Calls whose sequences have up to 16 rows a key head on average run the
+// few-rows kernel, which splits their keys into about 4 work-groups a CU.
+// Tiles: fewer of them than fit the device at once are split so that they
+// fill it; of more equal ones (one sequence, every key seen) the part of the
+// last round that would leave most of the device idle.
 AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     AttnPlan p{};
     const int group = a.heads / a.kv_heads;
-    const int n = a.seqs.n_seqs;
+    const int64_t n = a.seqs.n_seqs;
     const int64_t rows = (int64_t)a.seqs.tokens * group; // a key head
     const int64_t most = a.seqs.pages ? (int64_t)a.seqs.max_pages << a.seqs.page_shift : a.seqs.kv_tokens;
-    p.few = rows <= (int64_t)kFewRows * n;
+    p.few = rows <= kFewRows * n;
+    p.splits = 1;
     if (p.few) {
-        p.target = 4 * num_cus;
-        const int64_t units = (int64_t)n * a.kv_heads;
-        int64_t s = 4 * ((p.target + units - 1) / units);
-        s = s < 256 ? s : 256;
-        const int64_t fit = (most + kFewKeys * kWaves - 1) / (kFewKeys * kWaves);
-        if (s > fit) s = fit;
-        p.splits = split && s > 1 ? (int)s : 1;
-    } else {
-        const int64_t tiles = (rows / kRows + n) * a.kv_heads;
-        int64_t s = tiles < 2 * num_cus ? (2 * num_cus + tiles - 1) / tiles : 1;
-        const int64_t fit = most / (4 * kKeys);
-        if (s > fit) s = fit;
-        p.splits = split && s > 1 ? (int)s : 1;
-    }
-    // partial results no larger than 1 GiB
-    const int64_t each = (int64_t)a.seqs.tokens * a.heads * (a.head_dim + 2) * 4;
-    if ((int64_t)p.splits * each > (int64_t)1 << 30) p.splits = (int)(((int64_t)1 << 30) / each);
-    if (p.splits < 1) p.splits = 1;
-    if (p.few) {
+        const int64_t step = kFewKeys * kWaves, units = n * a.kv_heads, target = 4 * num_cus;
+        int64_t s = std::min<int64_t>({4 * ((target + units - 1) / units), 256, (most + step - 1) / step});
+        // partial results no larger than 1 GiB
+        s = std::min(s, ((int64_t)1 << 30) / ((int64_t)a.seqs.tokens * a.heads * (a.head_dim + 2) * 4));
+        if (split && s > 1) p.splits = (int)s, p.target = (int)target;
         // sum over sequences of ceil(len / unit) <= n + target / kv_heads
-        int64_t items = n + (p.splits > 1 ? p.target / a.kv_heads + 1 : 0);
-        const int64_t cap = (int64_t)n * p.splits;
-        if (items > cap) items = cap;
-        p.grid = ceil_div(items * a.kv_heads, 1);
-    } else {
-        p.grid = ceil_div((rows / kRows + n) * a.kv_heads * p.splits, 1);
+        p.grid = std::min(n * p.splits, n + (p.splits > 1 ? target / a.kv_heads + 1 : 0)) * a.kv_heads;
+        return p;
+    }
+    const int64_t slots = (int64_t)num_cus * (a.head_dim == 256 ? TileShapeOf<256>::waves : TileShapeOf<128>::waves);
+    p.tiles = (n == 1 ? (rows + kRows - 1) / kRows : rows / kRows + n) * a.kv_heads;
+    p.grid = p.tiles;
+    if (!split) return p;
+    if (p.tiles < slots) {
+        const int64_t s = std::min<int64_t>(most / kLeastKeys, 64);
+        if (s > 1) {
+            p.splits = (int)s;
+            p.target = (int)slots;
+            // tiles x ceil(keys / unit) <= tiles + slots
+            p.grid = std::min(p.tiles * s, p.tiles + slots + 1);
+        }
+    } else if (n == 1 && !a.causal) {
+        const int64_t rest = p.tiles % slots;
+        const int64_t s = rest ? std::min<int64_t>(slots / rest, most / (2 * kLeastKeys)) : 1;
+        if (s > 1) {
+            p.solo = (int)(p.tiles - rest);
+            p.splits = (int)s;
+            p.tiles = rest;
+            p.grid = p.solo + rest * s;
+        }
     }
     return p;
 }
 
 size_t round_256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-size_t part_bytes(const AttnArgs &a, int splits) {
-    if (splits <= 1) return 0;
-    const size_t rows = (size_t)splits * a.seqs.tokens * a.heads;
-    return round_256(rows * a.head_dim * 4) + round_256(rows * 8) + (size_t)a.seqs.tokens * a.heads * 4;
+// Partial results of a plan: their rows, and bytes of the three areas (sums
+// of values, maxima and sums of weights, ranges of a row).
+int64_t part_rows(const AttnArgs &a, const AttnPlan &p) {
+    if (p.splits <= 1) return 0;
+    return p.few ? (int64_t)p.splits * a.seqs.tokens * a.heads : (p.grid - p.solo) * kRows;
+}
+size_t part_bytes(const AttnArgs &a, const AttnPlan &p) {
+    const size_t rows = (size_t)part_rows(a, p);
+    if (rows == 0) return 0;
+    return round_256(rows * a.head_dim * 4) + round_256(rows * 8) + (p.few ? (size_t)a.seqs.tokens * a.heads * 4 : 0);
 }
 
 template <bool BF, int D>
@@ -885,36 +1036,37 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
         else
             hipLaunchKernelGGL((b1_attn_tile_kernel<BF, D, false>), grid, block, 0, s, a);
     }
-    if (p.splits > 1) {
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        const int64_t rows = (int64_t)a.seqs.tokens * a.heads;
-        if (p.splits <= 4)
-            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 1>), dim3(ceil_div(rows, 16)), block, 0, s, a);
-        else if (p.splits <= 16)
-            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 4>), dim3(ceil_div(rows, 4)), block, 0, s, a);
-        else
-            hipLaunchKernelGGL((b1_attn_join_kernel<BF, D, 16>), dim3(rows), block, 0, s, a);
-    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits <= 1) return e;
+    const int64_t rows = (int64_t)a.seqs.tokens * a.heads;
+    if (!p.few)
+        hipLaunchKernelGGL((b1_attn_tile_join_kernel<BF, D>), dim3(p.tiles * (kRows / 16)), block, 0, s, a);
+    else if (p.splits <= 4)
+        hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 1>), dim3((rows + 15) / 16), block, 0, s, a);
+    else if (p.splits <= 16)
+        hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 4>), dim3((rows + 3) / 4), block, 0, s, a);
+    else
+        hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 16>), dim3(rows), block, 0, s, a);
     return hipGetLastError();
 }
 
 } // namespace
 
-size_t attn_workspace_bytes(const AttnArgs &a, int num_cus) {
-    return part_bytes(a, attn_plan(a, num_cus, true).splits);
-}
+size_t attn_workspace_bytes(const AttnArgs &a, int num_cus) { return part_bytes(a, attn_plan(a, num_cus, true)); }
 
 hipError_t launch_attn(const AttnArgs &args, int num_cus, void *ws, size_t ws_bytes, hipStream_t s) {
     AttnArgs a = args;
     AttnPlan p = attn_plan(a, num_cus, true);
-    if (p.splits > 1 && (!ws || ws_bytes < part_bytes(a, p.splits))) p = attn_plan(a, num_cus, false);
+    if (p.splits > 1 && (!ws || ws_bytes < part_bytes(a, p))) p = attn_plan(a, num_cus, false);
     a.splits = p.splits;
     a.target = p.target;
+    a.solo = p.solo;
+    a.items = (int)(p.grid - p.solo);
     if (p.splits > 1) {
-        a.part_o = static_cast<float *>(ws);
-        const size_t rows = (size_t)p.splits * a.seqs.tokens * a.heads;
-        uint8_t *at = static_cast<uint8_t *>(ws) + round_256(rows * a.head_dim * 4);
+        const size_t rows = (size_t)part_rows(a, p);
+        uint8_t *at = static_cast<uint8_t *>(ws);
+        a.part_o = reinterpret_cast<float *>(at);
+        at += round_256(rows * a.head_dim * 4);
         a.part_ml = reinterpret_cast<float *>(at);
         a.part_n = reinterpret_cast<int32_t *>(at + round_256(rows * 8));
     }

@@ -630,7 +630,7 @@ static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
                                  !stride_ok(g->v_head)))
             return BONSAI_B1_ERR_ARG;
         // rows apart from one another, 64 of them within 32-bit offsets
-        const int64_t most = 1 << 24;
+        const int64_t most = 1 << 23;
         if (g->kv_tokens > 1 && (g->k_row < g->head_dim || g->v_row < g->head_dim || g->k_row > most ||
                                  g->v_row > most))
             return BONSAI_B1_ERR_ARG;

@@ -231,12 +231,14 @@ struct AttnArgs {
     int64_t ldo;
     int packed;
     int32_t *bad; // device counter of bad indexes, or NULL
-    // filled by attn_plan / launch_attn
-    int splits = 1;  // key ranges a row's keys may be split into
-    int target = 0;  // small kernel: work-groups wanted
-    float *part_o = nullptr;   // [splits][tokens * heads][head_dim]
-    float *part_ml = nullptr; // [splits][tokens * heads][2]: maximum (base 2), sum
-    int32_t *part_n = nullptr; // [tokens * heads]: the row's ranges
+    // filled by launch_attn
+    int splits = 1;            // most ranges that a row's keys are split into
+    int target = 0;            // work items wanted; 0: exactly `splits` ranges
+    int solo = 0;              // tiles that are not split, the first ones
+    int items = 0;             // work items behind those
+    float *part_o = nullptr;   // partial sums of values [..][head_dim]
+    float *part_ml = nullptr;  // their maxima (base 2) and sums of weights [..][2]
+    int32_t *part_n = nullptr; // few-rows kernel: ranges of a row [tokens * heads]
 };
 
 // Workspace bytes of a call, for a device of num_cus (0: none).

@@ -35,9 +35,11 @@ def attention(q, k, v, scale, causal=False, window=0):
     Returns (out, bound before the output's own rounding), float64.
 
     The bound, per element, with A = sum_j p_j |v_j| / sum_j p_j and the
-    largest weight 1: each weight is rounded to the inputs' type for the
-    product with v (half a step of it times A, and where that type is fp16
-    half its smallest step, 2^-25, for weights below 2^-14); a score's fp32
+    largest weight 1: each weight is rounded to the inputs' type, for the
+    product with v and for the sum it is divided by (half a step of it times
+    A in the product, and in the sum half a step times |out| <= A; where that
+    type is fp16 half its smallest step, 2^-25, in place of half a step for
+    weights below 2^-14, in both); a score's fp32
     sum of d products is off by at most e = (d + 2) U32 scale sum_d |q_d k_d|,
     which changes a weight by a factor 1 + e and the maximum it is relative to
     cancels, so numerator and denominator are off by e each; the sums over nk
@@ -71,8 +73,8 @@ def attention(q, k, v, scale, causal=False, window=0):
                 vi = vh[mask[i]]
                 o[i], big[i], flat[i] = p[i][mask[i]] @ vi, p[i][mask[i]] @ vi.abs(), vi.abs().sum(0)
         e = (d + 2) * U32 * mags.amax(1, keepdim=True)
-        rel = half_step(dtype) + 2 * e + 2 * (nk + 16) * U32
-        tiny = 2.0 ** -25 * flat if dtype == torch.float16 else 0.0
+        rel = 2 * half_step(dtype) + 2 * e + 2 * (nk + 16) * U32
+        tiny = 2.0 ** -25 * (flat + nk * big / total) if dtype == torch.float16 else 0.0
         out[:, h] = torch.where(some[:, None], o / total, 0.0)
         off[:, h] = torch.where(some[:, None], (rel * big + tiny) / total, 0.0)
     return out, off
