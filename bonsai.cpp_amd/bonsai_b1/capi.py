@@ -25,6 +25,7 @@ NOALLOC_SCRATCH_BYTES = 32 << 20
 MODES = {"auto": 0, "fast": 1, "exact": 2, "gemm": 3, "gemv": 4}
 
 _lib = None
+_torch = None  # set by load(): the entry points below run on every step of a model
 
 
 class B1Error(RuntimeError):
@@ -112,7 +113,9 @@ def load():
     global _lib
     if _lib is not None:
         return _lib
-    import torch  # noqa: F401  -- loads torch's libamdhip64 before ours
+    import torch  # loads torch's libamdhip64 before ours
+    global _torch
+    _torch = torch
     if not _LIB.exists():
         raise FileNotFoundError(f"{_LIB} is not built; run __graft_entry__.build() or make -C bonsai.cpp_amd")
     L = ctypes.CDLL(str(_LIB))
@@ -648,76 +651,77 @@ def norm_mod(x, scale, shift, eps: float = 1e-6, out=None, packed=None, stream=N
     return out
 
 
-def _on_current_device(*tensors):
-    """The tensors (None skipped) are cuda tensors of the current device."""
-    import torch
-    d = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("tensors must be cuda tensors")
-        if d is None:
-            d = t.get_device()
-            if d != torch.cuda.current_device():
-                raise ValueError("tensors must be on the current device")
-        elif t.get_device() != d:
+def _on_current_device(tensor, *others):
+    """The index of the current device, on which the tensors (None skipped) are."""
+    d = tensor.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
             raise ValueError("tensors must be on one device")
+    if d < 0 or not tensor.is_cuda:
+        raise ValueError("tensors must be cuda tensors")
+    if d != _torch._C._cuda_getDevice():
+        raise ValueError("tensors must be on the current device")
+    return d
 
 
-def _empty(stream, shape, dtype, device):
+def _raw_stream(stream, device: int):
+    """The handle of `stream`, or of the device's current one."""
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else _torch.cuda.current_stream().cuda_stream
+
+
+def _empty(stream, shape, dtype, device: int):
     """A new tensor that belongs to the stream the call runs on."""
-    import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return _torch.empty(shape, dtype=dtype, device=device)
+    with _torch.cuda.stream(stream):
+        return _torch.empty(shape, dtype=dtype, device=device)
 
 
-def _f32_rows(t, shape, what):
+def _f32_rows(t, rows, cols, what):
     """Row stride of a 2-D fp32 tensor with unit column stride."""
-    import torch
-    if t.dim() != 2 or t.dtype != torch.float32 or t.shape != shape or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what} must be fp32 {tuple(shape)} with unit column stride")
-    return t.stride(0) if shape[0] > 1 else shape[1]
+    if t.dtype is not _torch.float32 or t.shape != (rows, cols):
+        raise ValueError(f"{what} must be fp32 [{rows}, {cols}]")
+    ld, unit = t.stride()
+    if unit != 1 and cols > 1:
+        raise ValueError(f"{what} must have unit column stride")
+    return ld if rows > 1 else cols
 
 
 def _f32_vector(t, n, what):
     """Pointer of a contiguous fp32 vector of n values, or None."""
-    import torch
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not _torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be {n} contiguous fp32 values")
     return t.data_ptr()
 
 
 def _i32_vector(t, n, what):
     """Pointer of a contiguous int32 vector (of n values, if n is given), or None."""
-    import torch
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
+    if t.dtype is not _torch.int32 or t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 vector" + (f" of {n}" if n is not None else ""))
     return t.data_ptr()
 
 
 def _counter(t):
-    import torch
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.numel() < 1:
+    if t.dtype is not _torch.int32 or t.numel() < 1:
         raise ValueError("bad must be an int32 counter")
     return t.data_ptr()
 
 
 def _packed_rows(packed, ldp, rows, cols, stream, device):
     """A packed output (True: a new one) and its row stride in fp16 elements."""
-    import torch
     if packed is True:
         if ldp is not None:
             raise ValueError("ldp is the row length of a packed tensor that is given")
-        packed = _empty(stream, (max(rows * cols * 2, 16),), torch.uint8, device)
+        return _empty(stream, max(rows * cols * 2, 16), _torch.uint8, device), cols
     ldp = cols if ldp is None else ldp
     if not packed.is_contiguous() or (rows > 0 and packed.numel() * packed.element_size()
                                       < ((rows - 1) * ldp + cols) * 2):
@@ -731,105 +735,114 @@ def rms_norm(x, weight=None, eps: float = 1e-6, add=None, residual=None, out=Non
     uint8 tensor, the packed fp16 activations (bonsai_b1_rms_norm_pack_f16).
     With add, or with `residual` (where h is stored; may be x or add),
     returns (h, y), else y."""
-    import torch
-    _on_current_device(x, weight, add, residual, out, packed if packed is not True else None)
+    lib = _lib or load()
+    if packed is False:
+        packed = None
+    dev = _on_current_device(x, weight, add, residual, out, packed if packed is not True else None)
     if x.dim() != 2:
         raise ValueError("x must be [rows, H]")
     rows, h = x.shape
-    ldx = _f32_rows(x, x.shape, "x")
-    ld_add = _f32_rows(add, x.shape, "add") if add is not None else 0
+    ldx = _f32_rows(x, rows, h, "x")
+    add_p, ld_add = (add.data_ptr(), _f32_rows(add, rows, h, "add")) if add is not None else (None, 0)
     if residual is None and add is not None:
-        residual = _empty(stream, x.shape, torch.float32, x.device)
-    ldh = _f32_rows(residual, x.shape, "residual") if residual is not None else 0
-    args = (x.data_ptr(), ldx, add.data_ptr() if add is not None else None, ld_add, h, rows,
-            _f32_vector(weight, h, "weight"), eps, residual.data_ptr() if residual is not None else None, ldh)
-    if packed is not None and packed is not False:
+        residual = _empty(stream, (rows, h), _torch.float32, dev)
+    h_p, ldh = (residual.data_ptr(), _f32_rows(residual, rows, h, "residual")) if residual is not None else (None, 0)
+    w_p = _f32_vector(weight, h, "weight")
+    if packed is not None:
         if out is not None:
             raise ValueError("one of out and packed")
-        y, _ = _packed_rows(packed, None, rows, h, stream, x.device)
-        st = load().bonsai_b1_rms_norm_pack_f16(*args, y.data_ptr(), _stream_handle(stream))
+        y, _ = _packed_rows(packed, None, rows, h, stream, dev)
         what = "bonsai_b1_rms_norm_pack_f16"
+        st = lib.bonsai_b1_rms_norm_pack_f16(x.data_ptr(), ldx, add_p, ld_add, h, rows, w_p, eps, h_p, ldh,
+                                             y.data_ptr(), _raw_stream(stream, dev))
     else:
-        y = out if out is not None else _empty(stream, x.shape, torch.float32, x.device)
-        st = load().bonsai_b1_rms_norm_f32(*args, y.data_ptr(), _f32_rows(y, x.shape, "out"), _stream_handle(stream))
+        y = out if out is not None else _empty(stream, (rows, h), _torch.float32, dev)
         what = "bonsai_b1_rms_norm_f32"
+        st = lib.bonsai_b1_rms_norm_f32(x.data_ptr(), ldx, add_p, ld_add, h, rows, w_p, eps, h_p, ldh, y.data_ptr(),
+                                        _f32_rows(y, rows, h, "out"), _raw_stream(stream, dev))
     if st != OK:
         raise B1Error(st, what)
     return y if residual is None else (residual, y)
 
 
 def _dtype_code(dtype):
-    import torch
-    if dtype == torch.float16:
+    if dtype is _torch.float16:
         return F16
-    if dtype == torch.bfloat16:
+    if dtype is _torch.bfloat16:
         return BF16
     raise ValueError("queries, keys and values are fp16 or bf16")
 
 
 def _kv_pages(k_cache, v_cache, kv_len, pages, n_seqs):
     """The bonsai_b1_kv_pages of caches [pages, kv_heads, page_size, head_dim]."""
-    import torch
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
         raise ValueError("k_cache and v_cache must be [pages, kv_heads, page_size, head_dim] of one type")
     n, heads, size, d = k_cache.shape
-    sk, sv = k_cache.stride(), v_cache.stride()
-    if sk[3] != 1 or sk != sv:
+    s = k_cache.stride()
+    if s[3] != 1 or s != v_cache.stride():
         raise ValueError("k_cache and v_cache must have the same strides, 1 within a head")
-    if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != n_seqs or \
-            (pages.shape[1] > 1 and pages.stride(1) != 1):
+    if pages.dtype is not _torch.int32 or pages.dim() != 2 or pages.shape[0] != n_seqs:
         raise ValueError(f"pages must be int32 [{n_seqs}, pages a sequence]")
     most = pages.shape[1]
-    return KvPages(k_cache.data_ptr(), v_cache.data_ptr(), n, size, sk[0] if n > 1 else heads * size * d,
-                   sk[1] if heads > 1 else size * d, sk[2] if size > 1 else d, pages.data_ptr(),
-                   pages.stride(0) if n_seqs > 1 else most, most, _i32_vector(kv_len, n_seqs, "kv_len"))
+    ld, unit = pages.stride()
+    if unit != 1 and most > 1:
+        raise ValueError("a sequence's pages must lie side by side")
+    return KvPages(k_cache.data_ptr(), v_cache.data_ptr(), n, size, s[0] if n > 1 else heads * size * d,
+                   s[1] if heads > 1 else size * d, s[2] if size > 1 else d, pages.data_ptr(),
+                   ld if n_seqs > 1 else most, most, _i32_vector(kv_len, n_seqs, "kv_len"))
 
 
-def _n_seqs(q_start, tokens):
+def _n_seqs(q_start):
+    """Sequences of a call: one without starts."""
     if q_start is None:
-        return 1 if tokens else 0
+        return 1
     if q_start.dim() != 1 or q_start.numel() < 1:
         raise ValueError("q_start must hold the sequences' first rows and the last one's end")
     return q_start.numel() - 1
 
 
+def _heads_out(t, tokens, heads, d, dtype, stream, dev, what):
+    """A 16-bit output [tokens, heads, d] (None: a new one) and its row stride."""
+    if t is None:
+        return _empty(stream, (tokens, heads, d), dtype, dev), heads * d
+    if t.dtype is not dtype or t.shape != (tokens, heads, d):
+        raise ValueError(f"{what} must be {dtype} [{tokens}, {heads}, {d}]")
+    s = t.stride()
+    if tokens and (s[2] != 1 or (heads > 1 and s[1] != d)):
+        raise ValueError(f"a token's heads must lie side by side in {what}")
+    return t, s[0] if tokens > 1 else heads * d
+
+
 def _qkv(q, k, v, head_dim, q_weight, k_weight, eps, rope, positions, interleaved, dtype, q_out, k_out, v_out, pages,
-         n_seqs, q_start, bad, stream, kv_heads):
-    import torch
+         n_seqs, q_start, bad, stream, kv_heads, dev):
+    lib = _lib or load()
     if q.dim() != 2 or head_dim <= 0 or q.shape[1] % head_dim:
         raise ValueError("q must be [tokens, heads * head_dim]")
-    tokens, heads = q.shape[0], q.shape[1] // head_dim
-    kv = (tokens, kv_heads * head_dim)
-    ldq, ldk, ldv = _f32_rows(q, q.shape, "q"), _f32_rows(k, kv, "k"), _f32_rows(v, kv, "v")
-    rows = dim = 0
+    tokens, width = q.shape
+    heads, kv_width = width // head_dim, kv_heads * head_dim
+    rope_p, rows, dim = None, 0, 0
     if rope is not None:
-        if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
+        if rope.dim() != 2 or rope.dtype is not _torch.float32 or not rope.is_contiguous():
             raise ValueError("rope must be a contiguous fp32 table [positions, rope_dim]")
-        rows, dim = rope.shape
-
-    def output(t, n, what):
-        if t is None:
-            t = _empty(stream, (tokens, n, head_dim), dtype, q.device)
-        if t.dtype != dtype or t.shape != (tokens, n, head_dim) or (tokens and (
-                t.stride(2) != 1 or (n > 1 and t.stride(1) != head_dim))):
-            raise ValueError(f"{what} must be {dtype} [tokens, {n}, {head_dim}], a token's heads side by side")
-        return t, t.stride(0) if tokens > 1 else n * head_dim
-
-    q_out, ld_q = output(q_out, heads, "q_out")
+        rope_p, (rows, dim) = rope.data_ptr(), rope.shape
+    q_out, ld_q = _heads_out(q_out, tokens, heads, head_dim, dtype, stream, dev, "q_out")
+    k_p = v_p = kv_p = None
     ld_kv = 0
     if pages is None:
-        k_out, ld_kv = output(k_out, kv_heads, "k_out")
-        v_out, ld_v = output(v_out, kv_heads, "v_out")
+        k_out, ld_kv = _heads_out(k_out, tokens, kv_heads, head_dim, dtype, stream, dev, "k_out")
+        v_out, ld_v = _heads_out(v_out, tokens, kv_heads, head_dim, dtype, stream, dev, "v_out")
         if ld_v != ld_kv:
             raise ValueError("k_out and v_out must have one row stride")
-    args = QkvArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), ldq, ldk, ldv, tokens, heads, kv_heads, head_dim,
-                   _f32_vector(q_weight, head_dim, "q_weight"), _f32_vector(k_weight, head_dim, "k_weight"), eps,
-                   rope.data_ptr() if rope is not None else None, rows, dim, 1 if interleaved else 0,
-                   _i32_vector(positions, tokens, "positions"), _dtype_code(dtype), q_out.data_ptr(), ld_q,
-                   k_out.data_ptr() if pages is None else None, v_out.data_ptr() if pages is None else None, ld_kv,
-                   ctypes.pointer(pages) if pages is not None else None, n_seqs,
+        k_p, v_p = k_out.data_ptr(), v_out.data_ptr()
+    else:
+        kv_p = ctypes.pointer(pages)
+    args = QkvArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), _f32_rows(q, tokens, width, "q"),
+                   _f32_rows(k, tokens, kv_width, "k"), _f32_rows(v, tokens, kv_width, "v"), tokens, heads, kv_heads,
+                   head_dim, _f32_vector(q_weight, head_dim, "q_weight"), _f32_vector(k_weight, head_dim, "k_weight"),
+                   eps, rope_p, rows, dim, 1 if interleaved else 0, _i32_vector(positions, tokens, "positions"),
+                   _dtype_code(dtype), q_out.data_ptr(), ld_q, k_p, v_p, ld_kv, kv_p, n_seqs,
                    _i32_vector(q_start, None, "q_start"), _counter(bad))
-    st = load().bonsai_b1_qkv_rope(ctypes.byref(args), _stream_handle(stream))
+    st = lib.bonsai_b1_qkv_rope(ctypes.byref(args), _raw_stream(stream, dev))
     if st != OK:
         raise B1Error(st, "bonsai_b1_qkv_rope")
     return q_out, k_out, v_out
@@ -841,13 +854,14 @@ def qkv_rope(q, k, v, head_dim: int, q_weight=None, k_weight=None, eps: float = 
     heads * head_dim], k and v [tokens, kv_heads * head_dim], as 16-bit
     (q, k, v) [tokens, heads, head_dim] (bonsai_b1_qkv_rope).  rope: table
     [positions, rope_dim], cosines then sines; dtype: fp16 unless given."""
-    import torch
-    _on_current_device(q, k, v, q_weight, k_weight, rope, positions, q_out, k_out, v_out, bad)
+    if _lib is None:
+        load()
+    dev = _on_current_device(q, k, v, q_weight, k_weight, rope, positions, q_out, k_out, v_out, bad)
     if k.dim() != 2 or head_dim <= 0 or k.shape[1] % head_dim:
         raise ValueError("k must be [tokens, kv_heads * head_dim]")
     return _qkv(q, k, v, head_dim, q_weight, k_weight, eps, rope, positions, interleaved,
-                dtype if dtype is not None else torch.float16, q_out, k_out, v_out, None, 0, None, bad, stream,
-                k.shape[1] // head_dim)
+                dtype if dtype is not None else _torch.float16, q_out, k_out, v_out, None, 0, None, bad, stream,
+                k.shape[1] // head_dim, dev)
 
 
 def qkv_rope_paged(q, k, v, k_cache, v_cache, q_start, kv_len, pages, q_weight=None, k_weight=None,
@@ -857,51 +871,53 @@ def qkv_rope_paged(q, k, v, k_cache, v_cache, q_start, kv_len, pages, q_weight=N
     (k_cache, v_cache [pages, kv_heads, page_size, head_dim], strided views
     allowed): the tokens of sequence b, rows q_start[b] .. q_start[b + 1]
     (None: one sequence), are the last of its kv_len[b] keys.  Returns q."""
-    _on_current_device(q, k, v, k_cache, v_cache, q_start, kv_len, pages, q_weight, k_weight, rope, positions, q_out,
-                       bad)
-    n = _n_seqs(q_start, q.shape[0])
-    kv = _kv_pages(k_cache, v_cache, kv_len, pages, n if q_start is not None else 1)
+    if _lib is None:
+        load()
+    dev = _on_current_device(q, k, v, k_cache, v_cache, q_start, kv_len, pages, q_weight, k_weight, rope, positions,
+                             q_out, bad)
+    n = _n_seqs(q_start)
+    kv = _kv_pages(k_cache, v_cache, kv_len, pages, n)
     return _qkv(q, k, v, k_cache.shape[3], q_weight, k_weight, eps, rope, positions, interleaved, k_cache.dtype,
-                q_out, None, None, kv, n, q_start, bad, stream, k_cache.shape[1])[0]
+                q_out, None, None, kv, n, q_start, bad, stream, k_cache.shape[1], dev)[0]
 
 
 def _heads_strides(t, what):
     """Token and head strides of a 16-bit [tokens, heads, head_dim] tensor."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"{what} must be [tokens, heads, head_dim] with unit stride within a head")
     n, heads, d = t.shape
-    return t.stride(0) if n > 1 else heads * d, t.stride(1) if heads > 1 else d
+    s = t.stride()
+    if s[2] != 1 and d > 1:
+        raise ValueError(f"{what} must have unit stride within a head")
+    return s[0] if n > 1 else heads * d, s[1] if heads > 1 else d
 
 
 def _attention(q, k, v, pages, kv_heads, q_start, kv_start, n_seqs, causal, window, scale, out, packed, ldp, bad,
-               workspace, stream):
+               workspace, stream, dev):
     q_row, q_head = _heads_strides(q, "q")
     tokens, heads, d = q.shape
     if kv_heads <= 0 or heads % kv_heads:
         raise ValueError("heads must be a multiple of the key heads")
-    if packed is not None and packed is not False:
+    if packed is not None:
         if out is not None:
             raise ValueError("one of out and packed")
-        y, ldo = _packed_rows(packed, ldp, tokens, heads * d, stream, q.device)
+        y, ldo = _packed_rows(packed, ldp, tokens, heads * d, stream, dev)
         form = 1
     else:
-        y = out if out is not None else _empty(stream, (tokens, heads, d), q.dtype, q.device)
-        if y.dtype != q.dtype or y.shape != q.shape or (tokens and (y.stride(2) != 1 or (heads > 1
-                                                                                        and y.stride(1) != d))):
-            raise ValueError("out must be like q, a token's heads side by side")
-        ldo, form = y.stride(0) if tokens > 1 else heads * d, 0
+        y, ldo = _heads_out(out, tokens, heads, d, q.dtype, stream, dev, "out")
+        form = 0
+    k_p = v_p = kv_p = None
     k_row = k_head = v_row = v_head = kv_tokens = 0
     if pages is None:
         (k_row, k_head), (v_row, v_head), kv_tokens = _heads_strides(k, "k"), _heads_strides(v, "v"), k.shape[0]
-    args = AttentionArgs(q.data_ptr(), k.data_ptr() if pages is None else None,
-                         v.data_ptr() if pages is None else None, q_row, q_head, k_row, k_head, v_row, v_head,
-                         _dtype_code(q.dtype), heads, kv_heads, d, tokens, kv_tokens, n_seqs,
-                         _i32_vector(q_start, None, "q_start"), _i32_vector(kv_start, n_seqs + 1, "kv_start"),
-                         ctypes.pointer(pages) if pages is not None else None, 1 if causal else 0, window,
+        k_p, v_p = k.data_ptr(), v.data_ptr()
+    else:
+        kv_p = ctypes.pointer(pages)
+    args = AttentionArgs(q.data_ptr(), k_p, v_p, q_row, q_head, k_row, k_head, v_row, v_head, _dtype_code(q.dtype),
+                         heads, kv_heads, d, tokens, kv_tokens, n_seqs, _i32_vector(q_start, None, "q_start"),
+                         _i32_vector(kv_start, n_seqs + 1, "kv_start"), kv_p, 1 if causal else 0, window,
                          scale if scale is not None else d ** -0.5, y.data_ptr(), ldo, form, _counter(bad))
     ws, wsb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None \
         else (None, 0)
-    st = load().bonsai_b1_attention(ctypes.byref(args), ws, wsb, _stream_handle(stream))
+    st = _lib.bonsai_b1_attention(ctypes.byref(args), ws, wsb, _raw_stream(stream, dev))
     if st != OK:
         raise B1Error(st, "bonsai_b1_attention")
     return y
@@ -916,18 +932,21 @@ def attention(q, k, v, q_start=None, kv_start=None, causal: bool = False, window
     Returns out [tokens, heads, head_dim], or, with packed=True or a uint8
     tensor (with ldp a view at the target columns), the packed fp16
     activations of heads * head_dim columns."""
-    _on_current_device(q, k, v, q_start, kv_start, out, packed if packed is not True and packed is not False else None,
-                       bad, workspace)
-    if k.dim() != 3 or k.shape != v.shape or q.dim() != 3 or k.shape[2] != q.shape[2] or \
-            not q.dtype == k.dtype == v.dtype:
+    if _lib is None:
+        load()
+    if packed is False:
+        packed = None
+    dev = _on_current_device(q, k, v, q_start, kv_start, out, packed if packed is not True else None, bad, workspace)
+    dtype = q.dtype
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2] or k.dtype is not dtype or \
+            v.dtype is not dtype:
         raise ValueError("k and v must be [keys, kv_heads, head_dim] of q's type and head_dim")
     if kv_start is None and q_start is not None:
         if k.shape[0] != q.shape[0]:
             raise ValueError("keys apart from the tokens need kv_start")
         kv_start = q_start
-    n = _n_seqs(q_start, q.shape[0])
-    return _attention(q, k, v, None, k.shape[1], q_start, kv_start, n, causal, window, scale, out, packed, ldp, bad,
-                      workspace, stream)
+    return _attention(q, k, v, None, k.shape[1], q_start, kv_start, _n_seqs(q_start), causal, window, scale, out,
+                      packed, ldp, bad, workspace, stream, dev)
 
 
 def attention_paged(q, k_cache, v_cache, q_start, kv_len, pages, causal: bool = True, window: int = 0, scale=None,
@@ -936,14 +955,18 @@ def attention_paged(q, k_cache, v_cache, q_start, kv_len, pages, causal: bool = 
     page_size, head_dim], strided views allowed): sequence b's keys are the
     first kv_len[b] places of its pages, its tokens the last of them.  With
     packed-sequence starts q_start (None: one sequence)."""
-    _on_current_device(q, k_cache, v_cache, q_start, kv_len, pages, out,
-                       packed if packed is not True and packed is not False else None, bad, workspace)
-    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape[3] != q.shape[2] or k_cache.dtype != q.dtype:
+    if _lib is None:
+        load()
+    if packed is False:
+        packed = None
+    dev = _on_current_device(q, k_cache, v_cache, q_start, kv_len, pages, out, packed if packed is not True else None,
+                             bad, workspace)
+    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape[3] != q.shape[2] or k_cache.dtype is not q.dtype:
         raise ValueError("the caches must be [pages, kv_heads, page_size, head_dim] of q's type and head_dim")
-    n = _n_seqs(q_start, q.shape[0])
-    kv = _kv_pages(k_cache, v_cache, kv_len, pages, n if q_start is not None else 1)
+    n = _n_seqs(q_start)
+    kv = _kv_pages(k_cache, v_cache, kv_len, pages, n)
     return _attention(q, None, None, kv, k_cache.shape[1], q_start, None, n, causal, window, scale, out, packed, ldp,
-                      bad, workspace, stream)
+                      bad, workspace, stream, dev)
 
 
 class SafetensorsFile:
