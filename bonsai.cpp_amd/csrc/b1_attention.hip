@@ -168,6 +168,7 @@ template <int D>
 struct TileShapeOf {
     static constexpr int keys = D == 64 ? 64 : 32;
     static constexpr int waves = D == 256 ? 2 : 3;
+    static constexpr int stages = D == 256 ? 2 : 3; // in LDS
 };
 // A range of a split tile has at least this many keys, so that its fixed
 // costs (queries, partial sums out and in) stay small beside them.
@@ -321,11 +322,28 @@ __device__ __forceinline__ TileRange tile_range(const TileKeys &k, int splits, i
     return r;
 }
 
-// A range-checked resource over `bytes` from p (none where it is negative,
+// A buffer resource over `bytes` from p (uniform; none where it is negative,
 // as for keys past the last): reads at or past its end give zeros and touch
 // no memory.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t key_buffer(const uint16_t *p, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, max(0, bytes), kBufferFlags);
+__device__ __forceinline__ u32x4 key_buffer(const uint16_t *p, int bytes) {
+    const uint64_t v = (uint64_t)p;
+    return u32x4{(uint32_t)v, (uint32_t)(v >> 32) & 0xffffu, (uint32_t)max(0, bytes), (uint32_t)kBufferFlags};
+}
+
+// 16 bytes a lane from byte `off` of a resource to lds + 16 * lane (uniform
+// lds).  In assembly so that the compiler does not wait for the copy before
+// reads of LDS that other copies filled, as it does for its own builtin
+// where it cannot tell the two apart; there is no output register.  The
+// reader waits with wait_vmcnt and a barrier.  (The compiler's own counted
+// waits stay right: copies that it does not count only make them longer.)
+__device__ __forceinline__ void copy_to_lds(u32x4 rsrc, uint8_t *lds, uint32_t off) {
+    const uint32_t at = (uint32_t)(uintptr_t)(lds_void_t *)lds;
+    uint32_t m0; // the compiler's, kept
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+                 "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(at), "v"(off), "s"(rsrc)
+                 : "memory");
 }
 
 // Bound by the matrix units together with the vector instructions of the
@@ -335,11 +353,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t key_buffer(const uint16_t *p, 
 // another's LDS reads, barriers and copies.
 template <bool BF, int D, bool PAGED>
 __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kernel(AttnArgs a) {
-    constexpr int ST = D / 16, DT = D / 32, CH = D / 8, KK = TileShapeOf<D>::keys, KT = KK / 32;
-    // two stages of keys and values, as four objects: the compiler then knows
-    // that the copies into one stage do not concern the reads of the other,
-    // and does not wait for them before these
-    __shared__ __align__(1024) uint8_t k0[KK * D * 2], k1[KK * D * 2], v0[KK * D * 2], v1[KK * D * 2];
+    constexpr int ST = D / 16, DT = D / 32, CH = D / 8, KK = TileShapeOf<D>::keys, KT = KK / 32,
+                  S = TileShapeOf<D>::stages, SB = KK * D * 2;
+    __shared__ __align__(1024) uint8_t sk[S][SB], sv[S][SB];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int l31 = lane & 31, h = lane >> 5;
     const int group = a.heads / a.kv_heads;
@@ -376,41 +392,59 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 
     // Copies a stage.  A wave's instruction copies the NR rows that lie in 1
     // KiB; lane i lands at 16 i, so the swizzle is in which chunk of the row
-    // it reads.  Rows past the last key read zeros.  Paged: `page` is the
-    // page of key kb + lane, keys and values lie alike, and rows of more than
-    // one page (of fewer than NR keys) take an instruction a page.
-    constexpr int NR = 512 / D, NI = KK * D / 2048;
-    auto load = [&](int kb, int page, uint8_t *ks, uint8_t *vs) __attribute__((always_inline)) {
+    // it reads.  Rows past the last key read zeros.  Paged: keys and values
+    // lie alike, `page` holds the page of each instruction's first row, and
+    // rows of more than one page (of fewer than NR keys) take an instruction
+    // a page.
+    constexpr int NR = 512 / D, NI = SB / 4096;
+    struct Pages {
+        int id[PAGED ? NI : 1];
+    };
+    auto page_at = [&](int j) __attribute__((always_inline)) {
+        // a scalar read: it does not wait for the copies under way
+        typedef const __attribute__((address_space(4))) int32_t *scalar_ptr;
+        const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.seqs.pages + b * a.seqs.ld_pages);
+        return table[min(j, s.nk - 1) >> a.seqs.page_shift];
+    };
+    auto pages = [&](int kb) __attribute__((always_inline)) {
+        Pages p;
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) p.id[i] = page_at(kb + (wave * NI + i) * NR);
+        }
+        return p;
+    };
+    auto load = [&](int kb, const Pages &page, int to) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int at = wave * NI + i, row0 = at * NR;
             const int row = row0 + lane / CH;
             const int ck = ((lane % CH) ^ swizzle_k<D>(row)) * 16, cv = ((lane % CH) ^ swizzle_v<D>(row)) * 16;
+            uint8_t *const ks = sk[to] + at * 1024, *const vs = sv[to] + at * 1024;
             if constexpr (PAGED) {
-                const int size = 1 << a.seqs.page_shift, span = min(size, NR);
-                const int bytes = (int)kr.row * 2;
+                const int size = 1 << a.seqs.page_shift, bytes = (int)kr.row * 2;
                 const uint32_t off = (uint32_t)((kb + row) & (size - 1)) * (uint32_t)bytes;
-                for (int sub = 0; sub < NR; sub += span) {
-                    const int64_t at_page = __builtin_amdgcn_readlane(page, row0 + sub) * kr.page;
+                auto copy = [&](int id, int j) __attribute__((always_inline)) {
+                    if ((unsigned)id >= (unsigned)a.seqs.n_pages) bad = true, id = 0;
                     // keys of the page up to the sequence's last
-                    const int keys = min(size, s.nk - ((kb + row0 + sub) & -size));
-                    if (NR == span || (unsigned)(lane / CH - sub) < (unsigned)span) {
-                        dma_buf_lds16(key_buffer(kr.base + at_page, keys * bytes), ks + at * 1024, off + ck);
-                        dma_buf_lds16(key_buffer(vr.base + at_page, keys * bytes), vs + at * 1024, off + cv);
+                    const int keys = min(size, s.nk - (j & -size));
+                    copy_to_lds(key_buffer(kr.base + id * kr.page, keys * bytes), ks, off + ck);
+                    copy_to_lds(key_buffer(vr.base + id * vr.page, keys * bytes), vs, off + cv);
+                };
+                if (size >= NR) {
+                    copy(page.id[i], kb + row0);
+                } else {
+                    for (int sub = 0; sub < NR; sub += size) {
+                        const int id = page_at(kb + row0 + sub);
+                        if ((unsigned)(lane / CH - sub) < (unsigned)size) copy(id, kb + row0 + sub);
                     }
                 }
             } else {
                 const int keys = min(KK, s.nk - kb), kbytes = (int)kr.row * 2, vbytes = (int)vr.row * 2;
-                dma_buf_lds16(key_buffer(kr.base + kb * kr.row, keys * kbytes), ks + at * 1024, row * kbytes + ck);
-                dma_buf_lds16(key_buffer(vr.base + kb * vr.row, keys * vbytes), vs + at * 1024, row * vbytes + cv);
+                copy_to_lds(key_buffer(kr.base + kb * kr.row, keys * kbytes), ks, row * kbytes + ck);
+                copy_to_lds(key_buffer(vr.base + kb * vr.row, keys * vbytes), vs, row * vbytes + cv);
             }
         }
-    };
-    auto pages = [&](int kb) __attribute__((always_inline)) {
-        if constexpr (PAGED)
-            return page_of(a.seqs, b, min(kb + lane, s.nk - 1), bad);
-        else
-            return 0;
     };
 
     u32x4 qf[ST];
@@ -422,22 +456,30 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     float m = kLowest, l = 0.f;
     const float scale2 = a.scale * 1.44269504f; // exp(x) = exp2(x log2 e)
 
-    int next = 0; // pages of the stage after the one that is being copied
+    // S - 1 stages are being copied while one is read
+    Pages next = {}; // of the stage to copy next
     if (t0 < t1) {
-        load(t0 * KK, pages(t0 * KK), k0, v0);
-        next = pages((t0 + 1) * KK);
-    }
-    auto stage = [&](int tt, const uint8_t *ks, const uint8_t *vs, uint8_t *ks2, uint8_t *vs2)
-                     __attribute__((always_inline)) {
-        const int kb = tt * KK;
-        // every wave's copies of this stage are there, and its reads of the
-        // last one done
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (t0 + i < t1) load((t0 + i) * KK, pages((t0 + i) * KK), i);
+        next = pages((t0 + S - 1) * KK);
+        // the queries too, so that no wait for them remains in the loop
         wait_vmcnt<0>();
+    }
+    auto stage = [&](int tt, int at) __attribute__((always_inline)) {
+        const int kb = tt * KK;
+        const uint8_t *const ks = sk[at], *const vs = sv[at];
+        // every wave's copies of this stage are there (those of the next ones
+        // may be under way), and its reads of the last one done
+        if (S > 2 && tt + S - 2 < t1)
+            wait_vmcnt<2 * NI * (S - 2)>();
+        else
+            wait_vmcnt<0>();
         wait_lgkmcnt0();
         lds_barrier();
-        if (tt + 1 < t1) {
-            load(kb + KK, next, ks2, vs2);
-            next = pages(kb + 2 * KK);
+        if (tt + S - 1 < t1) {
+            load(kb + (S - 1) * KK, next, (at + S - 1) % S);
+            next = pages(kb + S * KK);
         }
         if (!wave_on || kb > last_hi || kb + KK - 1 < first_lo) return;
         // scores, transposed: column = row of q, register i of half h = key
@@ -504,9 +546,10 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
             }
         }
     };
-    for (int tt = t0; tt < t1; tt += 2) {
-        stage(tt, k0, v0, k1, v1);
-        if (tt + 1 < t1) stage(tt + 1, k1, v1, k0, v0);
+    for (int tt = t0; tt < t1; tt += S) {
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (tt + i < t1) stage(tt + i, i);
     }
     l = halves_sum(l);
 
