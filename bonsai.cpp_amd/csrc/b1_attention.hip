@@ -74,6 +74,11 @@ __device__ __forceinline__ u32x2 read_columns(const void *p) {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < kInf; }
 
+// x / group for 0 <= x < 2^28 (AttnArgs::div_m and div_s).
+__device__ __forceinline__ int div_group(const AttnArgs &a, int x) {
+    return (int)((__umulhi((uint32_t)x, a.div_m) + (uint32_t)x) >> a.div_s);
+}
+
 // One key head's keys (or values) of one sequence.
 struct KeyRows {
     const uint16_t *base; // contiguous: the sequence's first row
@@ -203,38 +208,58 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, i
     k.r0 = t * kRows;
     k.rows = min(kRows, s.nq * group - k.r0);
     int lo, hi, x;
-    visible(a, s, k.r0 / group, lo, x);
-    visible(a, s, (k.r0 + k.rows - 1) / group, x, hi);
+    visible(a, s, div_group(a, k.r0), lo, x);
+    visible(a, s, div_group(a, k.r0 + k.rows - 1), x, hi);
     k.k0 = lo;
     k.k1 = max(hi + 1, lo);
     return k;
 }
 __device__ __forceinline__ int seq_tiles(const Seq &s, int group) { return (s.nq * group + kRows - 1) / kRows; }
 
-// Into how many ranges a sequence's tiles are split: a fixed number, or so
-// that all ranges of all sequences have about the same number of keys and
-// make about a.target work items.
-__device__ __forceinline__ int seq_last_keys(const AttnArgs &a, const Seq &s, int group) {
-    const int n = seq_tiles(s, group);
-    if (n == 0) return 0;
-    const TileKeys k = tile_keys(a, s, group, n - 1);
-    return k.k1 - k.k0;
-}
-__device__ __forceinline__ int tile_unit(const AttnArgs &a, int group) {
-    if (a.splits == 1 || a.target == 0) return 0;
-    const int lane = threadIdx.x & 63;
-    float total = 0.f; // a range's size needs no more
-    for (int b = lane; b < a.seqs.n_seqs; b += 64) {
-        const Seq s = seq_of(a.seqs, b);
-        total += (float)seq_tiles(s, group) * (float)seq_last_keys(a, s, group);
+// Into how many ranges a call's tiles are split: a fixed number each
+// (a.target 0), or so that all ranges of all sequences have about the same
+// number of keys and make about a.target work items, where that pays.
+//
+// It does when the longest tile, alone with what shares its CU, takes longer
+// than everything at the rate of a full device and the partial sums' way out
+// and in.  In us at D = 128, measured: a 32-key step of a tile 0.72 with one
+// work-group a CU, 1.15 with two, 1.5 with three; a partial tile 0.026.
+// Split against whole (us): 128 tiles over 4096 keys 62 / 97, 8 over 4000
+// 27 / 96, 128 over 1000 31 / 32, 256 over 1024 (causal) 41 / 33, 480 over
+// 2560 126 / 99.
+struct SeqWork {
+    int tiles;         // of a key head
+    float last, total; // keys of the last tile, of all of them
+};
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, const Seq &s, int group) {
+    SeqWork w = {seq_tiles(s, group), 0.f, 0.f};
+    if (w.tiles > 0) {
+        const TileKeys x = tile_keys(a, s, group, 0), y = tile_keys(a, s, group, w.tiles - 1);
+        w.last = (float)(y.k1 - y.k0);
+        w.total = (float)w.tiles * 0.5f * ((float)(x.k1 - x.k0) + w.last);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
-    return max(kLeastKeys, (int)fminf(total * (float)a.kv_heads / (float)a.target, 1.0e9f) + 1);
+    return w;
 }
-__device__ __forceinline__ int seq_splits(const AttnArgs &a, const Seq &s, int group, int unit) {
-    if (a.splits == 1 || a.target == 0) return a.splits;
-    return max(1, min(a.splits, (seq_last_keys(a, s, group) + unit - 1) / unit));
+// Keys a range; 0: whole tiles.  `total`, `longest` and `tiles` over all
+// sequences.
+__device__ __forceinline__ float tile_unit(const AttnArgs &a, float total, float longest, float tiles) {
+    total *= (float)a.kv_heads;
+    tiles *= (float)a.kv_heads;
+    const float cus = (float)a.target * (1.f / TileShapeOf<128>::waves), scale = (float)a.head_dim * (1.f / 128);
+    const float whole = longest * (1.f / 32) * scale * (tiles <= cus ? 0.72f : tiles <= 2 * cus ? 1.15f : 1.5f);
+    const float parts = tiles + fminf((float)a.target, total * (1.f / kLeastKeys));
+    const float split = (total * (1.f / 32) * 1.7f / (float)a.target + 0.026f * parts) * scale + 8.f;
+    if (whole < 1.2f * split) return 0.f;
+    return fmaxf((float)kLeastKeys, total / (float)a.target + 1.f);
+}
+// The unit that makes `items` (of a key head, at the unit so far) fit the
+// device at once: a few more than that would run after all others.
+__device__ __forceinline__ float fit_unit(const AttnArgs &a, float unit, float items) {
+    return unit * fmaxf(1.f, items * (float)a.kv_heads / (float)a.target);
+}
+__device__ __forceinline__ int seq_splits(const AttnArgs &a, float last, float unit) {
+    if (unit == 0.f) return 1;
+    return max(1, min(a.splits, (int)ceilf(last / unit)));
 }
 
 // A work item: key head, row tile and range of one of the sequences.  The
@@ -243,38 +268,73 @@ __device__ __forceinline__ int seq_splits(const AttnArgs &a, const Seq &s, int g
 // part .. part + splits - 1.
 struct TileItem {
     int b, kvh, t, range, splits, part;
+    Seq s;
 };
 // Finds item i (or, of whole tiles, the i-th tile behind the solo ones), by
 // the whole wave; b = -1: none.
 __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int i, bool whole) {
     TileItem r;
     const int lane = threadIdx.x & 63;
-    const int unit = tile_unit(a, group);
-    int j = i, tiles0 = 0, items0 = 0, g;
+    int j = i, g = 0;
     r.b = -1;
     r.splits = 1;
     r.range = 0;
     r.part = 0;
-    if (a.solo > 0) { // one sequence
-        r.b = 0;
+    r.s = Seq{};
+    if (a.seqs.n_seqs == 1) {
+        r.s = seq_of(a.seqs, 0);
+        if (a.solo == 0 && a.splits > 1) {
+            const SeqWork w = seq_work(a, r.s, group);
+            float unit = tile_unit(a, w.total, w.last, (float)w.tiles);
+            if (unit > 0.f) unit = fit_unit(a, unit, (float)(w.tiles * seq_splits(a, w.last, unit)));
+            r.splits = seq_splits(a, w.last, unit);
+        }
         if (!whole && i < a.solo) {
             g = i;
         } else {
+            if (a.solo > 0) r.splits = a.splits;
             j = whole ? i : i - a.solo;
-            r.splits = a.splits;
             g = a.solo + (whole ? j : j / r.splits);
-            r.range = whole ? 0 : j % r.splits;
+            r.range = whole ? 0 : j - (g - a.solo) * r.splits;
             r.part = (g - a.solo) * r.splits;
         }
-        if (g >= seq_tiles(seq_of(a.seqs, 0), group) * a.kv_heads) r.b = -1;
+        if (g < seq_tiles(r.s, group) * a.kv_heads) r.b = 0;
     } else {
-        for (int b0 = 0; b0 < a.seqs.n_seqs && r.b < 0; b0 += 64) {
-            int n = 0, c = 1;
-            if (b0 + lane < a.seqs.n_seqs) {
-                const Seq s = seq_of(a.seqs, b0 + lane);
-                n = seq_tiles(s, group) * a.kv_heads;
-                c = seq_splits(a, s, group, unit);
+        // the first 64 sequences stay in registers for both passes
+        const Seq mine = lane < a.seqs.n_seqs ? seq_of(a.seqs, lane) : Seq{};
+        const SeqWork work = seq_work(a, mine, group);
+        float unit = 0.f;
+        if (a.splits > 1) {
+            float total = work.total, longest = work.last, tiles = (float)work.tiles;
+            for (int b = 64 + lane; b < a.seqs.n_seqs; b += 64) {
+                const SeqWork w = seq_work(a, seq_of(a.seqs, b), group);
+                total += w.total;
+                longest = fmaxf(longest, w.last);
+                tiles += (float)w.tiles;
             }
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) {
+                total += __shfl_xor(total, o);
+                longest = fmaxf(longest, __shfl_xor(longest, o));
+                tiles += __shfl_xor(tiles, o);
+            }
+            unit = tile_unit(a, total, longest, tiles);
+            for (int k = 0; k < 2 && unit > 0.f && a.seqs.n_seqs <= 64; ++k) {
+                int items = work.tiles * seq_splits(a, work.last, unit);
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) items += __shfl_xor(items, o);
+                unit = fit_unit(a, unit, (float)items);
+            }
+        }
+        int tiles0 = 0, items0 = 0;
+        for (int b0 = 0; b0 < a.seqs.n_seqs && r.b < 0; b0 += 64) {
+            Seq s = mine;
+            SeqWork w = work;
+            if (b0 > 0) {
+                s = b0 + lane < a.seqs.n_seqs ? seq_of(a.seqs, b0 + lane) : Seq{};
+                w = seq_work(a, s, group);
+            }
+            const int n = w.tiles * a.kv_heads, c = seq_splits(a, w.last, unit);
             int tiles = n, items = n * c;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -289,8 +349,13 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
                 const int at = __shfl(items - n * c, l) + items0;
                 j = i - (whole ? __shfl(tiles - n, l) + tiles0 : at);
                 g = whole ? j : j / r.splits;
-                r.range = whole ? 0 : j % r.splits;
+                r.range = whole ? 0 : j - g * r.splits;
                 r.part = at + g * r.splits;
+                r.s.q0 = __shfl(s.q0, l);
+                r.s.nq = __shfl(s.nq, l);
+                r.s.kv0 = __shfl(s.kv0, l);
+                r.s.nk = __shfl(s.nk, l);
+                r.s.bad = __shfl((int)s.bad, l);
             }
             tiles0 += __shfl(tiles, 63);
             items0 += __shfl(items, 63);
@@ -298,9 +363,14 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
     }
     if (r.b < 0) return r;
     r.b = uniform(r.b);
-    r.kvh = uniform(g % a.kv_heads);
+    r.s.q0 = uniform(r.s.q0);
+    r.s.nq = uniform(r.s.nq);
+    r.s.kv0 = uniform(r.s.kv0);
+    r.s.nk = uniform(r.s.nk);
+    const int t = g / a.kv_heads;
+    r.kvh = uniform(g - t * a.kv_heads);
     // the last tiles of a causal sequence have the most keys: first
-    r.t = uniform(seq_tiles(seq_of(a.seqs, r.b), group) - 1 - g / a.kv_heads);
+    r.t = uniform(seq_tiles(r.s, group) - 1 - t);
     r.range = uniform(r.range);
     r.splits = uniform(r.splits);
     r.part = uniform(r.part);
@@ -362,9 +432,9 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     if (a.bad && blockIdx.x == 0 && wave == 0) report_seqs(a.seqs, a.bad);
 
     const TileItem it = find_item(a, group, blockIdx.x, false);
-    const int b = it.b, kvh = it.kvh;
+    const int b = uniform(it.b), kvh = uniform(it.kvh);
     if (b < 0) return;
-    Seq s = seq_of(a.seqs, b);
+    Seq s = it.s;
     s.q0 = uniform(s.q0), s.nq = uniform(s.nq), s.kv0 = uniform(s.kv0), s.nk = uniform(s.nk);
     const TileKeys tk = tile_keys(a, s, group, it.t);
     const TileRange tr = tile_range<D>(tk, it.splits, it.range);
@@ -375,14 +445,14 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     const int wrow = wave * 32 + l31;
     const int r = tk.r0 + min(wrow, tk.rows - 1);
     const bool mine = wrow < tk.rows;
-    const int token = s.q0 + r / group, head = kvh * group + r % group;
+    const int ri = div_group(a, r), token = s.q0 + ri, head = kvh * group + r - ri * group;
     int lo, hi;
-    visible(a, s, r / group, lo, hi);
+    visible(a, s, ri, lo, hi);
     // the wave's rows: keys that some see, keys that all see
     const bool wave_on = wave * 32 < tk.rows;
     int first_lo, first_hi, last_lo, last_hi;
-    visible(a, s, (tk.r0 + min(wave * 32, tk.rows - 1)) / group, first_lo, first_hi);
-    visible(a, s, (tk.r0 + min(wave * 32 + 31, tk.rows - 1)) / group, last_lo, last_hi);
+    visible(a, s, div_group(a, tk.r0 + min(wave * 32, tk.rows - 1)), first_lo, first_hi);
+    visible(a, s, div_group(a, tk.r0 + min(wave * 32 + 31, tk.rows - 1)), last_lo, last_hi);
     first_lo = uniform(first_lo), first_hi = uniform(first_hi), last_lo = uniform(last_lo), last_hi = uniform(last_hi);
 
     const uint16_t *qrow = a.q + token * a.q_row + head * a.q_head;
@@ -734,9 +804,10 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
     for (int r0 = 0; r0 < rows; r0 += kFewRows) {
         bool bad = s.bad;
         const int r = min(r0 + c, rows - 1);
-        const uint16_t *qrow = a.q + (s.q0 + r / group) * a.q_row + (kvh * group + r % group) * a.q_head;
+        const int ri = div_group(a, r);
+        const uint16_t *qrow = a.q + (s.q0 + ri) * a.q_row + (kvh * group + r - ri * group) * a.q_head;
         int lo, hi;
-        visible(a, s, r / group, lo, hi);
+        visible(a, s, ri, lo, hi);
         u32x4 qf[ST];
 #pragma unroll
         for (int i = 0; i < ST; ++i) qf[i] = *reinterpret_cast<const u32x4 *>(qrow + 32 * i + 8 * g);
@@ -840,7 +911,7 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
         const int row = threadIdx.x / 16, c0 = (threadIdx.x & 15) * E;
         const int rr = min(r0 + row, rows - 1);
         const bool mine = r0 + row < rows;
-        const int token = s.q0 + rr / group, head = kvh * group + rr % group;
+        const int rri = div_group(a, rr), token = s.q0 + rri, head = kvh * group + rr - rri * group;
         float acc[E];
         float M = kLowest, L = 0.f;
 #pragma unroll
@@ -865,7 +936,7 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
             for (int x = 8; x >= 1; x >>= 1) odd |= __shfl_xor(odd, x); // the row's threads alike
             if (odd) {
                 int rlo, rhi;
-                visible(a, s, rr / group, rlo, rhi);
+                visible(a, s, rri, rlo, rhi);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = 0.f;
                 row_fp32<BF, D, PAGED>(a, kr, vr, b, a.q + token * a.q_row + head * a.q_head, max(rlo, j0),
@@ -939,7 +1010,7 @@ __global__ __launch_bounds__(256) void b1_attn_tile_join_kernel(AttnArgs a) {
     const int group = a.heads / a.kv_heads;
     const TileItem it = find_item(a, group, blockIdx.x / (kRows / 16), true);
     if (it.b < 0) return;
-    const Seq s = seq_of(a.seqs, it.b);
+    const Seq &s = it.s;
     const TileKeys tk = tile_keys(a, s, group, it.t);
     const int ranges = tile_range<D>(tk, it.splits, 0).ranges;
     const int row = blockIdx.x % (kRows / 16) * 16 + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * E;
@@ -947,10 +1018,10 @@ __global__ __launch_bounds__(256) void b1_attn_tile_join_kernel(AttnArgs a) {
     // that overlap, which no plan counts)
     if (ranges <= 1 || row - (int)(threadIdx.x >> 4) >= tk.rows || it.part + ranges > a.items) return;
     const bool mine = row < tk.rows;
-    const int r = tk.r0 + min(row, tk.rows - 1);
+    const int r = tk.r0 + min(row, tk.rows - 1), ri = div_group(a, r);
     float o[E];
     join_ranges<E>(a.part_o, a.part_ml, (int64_t)it.part * kRows + min(row, tk.rows - 1), kRows, ranges, 0, 1, c0, o);
-    store_row<BF, D>(a, s.q0 + r / group, it.kvh * group + r % group, c0, o, mine);
+    store_row<BF, D>(a, s.q0 + ri, it.kvh * group + r - ri * group, c0, o, mine);
 }
 
 // Rows of the few-rows kernel: P groups of 16 lanes take a row, each every
@@ -1031,7 +1102,8 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     p.grid = p.tiles;
     if (!split) return p;
     if (p.tiles < slots) {
-        const int64_t s = std::min<int64_t>(most / kLeastKeys, 64);
+        // (up to 512 keys splitting never paid)
+        const int64_t s = most <= 512 ? 1 : std::min<int64_t>(most / kLeastKeys, 64);
         if (s > 1) {
             p.splits = (int)s;
             p.target = (int)slots;
@@ -1105,6 +1177,11 @@ hipError_t launch_attn(const AttnArgs &args, int num_cus, void *ws, size_t ws_by
     a.target = p.target;
     a.solo = p.solo;
     a.items = (int)(p.grid - p.solo);
+    // x / group by a multiplication (x < 2^31): s = ceil(log2 group), m =
+    // floor(2^32 (2^s - group) / group) + 1, x / group = (hi(x m) + x) >> s
+    const uint32_t group = (uint32_t)(a.heads / a.kv_heads);
+    while ((1u << a.div_s) < group) ++a.div_s;
+    a.div_m = (uint32_t)(((((uint64_t)1 << a.div_s) - group) << 32) / group) + 1;
     if (p.splits > 1) {
         const size_t rows = (size_t)part_rows(a, p);
         uint8_t *at = static_cast<uint8_t *>(ws);
