@@ -216,20 +216,29 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, i
 }
 __device__ __forceinline__ int seq_tiles(const Seq &s, int group) { return (s.nq * group + kRows - 1) / kRows; }
 
-// Into how many ranges a call's tiles are split: a fixed number each
-// (a.target 0), or so that all ranges of all sequences have about the same
-// number of keys and make about a.target work items, where that pays.
+// Sum over the wave.
+__device__ __forceinline__ int wave_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false); // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false); // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false); // row_bcast:31
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// Keys a range: a tile with more is split (into at most a.splits ranges), so
+// that no range outlasts the rest of the call.
 //
-// It does when the longest tile, alone with what shares its CU, takes longer
-// than everything at the rate of a full device and the partial sums' way out
-// and in.  In us at D = 128, measured: a 32-key step of a tile 0.72 with one
-// work-group a CU, 1.15 with two, 1.5 with three; a partial tile 0.026.
-// Split against whole (us): 128 tiles over 4096 keys 62 / 97, 8 over 4000
-// 27 / 96, 128 over 1000 31 / 32, 256 over 1024 (causal) 41 / 33, 480 over
-// 2560 126 / 99.
+// Splitting pays where the longest tile takes longer than everything at the
+// rate of a full device and the partial sums' way out and in.  In us at D =
+// 128, measured: a 32-key step of a tile 0.72 with one work-group a CU, 1.15
+// with two, 1.5 with three; a partial tile 0.026.  Split against whole (us):
+// 128 tiles over 4096 keys 59 / 104, 8 over 4000 24 / 102, 128 over 1000
+// 36 / 33, 256 over 1024 (causal) 41 / 33, 480 over 2560 126 / 97.
 struct SeqWork {
     int tiles;         // of a key head
-    float last, total; // keys of the last tile, of all of them
+    float last, total; // keys of the last tile (the most), of all of them
 };
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, const Seq &s, int group) {
     SeqWork w = {seq_tiles(s, group), 0.f, 0.f};
@@ -240,125 +249,178 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, const Seq &s, int
     }
     return w;
 }
-// Keys a range; 0: whole tiles.  `total`, `longest` and `tiles` over all
-// sequences.
-__device__ __forceinline__ float tile_unit(const AttnArgs &a, float total, float longest, float tiles) {
+constexpr int kWhole = INT_MAX / 2; // a unit that splits nothing
+// From the keys of all tiles, as they are and if each had its sequence's
+// most, the longest tile's, and the tiles (of a key head, all sequences).
+__device__ __forceinline__ int tile_unit(const AttnArgs &a, float total, float reach, float longest, float tiles) {
     total *= (float)a.kv_heads;
+    reach *= (float)a.kv_heads;
     tiles *= (float)a.kv_heads;
-    const float cus = (float)a.target * (1.f / TileShapeOf<128>::waves), scale = (float)a.head_dim * (1.f / 128);
+    const float target = (float)a.target;
+    const float cus = target * (a.head_dim == 256 ? 1.f / TileShapeOf<256>::waves : 1.f / TileShapeOf<128>::waves);
+    const float scale = (float)a.head_dim * (1.f / 128);
     const float whole = longest * (1.f / 32) * scale * (tiles <= cus ? 0.72f : tiles <= 2 * cus ? 1.15f : 1.5f);
-    const float parts = tiles + fminf((float)a.target, total * (1.f / kLeastKeys));
-    const float split = (total * (1.f / 32) * 1.7f / (float)a.target + 0.026f * parts) * scale + 8.f;
-    if (whole < 1.2f * split) return 0.f;
-    return fmaxf((float)kLeastKeys, total / (float)a.target + 1.f);
+    const float parts = tiles + fminf(target, total * (1.f / kLeastKeys));
+    const float split = (total * (1.f / 32) * 1.7f / target + 0.026f * parts) * scale + 8.f;
+    if (whole < 1.2f * split) return kWhole;
+    // (so that tiles x ceil(most keys / unit) <= tiles + target)
+    return (int)fminf(fmaxf((float)kLeastKeys, reach / target + 1.f), (float)kWhole);
 }
-// The unit that makes `items` (of a key head, at the unit so far) fit the
+__device__ __forceinline__ int key_ranges(const AttnArgs &a, int keys, int unit) {
+    return max(1, min(a.splits, (keys + unit - 1) / unit));
+}
+// The unit that makes the items (of a key head, at the unit so far) fit the
 // device at once: a few more than that would run after all others.
-__device__ __forceinline__ float fit_unit(const AttnArgs &a, float unit, float items) {
-    return unit * fmaxf(1.f, items * (float)a.kv_heads / (float)a.target);
-}
-__device__ __forceinline__ int seq_splits(const AttnArgs &a, float last, float unit) {
-    if (unit == 0.f) return 1;
-    return max(1, min(a.splits, (int)ceilf(last / unit)));
+__device__ __forceinline__ int fit_unit(const AttnArgs &a, int unit, int items) {
+    const float have = (float)items * (float)a.kv_heads;
+    return have <= (float)a.target ? unit : (int)((float)unit * have / (float)a.target) + 1;
 }
 
 // A work item: key head, row tile and range of one of the sequences.  The
-// first a.solo items are whole tiles (of the one sequence of such a call);
-// after them each tile is `splits` items in a row, whose partial sums are at
-// part .. part + splits - 1.
+// first a.solo items are whole tiles; behind them a sequence's n tiles (key
+// heads counted) have as many items as its longest has ranges, the tiles'
+// first ranges before their second ones: neighbouring items run on different
+// XCDs, and each is to have its share of those that have something to do.
+// The partial sums of range i of the tile are number part + i * apart.
 struct TileItem {
-    int b, kvh, t, range, splits, part;
+    int b, kvh, t, range, unit, part, apart;
     Seq s;
 };
 // Finds item i (or, of whole tiles, the i-th tile behind the solo ones), by
-// the whole wave; b = -1: none.
+// the whole wave; b = -1: none.  Unsplit tiles come in the order of their
+// keys, the most first, so that the last work-groups to start are short: of
+// up to 64 causal sequences by levels, the tile's place behind the keys
+// before the sequence's first token, counted in tiles.
 __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int i, bool whole) {
     TileItem r;
     const int lane = threadIdx.x & 63;
-    int j = i, g = 0;
     r.b = -1;
-    r.splits = 1;
     r.range = 0;
     r.part = 0;
+    r.apart = 1;
+    r.unit = kWhole;
     r.s = Seq{};
+    int t = 0;
     if (a.seqs.n_seqs == 1) {
         r.s = seq_of(a.seqs, 0);
-        if (a.solo == 0 && a.splits > 1) {
-            const SeqWork w = seq_work(a, r.s, group);
-            float unit = tile_unit(a, w.total, w.last, (float)w.tiles);
-            if (unit > 0.f) unit = fit_unit(a, unit, (float)(w.tiles * seq_splits(a, w.last, unit)));
-            r.splits = seq_splits(a, w.last, unit);
+        const SeqWork w = seq_work(a, r.s, group);
+        const int n = w.tiles * a.kv_heads;
+        int g = i;
+        if (whole || i >= a.solo) {
+            r.apart = n - a.solo;
+            if (a.solo > 0) {
+                r.unit = ((int)w.last + a.splits - 1) / a.splits;
+            } else if (a.splits > 1) {
+                r.unit = tile_unit(a, w.total, (float)w.tiles * w.last, w.last, (float)w.tiles);
+                if (r.unit < kWhole) r.unit = fit_unit(a, r.unit, w.tiles * key_ranges(a, (int)w.last, r.unit));
+            }
+            if (!whole) {
+                g -= a.solo;
+                r.range = r.apart > 0 ? g / r.apart : 0;
+                g -= r.range * r.apart;
+            }
+            r.part = g;
+            g += a.solo;
         }
-        if (!whole && i < a.solo) {
-            g = i;
-        } else {
-            if (a.solo > 0) r.splits = a.splits;
-            j = whole ? i : i - a.solo;
-            g = a.solo + (whole ? j : j / r.splits);
-            r.range = whole ? 0 : j - (g - a.solo) * r.splits;
-            r.part = (g - a.solo) * r.splits;
-        }
-        if (g < seq_tiles(r.s, group) * a.kv_heads) r.b = 0;
+        const int q = g / a.kv_heads;
+        r.kvh = g - q * a.kv_heads;
+        t = w.tiles - 1 - q;
+        if (t >= 0) r.b = 0;
     } else {
-        // the first 64 sequences stay in registers for both passes
+        // the first 64 sequences stay in registers
         const Seq mine = lane < a.seqs.n_seqs ? seq_of(a.seqs, lane) : Seq{};
         const SeqWork work = seq_work(a, mine, group);
-        float unit = 0.f;
         if (a.splits > 1) {
-            float total = work.total, longest = work.last, tiles = (float)work.tiles;
+            float total = work.total, reach = (float)work.tiles * work.last, longest = work.last;
+            int tiles = work.tiles;
             for (int b = 64 + lane; b < a.seqs.n_seqs; b += 64) {
                 const SeqWork w = seq_work(a, seq_of(a.seqs, b), group);
                 total += w.total;
+                reach += (float)w.tiles * w.last;
                 longest = fmaxf(longest, w.last);
-                tiles += (float)w.tiles;
+                tiles += w.tiles;
             }
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) {
                 total += __shfl_xor(total, o);
+                reach += __shfl_xor(reach, o);
                 longest = fmaxf(longest, __shfl_xor(longest, o));
-                tiles += __shfl_xor(tiles, o);
             }
-            unit = tile_unit(a, total, longest, tiles);
-            for (int k = 0; k < 2 && unit > 0.f && a.seqs.n_seqs <= 64; ++k) {
-                int items = work.tiles * seq_splits(a, work.last, unit);
+            tiles = wave_sum(tiles);
+            r.unit = tile_unit(a, total, reach, longest, (float)tiles);
+            for (int k = 0; k < 2 && r.unit < kWhole && a.seqs.n_seqs <= 64; ++k)
+                r.unit = fit_unit(a, r.unit, wave_sum(work.tiles * key_ranges(a, (int)work.last, r.unit)));
+        }
+        int l = -1;
+        Seq s = mine;
+        if (a.causal && a.splits == 1 && a.seqs.n_seqs <= 64) {
+            const int q = i / a.kv_heads;
+            r.kvh = i - q * a.kv_heads;
+            const int off = (int)(((int64_t)max(0, mine.nk - mine.nq) * group) / kRows);
+            // tiles at a level or above it
+            auto from = [&](int level) { return min(work.tiles, max(0, work.tiles - max(0, level - off))); };
+            if (wave_sum(work.tiles) > q) {
+                int top = work.tiles > 0 ? off + work.tiles : 0;
 #pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) items += __shfl_xor(items, o);
-                unit = fit_unit(a, unit, (float)items);
+                for (int o = 32; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o));
+                int low = 0, high = uniform(top); // the tile's level is in [low, high)
+                while (high - low > 1) {
+                    const int mid = (low + high) >> 1;
+                    if (wave_sum(from(mid)) > q)
+                        low = mid;
+                    else
+                        high = mid;
+                }
+                // the q-th tile is one of those at this level, a sequence's each
+                const bool here = from(low) > from(low + 1);
+                const int above = wave_sum(from(low + 1));
+                const uint64_t at = __ballot(here);
+                const bool it = here && __popcll(at & ((1ull << lane) - 1)) == q - above;
+                l = __builtin_ctzll(__ballot(it));
+                r.b = l;
+                t = __shfl(low - off, l);
+            }
+        } else {
+            int tiles0 = 0, items0 = 0;
+            for (int b0 = 0; b0 < a.seqs.n_seqs && r.b < 0; b0 += 64) {
+                SeqWork w = work;
+                if (b0 > 0) {
+                    s = b0 + lane < a.seqs.n_seqs ? seq_of(a.seqs, b0 + lane) : Seq{};
+                    w = seq_work(a, s, group);
+                }
+                const int n = w.tiles * a.kv_heads, c = key_ranges(a, (int)w.last, r.unit);
+                int tiles = n, items = n * c;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int x = __shfl_up(tiles, o), y = __shfl_up(items, o);
+                    if (lane >= o) tiles += x, items += y;
+                }
+                const uint64_t past = __ballot((whole ? tiles0 + tiles : items0 + items) > i);
+                if (past) {
+                    l = __builtin_ctzll(past);
+                    r.b = b0 + l;
+                    r.apart = __shfl(n, l);
+                    const int base = items0 + __shfl(items - n * c, l);
+                    int g = i - (whole ? tiles0 + __shfl(tiles - n, l) : base);
+                    if (!whole) {
+                        r.range = g / r.apart;
+                        g -= r.range * r.apart;
+                    }
+                    r.part = base + g;
+                    const int q = g / a.kv_heads;
+                    r.kvh = g - q * a.kv_heads;
+                    t = __shfl(w.tiles, l) - 1 - q;
+                }
+                tiles0 += __shfl(tiles, 63);
+                items0 += __shfl(items, 63);
             }
         }
-        int tiles0 = 0, items0 = 0;
-        for (int b0 = 0; b0 < a.seqs.n_seqs && r.b < 0; b0 += 64) {
-            Seq s = mine;
-            SeqWork w = work;
-            if (b0 > 0) {
-                s = b0 + lane < a.seqs.n_seqs ? seq_of(a.seqs, b0 + lane) : Seq{};
-                w = seq_work(a, s, group);
-            }
-            const int n = w.tiles * a.kv_heads, c = seq_splits(a, w.last, unit);
-            int tiles = n, items = n * c;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(tiles, o), y = __shfl_up(items, o);
-                if (lane >= o) tiles += x, items += y;
-            }
-            const uint64_t past = __ballot((whole ? tiles0 + tiles : items0 + items) > i);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                r.b = b0 + l;
-                r.splits = __shfl(c, l);
-                const int at = __shfl(items - n * c, l) + items0;
-                j = i - (whole ? __shfl(tiles - n, l) + tiles0 : at);
-                g = whole ? j : j / r.splits;
-                r.range = whole ? 0 : j - g * r.splits;
-                r.part = at + g * r.splits;
-                r.s.q0 = __shfl(s.q0, l);
-                r.s.nq = __shfl(s.nq, l);
-                r.s.kv0 = __shfl(s.kv0, l);
-                r.s.nk = __shfl(s.nk, l);
-                r.s.bad = __shfl((int)s.bad, l);
-            }
-            tiles0 += __shfl(tiles, 63);
-            items0 += __shfl(items, 63);
+        if (l >= 0) {
+            r.s.q0 = __shfl(s.q0, l);
+            r.s.nq = __shfl(s.nq, l);
+            r.s.kv0 = __shfl(s.kv0, l);
+            r.s.nk = __shfl(s.nk, l);
+            r.s.bad = __shfl((int)s.bad, l);
         }
     }
     if (r.b < 0) return r;
@@ -367,28 +429,28 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
     r.s.nq = uniform(r.s.nq);
     r.s.kv0 = uniform(r.s.kv0);
     r.s.nk = uniform(r.s.nk);
-    const int t = g / a.kv_heads;
-    r.kvh = uniform(g - t * a.kv_heads);
-    // the last tiles of a causal sequence have the most keys: first
-    r.t = uniform(seq_tiles(r.s, group) - 1 - t);
+    r.kvh = uniform(r.kvh);
+    r.t = uniform(t);
     r.range = uniform(r.range);
-    r.splits = uniform(r.splits);
     r.part = uniform(r.part);
+    r.apart = uniform(r.apart);
+    r.unit = uniform(r.unit);
     return r;
 }
-// The stages [t0, t1) of a range, and how many ranges the tile has.
+// The stages [t0, t1) of a tile's range, and how many ranges it has.
 struct TileRange {
     int t0, t1, ranges;
 };
 template <int D>
-__device__ __forceinline__ TileRange tile_range(const TileKeys &k, int splits, int range) {
+__device__ __forceinline__ TileRange tile_range(const AttnArgs &a, const TileKeys &k, const TileItem &it) {
     constexpr int KK = TileShapeOf<D>::keys;
-    const int first = k.k0 / KK, last = (k.k1 + KK - 1) / KK;
-    const int per = max(kLeastKeys / KK, (last - first + splits - 1) / splits);
+    const int first = k.k0 / KK, last = (k.k1 + KK - 1) / KK, n = last - first;
     TileRange r;
-    r.ranges = splits == 1 ? 1 : max(1, (last - first + per - 1) / per);
-    r.t0 = first + range * per;
-    r.t1 = r.ranges == 1 ? last : min(r.t0 + per, last);
+    r.ranges = key_ranges(a, k.k1 - k.k0, it.unit);
+    const int per = r.ranges == 1 ? n : (n + r.ranges - 1) / r.ranges;
+    if (r.ranges > 1) r.ranges = (n + per - 1) / per; // none empty
+    r.t0 = first + it.range * per;
+    r.t1 = min(r.t0 + per, last);
     return r;
 }
 
@@ -437,7 +499,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     Seq s = it.s;
     s.q0 = uniform(s.q0), s.nq = uniform(s.nq), s.kv0 = uniform(s.kv0), s.nk = uniform(s.nk);
     const TileKeys tk = tile_keys(a, s, group, it.t);
-    const TileRange tr = tile_range<D>(tk, it.splits, it.range);
+    const TileRange tr = tile_range<D>(a, tk, it);
     const int ranges = uniform(tr.ranges), t0 = uniform(tr.t0), t1 = uniform(tr.t1);
     if (it.range >= ranges) return;
 
@@ -632,7 +694,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     float inv = l == 0.f ? 0.f : 1.0f / l;
     // columns 32 i .. of the row: register e of half h = column 8 (e / 4) +
     // 4 h + e % 4
-    const int64_t part = (int64_t)(it.part + it.range) * kRows + wrow;
+    const int64_t part = ((int64_t)it.range * it.apart + it.part) * kRows + wrow;
     auto store = [&](int i, floatx16 v) __attribute__((always_inline)) {
         if (!mine) return;
         if (ranges > 1) {
@@ -1003,25 +1065,28 @@ __device__ __forceinline__ void join_ranges(const float *part_o, const float *pa
     }
 }
 
-// Rows of split tiles: a work-group takes 16 rows of one.
+// Rows of split tiles: W work-groups a tile, each every W-th 16 of its rows.
 template <bool BF, int D>
-__global__ __launch_bounds__(256) void b1_attn_tile_join_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void b1_attn_tile_join_kernel(AttnArgs a, int W) {
     constexpr int E = D / 16;
     const int group = a.heads / a.kv_heads;
-    const TileItem it = find_item(a, group, blockIdx.x / (kRows / 16), true);
+    const int tile = blockIdx.x / W;
+    const TileItem it = find_item(a, group, tile, true);
     if (it.b < 0) return;
     const Seq &s = it.s;
     const TileKeys tk = tile_keys(a, s, group, it.t);
-    const int ranges = tile_range<D>(tk, it.splits, 0).ranges;
-    const int row = blockIdx.x % (kRows / 16) * 16 + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * E;
-    // (whole work-groups; part sums past the launched items: of sequences
-    // that overlap, which no plan counts)
-    if (ranges <= 1 || row - (int)(threadIdx.x >> 4) >= tk.rows || it.part + ranges > a.items) return;
-    const bool mine = row < tk.rows;
-    const int r = tk.r0 + min(row, tk.rows - 1), ri = div_group(a, r);
-    float o[E];
-    join_ranges<E>(a.part_o, a.part_ml, (int64_t)it.part * kRows + min(row, tk.rows - 1), kRows, ranges, 0, 1, c0, o);
-    store_row<BF, D>(a, s.q0 + ri, it.kvh * group + r - ri * group, c0, o, mine);
+    const int ranges = tile_range<D>(a, tk, it).ranges, c0 = (threadIdx.x & 15) * E;
+    // (partial sums past the launched items: of sequences that overlap, which
+    // no plan counts)
+    if (ranges <= 1 || (int64_t)(ranges - 1) * it.apart + it.part >= a.items) return;
+    for (int r0 = (blockIdx.x - tile * W) * 16; r0 < tk.rows; r0 += W * 16) {
+        const int row = r0 + (threadIdx.x >> 4), there = min(row, tk.rows - 1);
+        const int r = tk.r0 + there, ri = div_group(a, r);
+        float o[E];
+        join_ranges<E>(a.part_o, a.part_ml, (int64_t)it.part * kRows + there, (int64_t)it.apart * kRows, ranges, 0, 1,
+                       c0, o);
+        store_row<BF, D>(a, s.q0 + ri, it.kvh * group + r - ri * group, c0, o, row < tk.rows);
+    }
 }
 
 // Rows of the few-rows kernel: P groups of 16 lanes take a row, each every
@@ -1075,10 +1140,9 @@ struct AttnPlan {
 };
 
 // Calls whose sequences have up to 16 rows a key head on average run the
-// few-rows kernel, which splits their keys into about 4 work-groups a CU.
-// Tiles: fewer of them than fit the device at once are split so that they
-// fill it; of more equal ones (one sequence, every key seen) the part of the
-// last round that would leave most of the device idle.
+// few-rows kernel, others tiles.  Tiles of few rounds of the device are split
+// where that pays; of more equal ones (one sequence, every key seen) the part
+// of the last round that would leave most of the device idle.
 AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     AttnPlan p{};
     const int group = a.heads / a.kv_heads;
@@ -1088,7 +1152,12 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     p.few = rows <= kFewRows * n;
     p.splits = 1;
     if (p.few) {
-        const int64_t step = kFewKeys * kWaves, units = n * a.kv_heads, target = 4 * num_cus;
+        // Two work-groups a CU fit.  Where the sequences themselves make few,
+        // exactly those (32 heads over 32700 keys: 38 us, 45 with 4 a CU);
+        // else small pieces, so that none outlasts the rest (64 sequences of
+        // 60 to 8100 keys: 215 us, 245 with 2).
+        const int64_t step = kFewKeys * kWaves, units = n * a.kv_heads;
+        const int64_t target = (units <= num_cus ? 2 : 6) * num_cus;
         int64_t s = std::min<int64_t>({4 * ((target + units - 1) / units), 256, (most + step - 1) / step});
         // partial results no larger than 1 GiB
         s = std::min(s, ((int64_t)1 << 30) / ((int64_t)a.seqs.tokens * a.heads * (a.head_dim + 2) * 4));
@@ -1100,17 +1169,9 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     const int64_t slots = (int64_t)num_cus * (a.head_dim == 256 ? TileShapeOf<256>::waves : TileShapeOf<128>::waves);
     p.tiles = (n == 1 ? (rows + kRows - 1) / kRows : rows / kRows + n) * a.kv_heads;
     p.grid = p.tiles;
-    if (!split) return p;
-    if (p.tiles < slots) {
-        // (up to 512 keys splitting never paid)
-        const int64_t s = most <= 512 ? 1 : std::min<int64_t>(most / kLeastKeys, 64);
-        if (s > 1) {
-            p.splits = (int)s;
-            p.target = (int)slots;
-            // tiles x ceil(keys / unit) <= tiles + slots
-            p.grid = std::min(p.tiles * s, p.tiles + slots + 1);
-        }
-    } else if (n == 1 && !a.causal) {
+    if (!split || most <= 2 * kLeastKeys) return p;
+    if (p.tiles >= slots && n == 1 && !a.causal) {
+        // equal tiles: the last round's
         const int64_t rest = p.tiles % slots;
         const int64_t s = rest ? std::min<int64_t>(slots / rest, most / (2 * kLeastKeys)) : 1;
         if (s > 1) {
@@ -1119,6 +1180,10 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
             p.tiles = rest;
             p.grid = p.solo + rest * s;
         }
+    } else if (p.tiles < slots) { // the kernel decides
+        p.splits = (int)std::min<int64_t>(most / kLeastKeys, 64);
+        p.target = (int)slots;
+        p.grid = std::min(p.tiles * p.splits, p.tiles + slots + 1);
     }
     return p;
 }
@@ -1154,8 +1219,12 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
     const int64_t rows = (int64_t)a.seqs.tokens * a.heads;
-    if (!p.few)
-        hipLaunchKernelGGL((b1_attn_tile_join_kernel<BF, D>), dim3(p.tiles * (kRows / 16)), block, 0, s, a);
+    if (!p.few) {
+        // (where the kernel decided against splitting, a join only finds that
+        // out: few work-groups)
+        const int w = p.solo > 0 || p.tiles < 256 ? kRows / 16 : 2;
+        hipLaunchKernelGGL((b1_attn_tile_join_kernel<BF, D>), dim3(p.tiles * w), block, 0, s, a, w);
+    }
     else if (p.splits <= 4)
         hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 1>), dim3((rows + 15) / 16), block, 0, s, a);
     else if (p.splits <= 16)

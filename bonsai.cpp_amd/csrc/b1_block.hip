@@ -228,7 +228,9 @@ hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_
 
 hipError_t launch_qkv(const QkvArgs &a, hipStream_t s) {
     const int all = a.heads + 2 * a.kv_heads, round = 1024 / a.head_dim; // heads a pass of a work-group
-    const int per = (all + round - 1) / round * round;
+    // all of a token's heads to a work-group, or one pass where the tokens
+    // alone would leave CUs idle
+    const int per = a.tokens < 1024 ? round : (all + round - 1) / round * round;
     const dim3 grid(a.tokens, (all + per - 1) / per);
     auto run = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, per);
