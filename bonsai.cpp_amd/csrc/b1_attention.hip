@@ -171,8 +171,8 @@ constexpr int kRows = 128;
 // Keys in LDS at a time (a stage), and waves a SIMD, by head dim.
 template <int D>
 struct TileShapeOf {
-    static constexpr int keys = D == 64 ? 64 : 32;
-    static constexpr int waves = D == 256 ? 2 : 3;
+    static constexpr int keys = D == 128 ? 32 : 64;
+    static constexpr int waves = D == 256 ? 1 : 3;
     static constexpr int stages = D == 256 ? 2 : 3; // in LDS
 };
 // A range of a split tile has at least this many keys, so that its fixed
@@ -478,6 +478,19 @@ __device__ __forceinline__ void copy_to_lds(u32x4 rsrc, uint8_t *lds, uint32_t o
                  : "memory");
 }
 
+// Order for the scheduler: the LDS reads (PER each) of AHEAD products, then N
+// products with a read PER each behind them while there are any.
+template <int AHEAD, int PER, int N>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * PER, 0); // LDS reads
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); // matrix instructions
+        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+}
+
 // Bound by the matrix units together with the vector instructions of the
 // softmax (a 32 x 32 block of scores is 8 products of 32 cycles at D = 128,
 // as many for the values, and about 80 vector instructions, 16 of them
@@ -579,6 +592,22 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
         }
     };
 
+    // this lane's places in a stage: chunk 2 i + h of key row l31, and its
+    // share of the value columns 32 dt .. of 4 keys.  Opaque, so that they
+    // stay one register each beside a constant offset.
+    uint32_t ka[ST], va[DT];
+#pragma unroll
+    for (int i = 0; i < ST; ++i) {
+        ka[i] = l31 * (D * 2) + (((2 * i + h) ^ swizzle_k<D>(l31)) << 4);
+        asm("" : "+v"(ka[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+        const int row = 4 * h + (lane & 15) / 4, chunk = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        va[i] = row * (D * 2) + ((chunk ^ swizzle_v<D>(row)) << 4) + (lane & 1) * 8;
+        asm("" : "+v"(va[i]));
+    }
+
     u32x4 qf[ST];
 #pragma unroll
     for (int i = 0; i < ST; ++i) qf[i] = *reinterpret_cast<const u32x4 *>(qrow + 16 * i + 8 * h);
@@ -620,14 +649,12 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
             sc[kt] = floatx16{};
-            const int row = kt * 32 + l31;
 #pragma unroll
-            for (int i = 0; i < ST; ++i) {
-                const u32x4 kf = *reinterpret_cast<const u32x4 *>(ks + row * (D * 2) +
-                                                                  (((2 * i + h) ^ swizzle_k<D>(row)) << 4));
-                sc[kt] = mfma32<BF>(kf, qf[i], sc[kt]);
-            }
+            for (int i = 0; i < ST; ++i)
+                sc[kt] = mfma32<BF>(*reinterpret_cast<const u32x4 *>(ks + 32 * kt * (D * 2) + ka[i]), qf[i], sc[kt]);
         }
+        // three reads ahead of the products (1.03 of the compiler's own order)
+        reads_ahead<3, 1, KT * ST>();
         if (kb + KK - 1 > first_hi || kb < last_lo) {
             const int top = hi - kb - 4 * h, bot = lo - kb - 4 * h;
 #pragma unroll
@@ -668,15 +695,14 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
                 pf[e] = pack_16<BF>(p0, p1);
                 l = add_pair<BF>(pf[e], l);
             }
-            const int row = 16 * x + 4 * h + (lane & 15) / 4;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-                const uint8_t *at = vs + row * (D * 2) + ((chunk ^ swizzle_v<D>(row)) << 4) + (lane & 1) * 8;
+                const uint8_t *at = vs + 16 * x * (D * 2) + va[dt];
                 const u32x2 y = read_columns(at), z = read_columns(at + 8 * (D * 2));
                 o[dt] = mfma32<BF>(u32x4{y[0], y[1], z[0], z[1]}, pf, o[dt]);
             }
         }
+        reads_ahead<2, 2, 2 * KT * DT>();
     };
     for (int tt = t0; tt < t1; tt += S) {
 #pragma unroll
