@@ -108,6 +108,50 @@ def test_attention(torch, b1, case):
         assert torch.equal(out, again)
 
 
+# Tiles: many sequences (past the 64 a wave holds at once), split and not;
+# sequences of unlike lengths split by the call's work
+MANY = [
+    ([20 + i % 31 for i in range(70)], None, 4, 1, 64, "fp16", True, 0, False),
+    ([17 + i % 40 for i in range(130)], None, 2, 1, 128, "bf16", False, 0, True),
+    ([20 + i % 9 for i in range(66)], [700 + 7 * i for i in range(66)], 2, 1, 64, "fp16", True, 0, True),
+    ([100, 9, 260], [1500, 2900, 260], 4, 2, 128, "fp16", True, 0, False),
+    ([60, 500, 33], [3000, 600, 40], 8, 4, 64, "bf16", True, 300, True),
+    ([129, 40], [2000, 1100], 2, 2, 256, "fp16", False, 0, False),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{len(c[0])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}-{c[6]}-{c[7]}")
+def test_many_and_unlike_sequences(torch, b1, case):
+    ql, kl, heads, kv_heads, d, t, causal, window, packed = case
+    say(f"many {case}")
+    dtype = dtype_of(torch, t)
+    kl = ql if kl is None else kl
+    q, k, v = make(torch, 41, ql, kl, heads, kv_heads, d, dtype)
+    want, off = expect(torch, q, k, v, ql, kl, d ** -0.5, causal, window)
+    out = b1.attention(q, k, v, i32(torch, ref.starts(ql)), i32(torch, ref.starts(kl)), causal=causal, window=window,
+                       packed=packed)
+    if packed:
+        ref.check(ref.unpack(out, sum(ql), heads * d).view(-1, heads, d), want, off, torch.float16, "packed")
+    else:
+        ref.check(out, want, off, dtype, "rows")
+
+
+@pytest.mark.parametrize("n,heads,d", [(2100, 48, 64), (1300, 72, 128)])
+def test_last_round_of_equal_tiles(torch, b1, n, heads, d):
+    """More equal tiles than the device holds at once, by a part of a round:
+    the last ones are split (on 256 CUs: 816 and 792 tiles of 768 places)."""
+    say(f"last round {n} {heads} {d}")
+    q, k, v = make(torch, 42, [n], [n], heads, heads, d, torch.float16)
+    out = b1.attention(q, k, v)
+    for h in (0, heads // 2, heads - 1):
+        want, off = ref.attention(q[:, h:h + 1].cpu(), k[:, h:h + 1].cpu(), v[:, h:h + 1].cpu(), d ** -0.5)
+        ref.check(out[:, h:h + 1], want, off, torch.float16, f"head {h}")
+    whole = b1.attention(q, k, v, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    # both within the bound of the exact value and a rounding of it: 2^-9 of
+    # the largest value bounds twice either with room
+    assert float((out.double() - whole.double()).abs().max()) <= 2.0 ** -9 * float(v.abs().max())
+
+
 PAGED = [
     # (query lengths, key lengths, heads, key heads, head dim, type, page size, order, window, packed)
     ([1], [1], 2, 1, 64, "fp16", 16, "head", 0, False),

@@ -140,7 +140,7 @@ def head_ref(torch, x, w, rope, interleaved, eps):
 
 
 @pytest.mark.parametrize("tokens,heads,kv_heads,d", [(1, 1, 1, 64), (5, 8, 2, 128), (3, 5, 5, 256), (70, 3, 1, 64),
-                                                     (33, 24, 24, 128)])
+                                                     (33, 24, 24, 128), (1100, 6, 2, 64)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("t", ["fp16", "bf16"])
 def test_qkv_rope(torch, b1, tokens, heads, kv_heads, d, interleaved, t):
