@@ -651,7 +651,7 @@ static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
     a->head_dim = g->head_dim;
     a->bf16 = g->dtype == BONSAI_B1_BF16;
     a->causal = g->causal != 0;
-    a->window = g->window;
+    a->window = std::min(g->window, 1 << 30); // as wide as any sequence is long
     a->scale = g->scale;
     a->out = static_cast<uint16_t *>(g->out);
     a->ldo = g->ldo;

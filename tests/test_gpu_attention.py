@@ -136,6 +136,17 @@ def test_many_and_unlike_sequences(torch, b1, case):
         ref.check(out, want, off, dtype, "rows")
 
 
+@pytest.mark.parametrize("ql,kl", [([150, 40], [20, 30]), ([6, 9], [2, 700])])
+def test_window_of_any_size(torch, b1, ql, kl):
+    """A window that no sequence fills is none, with tokens before the first key too."""
+    say(f"window {ql} {kl}")
+    q, k, v = make(torch, 43, ql, kl, 4, 2, 128, torch.float16)
+    want, off = expect(torch, q, k, v, ql, kl, 128 ** -0.5, True, 0)
+    for window in (2 ** 31 - 1, 2 ** 30 + 1, 1000):
+        out = b1.attention(q, k, v, i32(torch, ref.starts(ql)), i32(torch, ref.starts(kl)), causal=True, window=window)
+        ref.check(out, want, off, torch.float16, f"window {window}")
+
+
 @pytest.mark.parametrize("n,heads,d", [(2100, 48, 64), (1300, 72, 128)])
 def test_last_round_of_equal_tiles(torch, b1, n, heads, d):
     """More equal tiles than the device holds at once, by a part of a round:
