@@ -137,8 +137,10 @@ __global__ __launch_bounds__(256) void b1_qkv_kernel(QkvArgs a, int per) {
         if (b < 0) return; // a row of no sequence
         const Seq s = seq_of(a.seqs, b);
         pos = s.nk - s.nq + (token - s.q0);
-        bad = s.bad || pos < 0;
-        if (pos >= 0) {
+        // more tokens than places; starts that do not ascend, which can give a
+        // token to a sequence that does not hold it
+        bad = s.bad || pos < 0 || pos >= s.nk;
+        if (pos >= 0 && pos < s.nk) {
             const int page = page_of(a.seqs, b, pos, bad);
             kv_at = page * a.kv_page + (pos & ((1 << a.seqs.page_shift) - 1)) * a.kv_row;
         }

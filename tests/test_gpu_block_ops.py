@@ -227,6 +227,24 @@ def test_qkv_rope_bad_indexes(torch, b1):
         assert int((kc != 9).any(3).any(1).sum()) == int((~wrong).sum())
 
 
+def test_qkv_rope_starts_that_do_not_ascend(torch, b1):
+    """Tokens that such starts put behind their sequence's end are stored
+    nowhere: places past a table's row are not looked up."""
+    heads, d, page, n = 2, 64, 16, 24
+    x = normal(torch, 13, n, 3 * heads * d)
+    q, k, v = x.split([heads * d] * 3, 1)
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for at, kl in (([0, 20, 5, 6], [20, 5, 16]), ([0, 24, 2, 3, 3], [24, 7, 1, 32]), ([7, 2, 1, 24], [3, 3, 30])):
+        kc, vc = (torch.full((9, heads, page, d), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+        pages = torch.arange(2 * len(kl), dtype=torch.int32, device="cuda").view(len(kl), 2)
+        bad.zero_()
+        qo = b1.qkv_rope_paged(q, k, v, kc, vc, i32(torch, at), i32(torch, kl), pages, bad=bad)
+        assert int(bad) > 0
+        if at[1] == 20:  # tokens 6 .. 19: of sequence 2 by the ends, behind its one row
+            assert bool(qo[6:20].isnan().all()) and bool((kc[2:] == 9).all()) and bool((vc[2:] == 9).all())
+        assert bool((kc[8] == 9).all()) and bool((vc[8] == 9).all())
+
+
 def test_block_chain_whole_and_in_chunks(torch, b1):
     """A decoder block's attention half over prompts at once (contiguous keys)
     and in chunks and single tokens through a paged cache, both against
