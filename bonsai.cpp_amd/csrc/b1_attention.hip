@@ -309,7 +309,7 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
         if (whole || i >= a.solo) {
             r.apart = n - a.solo;
             if (a.solo > 0) {
-                r.unit = ((int)w.last + a.splits - 1) / a.splits;
+                r.unit = max(1, ((int)w.last + a.splits - 1) / a.splits);
             } else if (a.splits > 1) {
                 r.unit = tile_unit(a, w.total, (float)w.tiles * w.last, w.last, (float)w.tiles);
                 if (r.unit < kWhole) r.unit = fit_unit(a, r.unit, w.tiles * key_ranges(a, (int)w.last, r.unit));

@@ -163,6 +163,27 @@ def test_last_round_of_equal_tiles(torch, b1, n, heads, d):
     assert float((out.double() - whole.double()).abs().max()) <= 2.0 ** -9 * float(v.abs().max())
 
 
+@pytest.mark.parametrize("m", [0, 1, 700])
+@pytest.mark.parametrize("paged", [True, False])
+def test_last_round_of_equal_tiles_over_few_keys(torch, b1, m, paged):
+    """The same where the cache could hold more keys than the sequence has, or has none."""
+    say(f"last round {m} {paged}")
+    n, heads, d, page = 12800, 8, 64, 64
+    q, k, v = make(torch, 44, [n], [2048], heads, heads, d, torch.float16)
+    if paged:
+        kc, vc = (x.view(2048 // page, page, heads, d).transpose(1, 2) for x in (k, v))
+        pages = torch.arange(2048 // page, dtype=torch.int32, device="cuda")[None]
+        out = b1.attention_paged(q, kc, vc, None, i32(torch, [m]), pages, causal=False)
+    else:
+        out = b1.attention(q, k, v, i32(torch, [0, n]), i32(torch, [0, m]))
+    if m == 0:
+        assert bool((out == 0).all())
+        return
+    rows = torch.cat([torch.arange(0, 300), torch.arange(n - 300, n)]).cuda()
+    want, off = ref.attention(q[rows].cpu(), k[:m].cpu(), v[:m].cpu(), d ** -0.5)
+    ref.check(out[rows], want, off, torch.float16, "first and last rows")
+
+
 PAGED = [
     # (query lengths, key lengths, heads, key heads, head dim, type, page size, order, window, packed)
     ([1], [1], 2, 1, 64, "fp16", 16, "head", 0, False),
