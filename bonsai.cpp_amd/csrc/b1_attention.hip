@@ -356,7 +356,7 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
         if (a.causal && a.splits == 1 && a.seqs.n_seqs <= 64) {
             const int q = i / a.kv_heads;
             r.kvh = i - q * a.kv_heads;
-            const int off = (int)(((int64_t)max(0, mine.nk - mine.nq) * group) / kRows);
+            const int off = (int)min((int64_t)max(0, mine.nk - mine.nq) * group / kRows, (int64_t)1 << 29);
             // tiles at a level or above it
             auto from = [&](int level) { return min(work.tiles, max(0, work.tiles - max(0, level - off))); };
             if (wave_sum(work.tiles) > q) {

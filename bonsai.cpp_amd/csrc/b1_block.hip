@@ -3,6 +3,8 @@
 // rotary embedding and store.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "b1_seqs.h"
 
 namespace b1 {
@@ -217,10 +219,18 @@ hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_
                            const float *w, float eps, float *h, int64_t ldh, float *y, int64_t ldy, void *packed,
                            hipStream_t s) {
     uint32_t *pk = static_cast<uint32_t *>(packed);
+    // a launch has less than 2^32 threads
+    constexpr int most = 1 << 23;
     auto run = [&](auto kernel, int per) {
-        hipLaunchKernelGGL(kernel, dim3((rows + per - 1) / per), dim3(256), 0, s, x, ldx, add, lda, H, rows, w, eps,
-                           h, ldh, y, ldy, pk);
-        return hipGetLastError();
+        for (int64_t r0 = 0; r0 < rows; r0 += most) {
+            const int n = (int)std::min<int64_t>(most, rows - r0);
+            hipLaunchKernelGGL(kernel, dim3((n + per - 1) / per), dim3(256), 0, s, x + r0 * ldx, ldx,
+                               add ? add + r0 * lda : nullptr, lda, H, n, w, eps, h ? h + r0 * ldh : nullptr, ldh,
+                               y ? y + r0 * ldy : nullptr, ldy, pk ? pk + r0 * (H / 2) : nullptr);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
     };
     if (H <= 2048) return run(b1_rms_norm_kernel<64, 4>, 4);
     if (H <= 4096) return run(b1_rms_norm_kernel<256, 2>, 1);

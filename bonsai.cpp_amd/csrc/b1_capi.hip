@@ -492,13 +492,14 @@ int bonsai_b1_rms_norm_pack_f16(const float *x, int64_t ldx, const float *add, i
 }
 
 // Head layout and counts shared by the q/k/v and attention entries.  A
-// call's rows (tokens x heads) stay below 2^28, which keeps every index of a
-// row or work item in 32 bits and every grid within the launch limit.
+// call's rows (tokens x heads) stay below 2^28, tokens below 2^24, heads
+// below 2^16, which keeps every index of a row or work item in 32 bits and
+// every grid within the launch limits (2^32 threads, 2^16 in y).
 static bool heads_ok(int tokens, int heads, int kv_heads, int head_dim, int dtype) {
     if (tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return false;
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return false;
     if (dtype != BONSAI_B1_F16 && dtype != BONSAI_B1_BF16) return false;
-    return (int64_t)tokens * heads < (1 << 28) && heads < (1 << 20) && tokens < (1 << 24);
+    return (int64_t)tokens * heads < (1 << 28) && heads < (1 << 16) && tokens < (1 << 24);
 }
 
 static bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0 && s < ((int64_t)1 << 40); }
@@ -598,7 +599,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *g, hipStream_t stream) {
 // Checks an attention call and fills the kernels' arguments.
 static int attention_args(const bonsai_b1_attention_args *g, b1::AttnArgs *a) {
     if (!g || !heads_ok(g->tokens, g->heads, g->kv_heads, g->head_dim, g->dtype)) return BONSAI_B1_ERR_ARG;
-    if (g->n_seqs < 0 || g->n_seqs >= (1 << 24) || g->window < 0 || (g->window > 0 && !g->causal))
+    // (a sequence takes at least a work-group of 256 threads a key head)
+    if (g->n_seqs < 0 || (int64_t)g->n_seqs * g->kv_heads >= (1 << 23) || g->window < 0 || (g->window > 0 && !g->causal))
         return BONSAI_B1_ERR_ARG;
     if (!(g->scale > 0.f) || g->scale > 3.0e38f) return BONSAI_B1_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(g->q_start) | reinterpret_cast<uintptr_t>(g->kv_start) |

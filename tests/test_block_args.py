@@ -100,6 +100,16 @@ def test_attention(lib, change):
     assert lib.bonsai_b1_attention_workspace_bytes(ctypes.byref(a)) == 0
 
 
+@pytest.mark.parametrize("change", [
+    dict(tokens=1 << 24), dict(heads=1 << 16, kv_heads=1 << 16), dict(tokens=1 << 22, heads=64, kv_heads=8),
+    dict(n_seqs=1 << 22, q_start=P, kv_start=P), dict(n_seqs=1 << 30, q_start=P, kv_start=P), dict(kv_tokens=1 << 30),
+    dict(k_row=(1 << 23) + 8), dict(v_row=1 << 24)])
+def test_attention_too_large(lib, change):
+    a = attention(**change)
+    assert lib.bonsai_b1_attention(ctypes.byref(a), None, 0, None) == capi.ERR_ARG
+    assert lib.bonsai_b1_attention_workspace_bytes(ctypes.byref(a)) == 0
+
+
 def test_attention_misaligned_workspace(lib):
     assert lib.bonsai_b1_attention(ctypes.byref(attention()), P + 8, 1 << 20, None) == capi.ERR_ARG
     assert lib.bonsai_b1_attention(None, None, 0, None) == capi.ERR_ARG

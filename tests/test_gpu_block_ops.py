@@ -108,6 +108,18 @@ def test_rms_norm_of_zeros_and_odd_values(torch, b1):
     assert b1.rms_norm(x[:0]).shape == (0, 256)
 
 
+def test_rms_norm_of_more_rows_than_a_launch(torch, b1):
+    rows, h = (1 << 26) + 5, 32
+    x = torch.empty((rows, h), dtype=torch.float32, device="cuda")
+    some = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, (1 << 24) + 1, rows - 2, rows - 1], device="cuda")
+    x.fill_(1.0)
+    x[some] = normal(torch, 9, len(some), h)
+    packed = b1.rms_norm(x, None, 1e-6, packed=True)
+    want, off = norm_ref(torch, x[some], None, 1e-6)
+    got = packed.view(torch.float16).view(rows, h)[some].contiguous().view(torch.uint8).flatten()
+    ref.check(ref.unpack(got, len(some), h), want, off, torch.float16, "rows")
+
+
 def table(torch, rows, dim):
     angle = torch.arange(rows).double()[:, None] * 100.0 ** (-torch.arange(dim // 2).double() / max(1, dim // 2))
     return torch.cat([angle.cos(), angle.sin()], 1).float().cuda().contiguous()
