@@ -784,6 +784,8 @@ def _kv_pages(k_cache, v_cache, kv_len, pages, n_seqs):
     if pages.dtype is not _torch.int32 or pages.dim() != 2 or pages.shape[0] != n_seqs:
         raise ValueError(f"pages must be int32 [{n_seqs}, pages a sequence]")
     most = pages.shape[1]
+    if (n | most) >> 30:
+        raise ValueError("a cache and a sequence are limited to 2^30 pages")
     ld, unit = pages.stride()
     if unit != 1 and most > 1:
         raise ValueError("a sequence's pages must lie side by side")
@@ -911,9 +913,12 @@ def _attention(q, k, v, pages, kv_heads, q_start, kv_start, n_seqs, causal, wind
         k_p, v_p = k.data_ptr(), v.data_ptr()
     else:
         kv_p = ctypes.pointer(pages)
+    # (ctypes cuts integers to the field's width: the limits of the C entry)
+    if (tokens | n_seqs) >> 24 or kv_tokens >> 30 or window < 0:
+        raise ValueError("tokens and sequences are limited to 2^24, keys to 2^30, window is at least 0")
     args = AttentionArgs(q.data_ptr(), k_p, v_p, q_row, q_head, k_row, k_head, v_row, v_head, _dtype_code(q.dtype),
                          heads, kv_heads, d, tokens, kv_tokens, n_seqs, _i32_vector(q_start, None, "q_start"),
-                         _i32_vector(kv_start, n_seqs + 1, "kv_start"), kv_p, 1 if causal else 0, window,
+                         _i32_vector(kv_start, n_seqs + 1, "kv_start"), kv_p, 1 if causal else 0, min(window, 1 << 30),
                          scale if scale is not None else d ** -0.5, y.data_ptr(), ldo, form, _counter(bad))
     ws, wsb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None \
         else (None, 0)

@@ -142,9 +142,11 @@ def test_window_of_any_size(torch, b1, ql, kl):
     say(f"window {ql} {kl}")
     q, k, v = make(torch, 43, ql, kl, 4, 2, 128, torch.float16)
     want, off = expect(torch, q, k, v, ql, kl, 128 ** -0.5, True, 0)
-    for window in (2 ** 31 - 1, 2 ** 30 + 1, 1000):
+    for window in (2 ** 31 - 1, 2 ** 30 + 1, 1000, 2 ** 32 + 1, 2 ** 40):
         out = b1.attention(q, k, v, i32(torch, ref.starts(ql)), i32(torch, ref.starts(kl)), causal=True, window=window)
         ref.check(out, want, off, torch.float16, f"window {window}")
+    with pytest.raises(ValueError):
+        b1.attention(q, k, v, i32(torch, ref.starts(ql)), i32(torch, ref.starts(kl)), causal=True, window=-2 ** 32)
 
 
 @pytest.mark.parametrize("n,heads,d", [(2100, 48, 64), (1300, 72, 128)])
