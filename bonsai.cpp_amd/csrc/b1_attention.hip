@@ -793,19 +793,30 @@ __device__ __forceinline__ int few_len(const AttnArgs &a, const Seq &s, int &at)
     at = min(at, s.nk);
     return s.nk - at;
 }
-// Keys a range, from the lengths of all sequences (by the whole wave).
+// Keys a range, from the lengths of all sequences (by the whole wave).  None
+// is split where a CU's share of all keys is twice the longest's or more (64
+// sequences of 2000 keys, 8 key heads: 102 us, split 111; 100 of 60 to 4000
+// keys 188, split 161, and 64 of 60 to 8100 keys 268, split 217: their
+// longest is more than half a share).
 __device__ __forceinline__ int few_unit(const AttnArgs &a) {
     constexpr int step = kFewKeys * kWaves;
     if (a.splits == 1) return INT_MAX;
     const int lane = threadIdx.x & 63;
-    float total = 0.f; // a split size needs no more
+    float total = 0.f, longest = 0.f; // a split size needs no more
     for (int b = lane; b < a.seqs.n_seqs; b += 64) {
         int at;
-        total += (float)few_len(a, seq_of(a.seqs, b), at);
+        const float len = (float)few_len(a, seq_of(a.seqs, b), at);
+        total += len;
+        longest = fmaxf(longest, len);
     }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += __shfl_xor(total, o);
-    const int want = (int)fminf(total * (float)a.kv_heads / (float)a.target, 1.9e9f);
+    for (int o = 32; o >= 1; o >>= 1) {
+        total += __shfl_xor(total, o);
+        longest = fmaxf(longest, __shfl_xor(longest, o));
+    }
+    total *= (float)a.kv_heads;
+    if (2.f * longest * (float)a.cus <= total) return INT_MAX;
+    const int want = (int)fminf(total / (float)a.target, 1.9e9f);
     return (want / step + 1) * step;
 }
 __device__ __forceinline__ FewPlan few_plan(const AttnArgs &a, const Seq &s, int unit) {
@@ -860,6 +871,7 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
     // work item -> sequence and key range
     const int unit = few_unit(a);
     int b = -1, range = 0, run = 0;
+    if (a.splits == 1) b = item;
     for (int b0 = 0; b0 < a.seqs.n_seqs && b < 0; b0 += 64) {
         int n = 0;
         if (b0 + lane < a.seqs.n_seqs) n = few_plan(a, seq_of(a.seqs, b0 + lane), unit).ranges;
@@ -881,6 +893,7 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
     if (b < 0) return;
     const Seq s = seq_of(a.seqs, b);
     const FewPlan plan = few_plan(a, s, unit);
+    if (plan.ranges == 0) return; // no tokens
     const int j0 = plan.at + range * plan.keys, j1 = min(j0 + plan.keys, s.nk);
 
     const KeyRows kr = key_rows<PAGED>(a.k, a.k_page, a.k_row, a.k_head, kvh, s);
@@ -1181,8 +1194,13 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
         // Two work-groups a CU fit.  Where the sequences themselves make few,
         // exactly those (32 heads over 32700 keys: 38 us, 45 with 4 a CU);
         // else small pieces, so that none outlasts the rest (64 sequences of
-        // 60 to 8100 keys: 215 us, 245 with 2).
+        // 60 to 8100 keys: 215 us, 245 with 2).  Four rounds of whole sequences
+        // even out by themselves (256 of 60 to 4000 keys, 8 key heads: 379 us,
+        // split 393; 1024 of them 1413, 1543; 128 of them 225, 210), and with
+        // a work-group a CU short ones cost less than a join (33 of 500 keys:
+        // 20 us, split 32; of 2000 keys 52, 64, but of 60 to 4000 93, 73).
         const int64_t step = kFewKeys * kWaves, units = n * a.kv_heads;
+        split = split && units < 8 * num_cus && (units < num_cus || most > 1024);
         const int64_t target = (units <= num_cus ? 2 : 6) * num_cus;
         int64_t s = std::min<int64_t>({4 * ((target + units - 1) / units), 256, (most + step - 1) / step});
         // partial results no larger than 1 GiB
@@ -1271,6 +1289,7 @@ hipError_t launch_attn(const AttnArgs &args, int num_cus, void *ws, size_t ws_by
     a.splits = p.splits;
     a.target = p.target;
     a.solo = p.solo;
+    a.cus = num_cus;
     a.items = (int)(p.grid - p.solo);
     // x / group by a multiplication (x < 2^31): s = ceil(log2 group), m =
     // floor(2^32 (2^s - group) / group) + 1, x / group = (hi(x m) + x) >> s

@@ -236,6 +236,7 @@ struct AttnArgs {
     int target = 0;            // work items wanted; 0: exactly `splits` ranges
     int solo = 0;              // tiles that are not split, the first ones
     int items = 0;             // work items behind those
+    int cus = 0;               // of the device
     uint32_t div_m = 0, div_s = 0; // division by heads / kv_heads
     float *part_o = nullptr;   // partial sums of values [..][head_dim]
     float *part_ml = nullptr;  // their maxima (base 2) and sums of weights [..][2]

@@ -111,6 +111,10 @@ def test_attention(torch, b1, case):
 # Tiles: many sequences (past the 64 a wave holds at once), split and not;
 # sequences of unlike lengths split by the call's work
 MANY = [
+    # few rows: as many whole sequences as fill the device several times, some
+    # of them without tokens; whole by their equal lengths
+    ([i % 5 // 2 for i in range(300)], [30 + 7 * i for i in range(300)], 16, 8, 64, "fp16", True, 0, True),
+    ([1] * 80, [1200] * 80, 16, 8, 64, "bf16", True, 0, False),
     ([20 + i % 31 for i in range(70)], None, 4, 1, 64, "fp16", True, 0, False),
     ([17 + i % 40 for i in range(130)], None, 2, 1, 128, "bf16", False, 0, True),
     ([20 + i % 9 for i in range(66)], [700 + 7 * i for i in range(66)], 2, 1, 64, "fp16", True, 0, True),
