@@ -104,11 +104,6 @@ __device__ __forceinline__ void dma_lds4(const void *src, void *lds) {
     __builtin_amdgcn_global_load_lds(src, (lds_void_t *)lds, 4, 0, 0);
 }
 
-// The same, 16 bytes per lane, landing at lds + 16 * lane.
-__device__ __forceinline__ void dma_lds16(const void *src, void *lds) {
-    __builtin_amdgcn_global_load_lds(src, (lds_void_t *)lds, 16, 0, 0);
-}
-
 // Raw buffer loads with range checking (offsets at or past num_records read
 // zeros); word 3 of the resource for gfx9-family raw buffers.
 constexpr int kBufferFlags = 0x00020000;

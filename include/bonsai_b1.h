@@ -567,7 +567,8 @@ int bonsai_b1_swiglu_pack_f16_ld(const float *act, int64_t lda, int hidden,
  *   h = x + add,  y = h / sqrt(mean(h^2) + eps) * weight
  * over rows of H, in fp32.  add may be NULL (h = x); h is stored when `h` is
  * given, which may be x or add themselves (same row stride), and must not
- * overlap them otherwise.  weight may be NULL (1).  The _pack form writes
+ * overlap them otherwise; y and packed must not overlap the other arrays.
+ * weight may be NULL (1).  The _pack form writes
  * the packed fp16 activations of y that bonsai_b1_linear_packed_f16 reads
  * (row stride H; |y| beyond 65504 becomes +-inf there).  H % 32 == 0;
  * pointers 16-byte aligned, row strides multiples of 4.
@@ -592,9 +593,11 @@ enum { BONSAI_B1_F16 = 0, BONSAI_B1_BF16 = 1 };
  * j / page_size]; kv head h of row r of page p starts at element
  * p * page_stride + h * head_stride + r * row_stride of k and of v.
  * page_size: a power of two.  Strides: multiples of 8 elements; k and v
- * 16-byte aligned.  Sequence b has kv_len[b] keys, its new tokens among
- * them (they are its last ones).  Table entries behind a sequence's last
- * page are not read.  max_pages * page_size < 2^30.
+ * 16-byte aligned; rows, heads and pages apart from one another by at least
+ * head_dim.  Sequence b has kv_len[b] keys, its new tokens among them (they
+ * are its last ones).  Table entries behind a sequence's last page are not
+ * read; sequences may share pages that a call only reads.  max_pages *
+ * page_size < 2^30, page_size * row_stride < 2^30.
  */
 typedef struct bonsai_b1_kv_pages {
     void *k, *v;          /* device */
@@ -633,7 +636,8 @@ typedef struct bonsai_b1_kv_pages {
  * same place in memory (pages that two sequences share).
  * head_dim 64, 128 or 256; fp32 pointers 16-byte aligned, row strides
  * multiples of 4; 16-bit pointers 16-byte aligned, strides multiples of 8;
- * rope_dim a multiple of 8, <= head_dim.  The reference computes these as
+ * rope_dim a multiple of 8, <= head_dim; tokens < 2^24, heads < 2^16, tokens
+ * * heads < 2^28; outputs apart from the inputs.  The reference computes these as
  * separate ggml ops on q and k (src/diffuser_graph.cpp:354-406 and
  * src/b1_0_kernel.h:309-361, interleaved).
  */
@@ -667,8 +671,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * are rows kv_start[b] .. of k and v (NULL: all kv_tokens), or, with pages,
  * its places in the cache.  With n tokens and m keys, causal token i sees
  * keys 0 .. m - n + i, and with window > 0 (causal only) the last `window`
- * of those; a token that sees none gets zeros.  Masked and absent keys do
- * not reach the output, whatever they hold.  Rows of no sequence are left as
+ * of those; a token that sees none, or whose scores are all -inf, gets
+ * zeros.  Masked and absent keys do not reach the output, whatever they hold.  Rows of no sequence are left as
  * they were.
  * Scores and sums are fp32; softmax weights are rounded to the inputs' type
  * for the product with v.  out: rows of heads * head_dim in the inputs' type
@@ -678,12 +682,17 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * ggml_flash_attn_ext feeds its output projections
  * (src/diffuser_graph.cpp:406-441,509-536).
  * head_dim 64, 128 or 256; pointers 16-byte aligned; strides in elements,
- * multiples of 8; scale > 0; out apart from the inputs.
+ * multiples of 8; scale > 0; out apart from the inputs.  Query strides may
+ * be 0, rows of several keys lie head_dim to 2^23 elements apart; tokens <
+ * 2^24, heads < 2^16, tokens * heads < 2^28, n_seqs * kv_heads < 2^23,
+ * kv_tokens < 2^30.
  * workspace: bonsai_b1_attention_workspace_bytes(args) bytes (16-byte
  * aligned) for calls whose keys are split over work-groups, or NULL for the
- * library's per-stream workspace.  Without one (a capture never allocates)
- * the call runs unsplit: the same values up to the order of fp32 sums,
- * slower for few rows over many keys.
+ * library's per-stream workspace, with the rules of bonsai_b1_linear_f32's
+ * for captures.  Without one (a capture never allocates) the call runs
+ * unsplit: the same values up to the order of fp32 sums, slower for few rows
+ * over many keys.  A workspace serves one call at a time: give graphs that
+ * may be replayed at once one each.
  */
 typedef struct bonsai_b1_attention_args {
     const void *q, *k, *v; /* k, v unused with pages */

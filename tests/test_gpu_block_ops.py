@@ -321,3 +321,59 @@ def test_block_chain_whole_and_in_chunks(torch, b1):
     err = float((got - y).double().norm() / (y - x).double().norm())
     say(f"chunks against whole prompts: {err:.2e}")
     assert err < 0.02
+
+
+def test_captured_decode_step(torch, b1):
+    """One step of several sequences over a paged cache captured once and
+    replayed while the lengths in device memory grow, with eager work between
+    the replays; the sequences share the pages of a common prefix."""
+    from bonsai_b1 import synth
+    hidden, heads, kv_heads, d, page, n = 768, 12, 3, 64, 16, 3  # the linears read multiples of 384
+    width = (heads + 2 * kv_heads) * d
+    x = normal(torch, 30, n, hidden)
+    w_norm = 1.0 + normal(torch, 31, hidden, spread=0.2)
+    wqkv, wo = synth.device_packed_weights(width, hidden, 32), synth.device_packed_weights(hidden, heads * d, 33)
+    rope = table(torch, 2048, d)
+    split = [heads * d, kv_heads * d, kv_heads * d]
+    prefix, most = 60, 80  # pages; 960 shared keys
+    pages = torch.empty(n, most, dtype=torch.int32)
+    pages[:, :prefix] = torch.arange(prefix)
+    for b in range(n):
+        pages[b, prefix:] = prefix + b * (most - prefix) + torch.arange(most - prefix).flip(0)
+    pages = pages.cuda()
+    total = prefix + n * (most - prefix)
+    kc, vc = (normal(torch, s, total, kv_heads, page, d).half() for s in (34, 35))
+    start, first = i32(torch, [0, 1, 2, 3]), [960, 975, 1100]
+    lens = i32(torch, [m + 1 for m in first])
+
+    def step(k_cache, v_cache, ws):
+        h, packed = b1.rms_norm(x, w_norm, add=x, packed=True)
+        q, k, v = b1.linear_packed_f16(packed, wqkv, hidden, width, n).split(split, 1)
+        q16 = b1.qkv_rope_paged(q, k, v, k_cache, v_cache, start, lens, pages, rope=rope)
+        out = b1.attention_paged(q16, k_cache, v_cache, start, lens, pages, packed=True, workspace=ws)
+        return h, b1.linear_packed_f16(out, wo, heads * d, hidden, n)
+
+    ws, ws2 = (torch.empty(64 << 20, dtype=torch.uint8, device="cuda") for _ in range(2))
+    kg, vg, ke, ve = kc.clone(), vc.clone(), kc.clone(), vc.clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(kc, vc, ws)  # what the library allocates once
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            h, y = step(kg, vg, ws)
+        for turn in range(5):
+            graph.replay()
+            stream.synchronize()
+            he, ye = step(ke, ve, ws2)
+            stream.synchronize()
+            assert bool(ye.isfinite().all()), f"step {turn}"
+            assert torch.equal(h, he) and torch.equal(y, ye), f"step {turn}"
+            assert torch.equal(kg, ke) and torch.equal(vg, ve), f"step {turn}"
+            lens += 1
+            x.mul_(0.75)
+        stream.synchronize()
+    # the shared pages are as they were, the steps' places are not
+    assert torch.equal(kg[:prefix], kc[:prefix]) and not torch.equal(kg[prefix:], kc[prefix:])
+    del graph
