@@ -1077,11 +1077,29 @@ template <int E>
 __device__ __forceinline__ void join_ranges(const float *part_o, const float *part_ml, int64_t row, int64_t apart,
                                             int ranges, int first, int step, int c0, float (&o)[E]) {
     const int lane16 = threadIdx.x & 15;
-    float M = kLowest, L = 0.f;
-    for (int i = lane16; i < ranges; i += 16) M = fmaxf(M, part_ml[2 * (row + i * apart)]);
+    auto sums = [&](int i, int c) {
+        return *reinterpret_cast<const floatx4 *>(part_o + (row + i * apart) * (16 * E) + c0 + c);
+    };
+    // the first sums are on their way while the maxima are joined
+    constexpr int PRE = 4;
+    floatx4 pre[PRE][E / 4];
+#pragma unroll
+    for (int k = 0; k < PRE; ++k)
+#pragma unroll
+        for (int c = 0; c < E / 4; ++c) {
+            pre[k][c] = floatx4{};
+            if (first + k * step < ranges) pre[k][c] = sums(first + k * step, 4 * c);
+        }
+    // lane i: range i, i + 16, ..
+    const float2v none = {kLowest, 0.f};
+    const float2v mine =
+        lane16 < ranges ? *reinterpret_cast<const float2v *>(part_ml + 2 * (row + lane16 * apart)) : none;
+    float M = mine[0];
+    for (int i = lane16 + 16; i < ranges; i += 16) M = fmaxf(M, part_ml[2 * (row + i * apart)]);
 #pragma unroll
     for (int x = 8; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
-    for (int i = lane16; i < ranges; i += 16) {
+    float L = __builtin_amdgcn_exp2f(mine[0] - M) * mine[1];
+    for (int i = lane16 + 16; i < ranges; i += 16) {
         const float2v ml = *reinterpret_cast<const float2v *>(part_ml + 2 * (row + i * apart));
         L += __builtin_amdgcn_exp2f(ml[0] - M) * ml[1];
     }
@@ -1091,16 +1109,26 @@ __device__ __forceinline__ void join_ranges(const float *part_o, const float *pa
     const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.f;
+    auto add = [&](float m, floatx4 v, int c) {
+        const float f = __builtin_amdgcn_exp2f(m - M) * inv;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[4 * c + k] += f * v[k];
+    };
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) {
+        const int i = first + k * step;
+        const float m = i < 16       ? __shfl(mine[0], (threadIdx.x & 48) + (i & 15))
+                        : i < ranges ? part_ml[2 * (row + i * apart)]
+                                     : 0.f;
+        if (i < ranges)
+#pragma unroll
+            for (int c = 0; c < E / 4; ++c) add(m, pre[k][c], c);
+    }
 #pragma unroll 4
-    for (int i = first; i < ranges; i += step) {
-        const int64_t at = row + i * apart;
-        const float f = __builtin_amdgcn_exp2f(part_ml[2 * at] - M) * inv;
+    for (int i = first + PRE * step; i < ranges; i += step) {
+        const float m = part_ml[2 * (row + i * apart)];
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const floatx4 v = *reinterpret_cast<const floatx4 *>(part_o + at * (16 * E) + c0 + e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[e + k] += f * v[k];
-        }
+        for (int c = 0; c < E / 4; ++c) add(m, sums(i, 4 * c), c);
     }
 }
 
