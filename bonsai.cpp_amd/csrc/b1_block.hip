@@ -21,19 +21,22 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // y = h / sqrt(mean(h^2) + eps) * w over rows of h = x + add.
 //
 // Bound by HBM: x, add and h at 4 bytes a value, y at 4 or (packed) 2, so a
-// row is read once and kept in registers between the sum and the scaling.
-// T threads take a row, U units of 8 values each (4 + 4 values 16 columns
-// apart: the halves of a packed word quad); U = 0 reads wider rows twice.
-// The sum is fp32, at most 8 U values a thread and then a tree.
+// row is read once and kept in registers between the sum and the scaling
+// (8192 rows of 4096 with add: 86 us, 5.4 TB/s).
+// T threads take a row (a work-group has 256 threads or T), U units of 8
+// values each (4 + 4 values 16 columns apart: the halves of a packed word
+// quad); U = 0 reads wider rows twice.  The sum is fp32, at most 8 U values a
+// thread and then a tree.
 template <int T, int U>
-__global__ __launch_bounds__(256) void b1_rms_norm_kernel(const float *x, int64_t ldx, const float *add, int64_t lda,
+__global__ __launch_bounds__(T < 256 ? 256 : T) void b1_rms_norm_kernel(const float *x, int64_t ldx, const float *add, int64_t lda,
                                                           int H, int rows, const float *__restrict__ w, float eps,
                                                           float *h, int64_t ldh, float *__restrict__ y, int64_t ldy,
                                                           uint32_t *__restrict__ packed) {
-    __shared__ float part[4];
+    constexpr int ROWS = T < 256 ? 256 / T : 1; // a work-group
+    __shared__ float part[T / 64];
     const int t = threadIdx.x % T;
-    const int row = blockIdx.x * (256 / T) + threadIdx.x / T;
-    if (T == 64 && row >= rows) return; // whole wave; T = 256 has a row a work-group
+    const int row = blockIdx.x * ROWS + threadIdx.x / T;
+    if (T == 64 && row >= rows) return; // whole wave; others have a row a work-group
     const float *xr = x + (size_t)row * ldx;
     const float *ar = add ? add + (size_t)row * lda : nullptr;
     float *hr = h ? h + (size_t)row * ldh : nullptr;
@@ -47,10 +50,10 @@ __global__ __launch_bounds__(256) void b1_rms_norm_kernel(const float *x, int64_
     auto squares = [](floatx4 v) { return (v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3]); };
     auto total = [&](float s) {
         s = lanes_sum<64>(s);
-        if constexpr (T == 256) {
+        if constexpr (T > 64) {
             if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
             __syncthreads();
-            s = (part[0] + part[1]) + (part[2] + part[3]);
+            s = lanes_sum<T / 64>(part[threadIdx.x & (T / 64 - 1)]);
         }
         return 1.0f / sqrtf(s / (float)H + eps);
     };
@@ -221,10 +224,10 @@ hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_
     uint32_t *pk = static_cast<uint32_t *>(packed);
     // a launch has less than 2^32 threads
     constexpr int most = 1 << 23;
-    auto run = [&](auto kernel, int per) {
+    auto run = [&](auto kernel, int per, int threads) {
         for (int64_t r0 = 0; r0 < rows; r0 += most) {
             const int n = (int)std::min<int64_t>(most, rows - r0);
-            hipLaunchKernelGGL(kernel, dim3((n + per - 1) / per), dim3(256), 0, s, x + r0 * ldx, ldx,
+            hipLaunchKernelGGL(kernel, dim3((n + per - 1) / per), dim3(threads), 0, s, x + r0 * ldx, ldx,
                                add ? add + r0 * lda : nullptr, lda, H, n, w, eps, h ? h + r0 * ldh : nullptr, ldh,
                                y ? y + r0 * ldy : nullptr, ldy, pk ? pk + r0 * (H / 2) : nullptr);
             const hipError_t e = hipGetLastError();
@@ -232,17 +235,29 @@ hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_
         }
         return hipSuccess;
     };
-    if (H <= 2048) return run(b1_rms_norm_kernel<64, 4>, 4);
-    if (H <= 4096) return run(b1_rms_norm_kernel<256, 2>, 1);
-    if (H <= 16384) return run(b1_rms_norm_kernel<256, 8>, 1);
-    return run(b1_rms_norm_kernel<256, 0>, 1);
+    // Few units a thread and as many threads as that takes: all of a row's
+    // loads are on their way at once, with few registers held.  Measured (us
+    // of a norm of x + add into h and packed): 32768 x 512 40.7 (256 threads
+    // a row 47.3), 8192 x 2048 41.2 (a wave a row 50.8), 8192 x 4096 86.4
+    // (256 threads 93.8), 4096 x 8192 88.0 (512 threads 94.9, 256 98.3),
+    // 2048 x 16384 96.8 = 4.9 TB/s (256 threads 117), 2048 x 32768 188 (row
+    // read twice 303).
+    if (H <= 512) return run(b1_rms_norm_kernel<64, 1>, 4, 256);
+    if (H <= 2048) return run(b1_rms_norm_kernel<256, 1>, 1, 256);
+    if (H <= 4096) return run(b1_rms_norm_kernel<512, 1>, 1, 512);
+    if (H <= 8192) return run(b1_rms_norm_kernel<1024, 1>, 1, 1024);
+    if (H <= 16384) return run(b1_rms_norm_kernel<1024, 2>, 1, 1024);
+    if (H <= 32768) return run(b1_rms_norm_kernel<1024, 4>, 1, 1024);
+    return run(b1_rms_norm_kernel<1024, 0>, 1, 1024);
 }
 
 hipError_t launch_qkv(const QkvArgs &a, hipStream_t s) {
     const int all = a.heads + 2 * a.kv_heads, round = 1024 / a.head_dim; // heads a pass of a work-group
-    // all of a token's heads to a work-group, or one pass where the tokens
-    // alone would leave CUs idle
-    const int per = a.tokens < 1024 ? round : (all + round - 1) / round * round;
+    // all of a token's heads to a work-group (4608 tokens of 72 heads 50 us,
+    // 4.9 TB/s; a pass of heads each 75), or one pass where the tokens alone
+    // would leave CUs idle (64 tokens of 48 heads 3.9 us, all of them 6.8;
+    // 640 tokens 9.0 and 9.7, 768 tokens 10.1 and 9.7)
+    const int per = a.tokens < 700 ? round : (all + round - 1) / round * round;
     const dim3 grid(a.tokens, (all + per - 1) / per);
     auto run = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, per);

@@ -54,7 +54,8 @@ def norm_ref(torch, h, w, eps):
 
 
 @pytest.mark.parametrize("rows,h", [(1, 32), (5, 96), (3, 2048), (2, 2080), (7, 2560), (4, 4096), (3, 4128),
-                                    (300, 1024), (2, 16384), (3, 16416), (2, 20000)])
+                                    (300, 1024), (2, 16384), (3, 16416), (2, 20000), (9, 512), (5, 544), (3, 8192), (2, 8224),
+                                    (2, 32768), (3, 32800), (2, 70016)])
 @pytest.mark.parametrize("with_add", [True, False])
 def test_rms_norm(torch, b1, rows, h, with_add):
     say(f"rms_norm {rows} {h} {with_add}")
@@ -78,7 +79,7 @@ def test_rms_norm(torch, b1, rows, h, with_add):
     ref.check(bare, want, off, torch.float32, "no weight")
 
 
-@pytest.mark.parametrize("h", [64, 2560, 20000])
+@pytest.mark.parametrize("h", [64, 2560, 20000, 40000])
 @pytest.mark.parametrize("into", ["x", "add"])
 def test_rms_norm_in_place_and_strided(torch, b1, h, into):
     rows = 37
