@@ -18,7 +18,6 @@
 namespace b1 {
 namespace {
 
-
 // Below every score, and finite: a masked score is -inf, and -inf minus this
 // is -inf (weight 0), where -inf - -inf would be NaN.
 constexpr float kLowest = -3.4028235e38f;
@@ -168,7 +167,12 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // ---- tiles of 128 rows ------------------------------------------------------
 
 constexpr int kRows = 128;
-// Keys in LDS at a time (a stage), and waves a SIMD, by head dim.
+// Keys in LDS at a time (a stage), waves a SIMD (= work-groups a CU) and
+// stages in LDS, by head dim.  Three work-groups hide one another's waits:
+// at D = 128 that takes stages of 32 keys (4608 tokens x 24 heads 299 us, of
+// 64 keys and two work-groups 310; 4096 causal tokens x 32 heads 156, 167);
+// at D = 64 stages of 64 fit too (168, 179 of 32 keys).  At D = 256 the
+// registers of a row's sums leave one: 690 TFLOP/s, 520 of two that spill.
 template <int D>
 struct TileShapeOf {
     static constexpr int keys = D == 128 ? 32 : 64;
@@ -491,11 +495,20 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
 }
 
+// One pass over the keys: S^T = K Q^T by 32x32x16 products leaves a lane the
+// scores of one row, whose maximum and sum then need one exchange between the
+// wave's halves; O^T += V^T P^T takes the weights in the registers and the key
+// order they are in.  Four waves of 32 rows share a stage's keys and values.
+//
 // Bound by the matrix units together with the vector instructions of the
 // softmax (a 32 x 32 block of scores is 8 products of 32 cycles at D = 128,
 // as many for the values, and about 80 vector instructions, 16 of them
 // exponentials), and by how well three independent work-groups a CU hide one
-// another's LDS reads, barriers and copies.
+// another's LDS reads, barriers and copies.  Left out in turn at D = 128, 8192
+// tokens (1103 us, 1.0 PFLOP/s): reads of keys 21 %, softmax 15 %, copies 10
+// %, reads of values 9 %; matrix units busy 62 % of the cycles, no bank
+// conflicts.  0.96 PFLOP/s at 4608 tokens x 24 heads of 128, 0.8 at 8191
+// causal tokens x 16 heads of 64.
 template <bool BF, int D, bool PAGED>
 __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kernel(AttnArgs a) {
     constexpr int ST = D / 16, DT = D / 32, CH = D / 8, KK = TileShapeOf<D>::keys, KT = KK / 32,
@@ -775,7 +788,16 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 }
 
 // ---- few rows a sequence ----------------------------------------------------
-
+//
+// Up to 16 rows of a key head take one 16x16x32 product's columns; keys and
+// values go from memory to registers once, each lane the 16 bytes that its
+// matrix operand needs (values are put together from two keys' words), so
+// that a wave's 32 keys of both are in flight together.  The weights of bf16
+// inputs are two products' worth of bf16 (the value and what its rounding
+// left): 2^-17 in place of 2^-9, for a product that costs nothing beside the
+// reads.  Bound by HBM: 64 bf16 caches of 60 to 8100 keys, 1.04 GB, 210 us,
+// 4.9 TB/s (the rate of a large copy); one of 32700 keys, 134 MB, 27 us and a
+// join of 5.6, latency at both ends.
 constexpr int kFewRows = 16, kFewKeys = 32, kWaves = 4;
 
 // The keys that any token of a sequence sees, and into how many ranges of
@@ -1207,7 +1229,9 @@ struct AttnPlan {
 };
 
 // Calls whose sequences have up to 16 rows a key head on average run the
-// few-rows kernel, others tiles.  Tiles of few rounds of the device are split
+// few-rows kernel, others tiles (8 sequences over 3000 keys, 8 key heads, us:
+// 16 rows 27.3, as tiles 32.0; 24 rows 42.1, 32.8; 32 sequences over 2000: 16
+// rows 52.0, 50.0; 24 rows 89.8, 50.5).  Tiles of few rounds of the device are split
 // where that pays; of more equal ones (one sequence, every key seen) the part
 // of the last round that would leave most of the device idle.
 AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
@@ -1296,8 +1320,7 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
         // out: few work-groups)
         const int w = p.solo > 0 || p.tiles < 256 ? kRows / 16 : 2;
         hipLaunchKernelGGL((b1_attn_tile_join_kernel<BF, D>), dim3(p.tiles * w), block, 0, s, a, w);
-    }
-    else if (p.splits <= 4)
+    } else if (p.splits <= 4)
         hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 1>), dim3((rows + 15) / 16), block, 0, s, a);
     else if (p.splits <= 16)
         hipLaunchKernelGGL((b1_attn_few_join_kernel<BF, D, 4>), dim3((rows + 3) / 4), block, 0, s, a);

@@ -233,7 +233,7 @@ struct AttnArgs {
     int32_t *bad; // device counter of bad indexes, or NULL
     // filled by launch_attn
     int splits = 1;            // most ranges that a row's keys are split into
-    int target = 0;            // work items wanted; 0: exactly `splits` ranges
+    int target = 0;            // work items that fill the device
     int solo = 0;              // tiles that are not split, the first ones
     int items = 0;             // work items behind those
     int cus = 0;               // of the device
