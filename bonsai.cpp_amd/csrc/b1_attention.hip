@@ -794,7 +794,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 // matrix operand needs (values are put together from two keys' words), so
 // that a wave's 32 keys of both are in flight together.  The weights of bf16
 // inputs are two products' worth of bf16 (the value and what its rounding
-// left): 2^-17 in place of 2^-9, for a product that costs nothing beside the
+// left): 2^-16 in place of 2^-8, for a product that costs nothing beside the
 // reads.  Bound by HBM: 64 bf16 caches of 60 to 8100 keys, 1.04 GB, 210 us,
 // 4.9 TB/s (the rate of a large copy); one of 32700 keys, 134 MB, 27 us and a
 // join of 5.6, latency at both ends.
