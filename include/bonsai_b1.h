@@ -613,8 +613,8 @@ typedef struct bonsai_b1_kv_pages {
 /*
  * Indexes in device memory (starts, lengths, page tables, positions) are
  * read by the kernels alone.  Each is brought into range before it addresses
- * anything; a row that depends on one that was not in range comes out NaN,
- * nothing of it is stored in a cache, and the optional device counter `bad`
+ * anything; a row that depends on one that was not in range comes out NaN (as
+ * may rows of the same sequence beside it), nothing of it is stored in a cache, and the optional device counter `bad`
  * grows by at least 1 a call.  Sequences must not overlap; where they do,
  * the rows they share are unspecified.
  */
@@ -689,8 +689,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * workspace: bonsai_b1_attention_workspace_bytes(args) bytes (16-byte
  * aligned) for calls whose keys are split over work-groups, or NULL for the
  * library's per-stream workspace, with the rules of bonsai_b1_linear_f32's
- * for captures.  Without one (a capture never allocates) the call runs
- * unsplit: the same values up to the order of fp32 sums, slower for few rows
+ * for captures.  Without one (a capture never allocates), or with one too
+ * small, the call runs unsplit: the same values up to the order of fp32 sums, slower for few rows
  * over many keys.  A workspace serves one call at a time: give graphs that
  * may be replayed at once one each.
  */

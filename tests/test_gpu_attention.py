@@ -205,7 +205,35 @@ PAGED = [
     ([1, 1], [3000, 90], 8, 2, 64, "bf16", 256, "token", 700, False),
     ([60], [5000], 4, 1, 128, "fp16", 128, "head", 0, False),
     ([12], [5], 4, 2, 128, "fp16", 16, "head", 0, False),  # tokens before the first key
+    # tiles over pages of fewer keys than one copy of a wave takes
+    ([150], [170], 2, 2, 64, "fp16", 1, "head", 0, False),
+    ([40, 90], [140, 333], 4, 2, 64, "bf16", 2, "token", 0, True),
+    ([130], [261], 2, 1, 64, "fp16", 4, "head", 70, False),
+    ([33, 70], [45, 301], 4, 2, 128, "fp16", 1, "token", 0, False),
+    ([129], [2000], 2, 1, 128, "bf16", 2, "head", 0, True),
+    ([40, 5], [170, 77], 4, 1, 256, "fp16", 1, "head", 0, False),
+    # many sequences as tiles
+    ([20 + i % 9 for i in range(70)], [30 + 5 * i for i in range(70)], 2, 1, 128, "fp16", 16, "token", 0, True),
 ]
+
+
+@pytest.mark.parametrize("d,page", [(64, 1), (64, 16), (128, 2), (256, 1), (256, 64)])
+def test_bad_page_in_tiles(torch, b1, d, page):
+    """A page out of range in a sequence of tiles: NaN from the first token that sees it on."""
+    say(f"bad page {d} {page}")
+    heads, kv_heads, ql, kl = 4, 2, [100, 90], [100, 200]
+    q, k, v = make(torch, 45, ql, kl, heads, kv_heads, d, torch.float16)
+    kc, vc, table = paged(torch, 6, k, v, kl, page, "head")
+    table[1, 3] = 1 << 20
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = b1.attention_paged(q, kc, vc, i32(torch, ref.starts(ql)), i32(torch, kl), table, bad=bad)
+    assert int(bad) > 0
+    want, off = expect(torch, q, k, v, ql, kl, d ** -0.5, True, 0)
+    ref.check(out[:100], want[:100], off[:100], torch.float16, "the other sequence")
+    if 4 * page <= 110:  # every token sees places 0 .. 110
+        assert bool(out[100:].isnan().all())
+    else:  # page 3 of 64 keys: places 192 on, the last 8 tokens'
+        assert bool(out[182:].isnan().all())
 
 
 def paged(torch, seed, k, v, kl, page, order, spare=2):
