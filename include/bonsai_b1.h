@@ -638,7 +638,7 @@ typedef struct bonsai_b1_kv_pages {
  * multiples of 4; 16-bit pointers 16-byte aligned, strides multiples of 8;
  * rope_dim a multiple of 8, <= head_dim; tokens < 2^24, heads < 2^16, tokens
  * * heads < 2^28; outputs apart from the inputs.  The reference computes these as
- * separate ggml ops on q and k (src/diffuser_graph.cpp:354-406 and
+ * separate ops on q and k (src/diffuser_graph.cpp:354-406 and
  * src/b1_0_kernel.h:309-361, interleaved).
  */
 typedef struct bonsai_b1_qkv_args {
@@ -678,8 +678,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * for the product with v.  out: rows of heads * head_dim in the inputs' type
  * (packed = 0), or the packed fp16 activations of the next B1_0 linear
  * (packed = 1: bonsai_b1_pack_act_f16_ld's layout with row stride ldo, so
- * that `out` may be a column range of wider activations), as the reference's
- * ggml_flash_attn_ext feeds its output projections
+ * that `out` may be a column range of wider activations), as the attention
+ * of the reference's blocks feeds their output projections
  * (src/diffuser_graph.cpp:406-441,509-536).
  * head_dim 64, 128 or 256; pointers 16-byte aligned; strides in elements,
  * multiples of 8; scale > 0; out apart from the inputs.  Query strides may
