@@ -172,12 +172,16 @@ constexpr int kRows = 128;
 // at D = 128 that takes stages of 32 keys (4608 tokens x 24 heads 299 us, of
 // 64 keys and two work-groups 310; 4096 causal tokens x 32 heads 156, 167);
 // at D = 64 stages of 64 fit too (168, 179 of 32 keys).  At D = 256 the
-// registers of a row's sums leave one: 690 TFLOP/s, 520 of two that spill.
+// registers of a row's sums leave one (690 TFLOP/s, 520 of two that spill),
+// and LDS has room for four stages of 32 keys (4608 tokens x 12 heads 375 us,
+// two of 64 keys 385).  Two stages at D = 128 against three: chunks over a
+// paged cache 156 us, 164, others alike; three at D = 64 against two: 8191
+// causal tokens 178, 179.
 template <int D>
 struct TileShapeOf {
-    static constexpr int keys = D == 128 ? 32 : 64;
+    static constexpr int keys = D == 64 ? 64 : 32;
     static constexpr int waves = D == 256 ? 1 : 3;
-    static constexpr int stages = D == 256 ? 2 : 3; // in LDS
+    static constexpr int stages = D == 64 ? 3 : D == 128 ? 2 : 4;
 };
 // A range of a split tile has at least this many keys, so that its fixed
 // costs (queries, partial sums out and in) stay small beside them.

@@ -22,16 +22,15 @@ __device__ __forceinline__ float lanes_sum(float v) {
 //
 // Bound by HBM: x, add and h at 4 bytes a value, y at 4 or (packed) 2, so a
 // row is read once and kept in registers between the sum and the scaling
-// (8192 rows of 4096 with add: 86 us, 5.4 TB/s).
+// (8192 rows of 4096 with add: 84 us, 5.6 TB/s).
 // T threads take a row (a work-group has 256 threads or T), U units of 8
 // values each (4 + 4 values 16 columns apart: the halves of a packed word
 // quad); U = 0 reads wider rows twice.  The sum is fp32, at most 8 U values a
 // thread and then a tree.
 template <int T, int U>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void b1_rms_norm_kernel(const float *x, int64_t ldx, const float *add, int64_t lda,
-                                                          int H, int rows, const float *__restrict__ w, float eps,
-                                                          float *h, int64_t ldh, float *__restrict__ y, int64_t ldy,
-                                                          uint32_t *__restrict__ packed) {
+__global__ __launch_bounds__(T < 256 ? 256 : T) void b1_rms_norm_kernel(
+    const float *x, int64_t ldx, const float *add, int64_t lda, int H, int rows, const float *__restrict__ w,
+    float eps, float *h, int64_t ldh, float *__restrict__ y, int64_t ldy, uint32_t *__restrict__ packed) {
     constexpr int ROWS = T < 256 ? 256 / T : 1; // a work-group
     __shared__ float part[T / 64];
     const int t = threadIdx.x % T;
