@@ -510,7 +510,7 @@ __device__ __forceinline__ void reads_ahead() {
 // exponentials), and by how well three independent work-groups a CU hide one
 // another's LDS reads, barriers and copies.  Left out in turn at D = 128, 8192
 // tokens (1103 us, 1.0 PFLOP/s): reads of keys 21 %, softmax 15 %, copies 10
-// %, reads of values 9 %; matrix units busy 62 % of the cycles, no bank
+// %, reads of values 9 %; matrix units busy 63 % of the cycles, no bank
 // conflicts.  0.96 PFLOP/s at 4608 tokens x 24 heads of 128, 0.8 at 8191
 // causal tokens x 16 heads of 64.
 template <bool BF, int D, bool PAGED>
