@@ -12,6 +12,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <vector>
 
 #include "b1_seqs.h"
 
@@ -74,8 +75,9 @@ __device__ __forceinline__ u32x2 read_columns(const void *p) {
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < kInf; }
 
 // x / group for 0 <= x < 2^28 (AttnArgs::div_m and div_s).
-__device__ __forceinline__ int div_group(const AttnArgs &a, int x) {
-    return (int)((__umulhi((uint32_t)x, a.div_m) + (uint32_t)x) >> a.div_s);
+__host__ __device__ __forceinline__ int div_group(const AttnArgs &a, int x) {
+    const uint32_t hi = (uint32_t)(((uint64_t)(uint32_t)x * a.div_m) >> 32);
+    return (int)((hi + (uint32_t)x) >> a.div_s);
 }
 
 // One key head's keys (or values) of one sequence.
@@ -106,7 +108,7 @@ __device__ __forceinline__ int64_t key_at(const AttnArgs &a, const KeyRows &r, i
 }
 
 // The keys [lo, hi] that token i of a sequence sees.
-__device__ __forceinline__ void visible(const AttnArgs &a, const Seq &s, int i, int &lo, int &hi) {
+__host__ __device__ __forceinline__ void visible(const AttnArgs &a, const Seq &s, int i, int &lo, int &hi) {
     lo = 0;
     hi = s.nk - 1;
     if (a.causal) {
@@ -211,7 +213,7 @@ struct TileKeys {
     int r0, rows; // first row, rows there (<= kRows)
     int k0, k1;
 };
-__device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, int group, int t) {
+__host__ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, int group, int t) {
     TileKeys k;
     k.r0 = t * kRows;
     k.rows = min(kRows, s.nq * group - k.r0);
@@ -222,7 +224,9 @@ __device__ __forceinline__ TileKeys tile_keys(const AttnArgs &a, const Seq &s, i
     k.k1 = max(hi + 1, lo);
     return k;
 }
-__device__ __forceinline__ int seq_tiles(const Seq &s, int group) { return (s.nq * group + kRows - 1) / kRows; }
+__host__ __device__ __forceinline__ int seq_tiles(const Seq &s, int group) {
+    return (s.nq * group + kRows - 1) / kRows;
+}
 
 // Sum over the wave.
 __device__ __forceinline__ int wave_sum(int v) {
@@ -244,56 +248,102 @@ __device__ __forceinline__ int wave_sum(int v) {
 // with two, 1.5 with three; a partial tile 0.026.  Split against whole (us):
 // 128 tiles over 4096 keys 59 / 104, 8 over 4000 24 / 102, 128 over 1000
 // 36 / 33, 256 over 1024 (causal) 41 / 33, 480 over 2560 126 / 97.
+// (Without contraction: the two kernels that build a plan from the lengths,
+// and the host, compute the same values.)
 struct SeqWork {
-    int tiles;         // of a key head
-    float last, total; // keys of the last tile (the most), of all of them
+    int tiles;   // of a key head
+    int most;    // keys of a tile, no tile has more
+    float total; // keys of all tiles
 };
-__device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, const Seq &s, int group) {
-    SeqWork w = {seq_tiles(s, group), 0.f, 0.f};
+// A tile's rows are of at most `span` tokens, so that a window leaves it
+// window + span - 1 keys at most; a last tile of fewer rows has fewer.
+__host__ __device__ __forceinline__ SeqWork seq_work(const AttnArgs &a, const Seq &s, int group) {
+#pragma clang fp contract(off)
+    SeqWork w = {seq_tiles(s, group), 0, 0.f};
     if (w.tiles > 0) {
-        const TileKeys x = tile_keys(a, s, group, 0), y = tile_keys(a, s, group, w.tiles - 1);
-        w.last = (float)(y.k1 - y.k0);
-        w.total = (float)w.tiles * 0.5f * ((float)(x.k1 - x.k0) + w.last);
+        const int span = min(s.nq, (kRows - 2 + 2 * group) / group);
+        w.most = a.window ? min(s.nk, a.window + span - 1) : s.nk;
+        const TileKeys x = tile_keys(a, s, group, 0);
+        w.total = (float)w.tiles * 0.5f * ((float)(x.k1 - x.k0) + (float)w.most);
     }
     return w;
 }
+// Of a call's sequences: the keys of all tiles, as they are and if each had
+// its sequence's most, the longest tile's, and the tiles (of a key head).
+struct CallWork {
+    float total, reach, longest;
+    int tiles;
+};
+__host__ __device__ __forceinline__ CallWork call_work(const SeqWork &w) {
+    return CallWork{w.total, (float)w.tiles * (float)w.most, (float)w.most, w.tiles};
+}
+__host__ __device__ __forceinline__ void add_work(CallWork &c, const CallWork &w) {
+#pragma clang fp contract(off)
+    c.total += w.total;
+    c.reach += w.reach;
+    c.longest = fmaxf(c.longest, w.longest);
+    c.tiles += w.tiles;
+}
 constexpr int kWhole = INT_MAX / 2; // a unit that splits nothing
-// From the keys of all tiles, as they are and if each had its sequence's
-// most, the longest tile's, and the tiles (of a key head, all sequences).
-__device__ __forceinline__ int tile_unit(const AttnArgs &a, float total, float reach, float longest, float tiles) {
-    total *= (float)a.kv_heads;
-    reach *= (float)a.kv_heads;
-    tiles *= (float)a.kv_heads;
+__host__ __device__ __forceinline__ int tile_unit(const AttnArgs &a, const CallWork &w) {
+#pragma clang fp contract(off)
+    const float total = w.total * (float)a.kv_heads, reach = w.reach * (float)a.kv_heads;
+    const float tiles = (float)w.tiles * (float)a.kv_heads;
     const float target = (float)a.target;
     const float cus = target * (a.head_dim == 256 ? 1.f / TileShapeOf<256>::waves : 1.f / TileShapeOf<128>::waves);
     const float scale = (float)a.head_dim * (1.f / 128);
-    const float whole = longest * (1.f / 32) * scale * (tiles <= cus ? 0.72f : tiles <= 2 * cus ? 1.15f : 1.5f);
+    const float whole = w.longest * (1.f / 32) * scale * (tiles <= cus ? 0.72f : tiles <= 2 * cus ? 1.15f : 1.5f);
     const float parts = tiles + fminf(target, total * (1.f / kLeastKeys));
     const float split = (total * (1.f / 32) * 1.7f / target + 0.026f * parts) * scale + 8.f;
     if (whole < 1.2f * split) return kWhole;
-    // (so that tiles x ceil(most keys / unit) <= tiles + target)
+    // so that tiles x ceil(most keys / unit) <= tiles + target, which the
+    // grid has room for
     return (int)fminf(fmaxf((float)kLeastKeys, reach / target + 1.f), (float)kWhole);
 }
-__device__ __forceinline__ int key_ranges(const AttnArgs &a, int keys, int unit) {
+__host__ __device__ __forceinline__ int key_ranges(const AttnArgs &a, int keys, int unit) {
     return max(1, min(a.splits, (keys + unit - 1) / unit));
 }
-// The unit that makes the items (of a key head, at the unit so far) fit the
-// device at once: a few more than that would run after all others.
-__device__ __forceinline__ int fit_unit(const AttnArgs &a, int unit, int items) {
+// A larger unit where the items (of a key head, at the unit so far) are more
+// than the device holds at once, by as much: those left over would run after
+// all others.  (Ranges are whole, so a few may still be.)
+__host__ __device__ __forceinline__ int fit_unit(const AttnArgs &a, int unit, int items) {
+#pragma clang fp contract(off)
     const float have = (float)items * (float)a.kv_heads;
-    return have <= (float)a.target ? unit : (int)((float)unit * have / (float)a.target) + 1;
+    return have <= (float)a.target ? unit : (int)fminf((float)unit * have / (float)a.target, (float)kWhole) + 1;
+}
+// The unit of the only sequence of a call, of its last tiles where the first
+// a.solo are whole.
+__host__ __device__ __forceinline__ int one_seq_unit(const AttnArgs &a, const SeqWork &w) {
+    if (a.solo > 0) return max(1, (w.most + a.splits - 1) / a.splits);
+    if (a.splits == 1) return kWhole;
+    const int unit = tile_unit(a, call_work(w));
+    return unit < kWhole ? fit_unit(a, unit, w.tiles * key_ranges(a, w.most, unit)) : unit;
 }
 
 // A work item: key head, row tile and range of one of the sequences.  The
 // first a.solo items are whole tiles; behind them a sequence's n tiles (key
-// heads counted) have as many items as its longest has ranges, the tiles'
-// first ranges before their second ones: neighbouring items run on different
+// heads counted) have as many items each as one of its most keys has ranges,
+// the tiles' first ranges before their second ones: neighbouring items run on different
 // XCDs, and each is to have its share of those that have something to do.
 // The partial sums of range i of the tile are number part + i * apart.
 struct TileItem {
     int b, kvh, t, range, unit, part, apart;
     Seq s;
 };
+// Item g of a sequence's (its tile alone, where whole), whose partial sums
+// begin at number `base`, behind a.solo whole tiles.
+__host__ __device__ __forceinline__ void place_item(const AttnArgs &a, const SeqWork &w, int g, int base, bool whole,
+                                                    TileItem &r) {
+    if (!whole) {
+        r.range = r.apart > 0 ? g / r.apart : 0;
+        g -= r.range * r.apart;
+    }
+    r.part = base + g;
+    g += a.solo;
+    const int q = g / a.kv_heads;
+    r.kvh = g - q * a.kv_heads;
+    r.t = w.tiles - 1 - q;
+}
 // Finds item i (or, of whole tiles, the i-th tile behind the solo ones), by
 // the whole wave; b = -1: none.  Unsplit tiles come in the order of their
 // keys, the most first, so that the last work-groups to start are short: of
@@ -308,56 +358,35 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
     r.apart = 1;
     r.unit = kWhole;
     r.s = Seq{};
-    int t = 0;
+    r.t = 0;
     if (a.seqs.n_seqs == 1) {
         r.s = seq_of(a.seqs, 0);
         const SeqWork w = seq_work(a, r.s, group);
-        const int n = w.tiles * a.kv_heads;
-        int g = i;
         if (whole || i >= a.solo) {
-            r.apart = n - a.solo;
-            if (a.solo > 0) {
-                r.unit = max(1, ((int)w.last + a.splits - 1) / a.splits);
-            } else if (a.splits > 1) {
-                r.unit = tile_unit(a, w.total, (float)w.tiles * w.last, w.last, (float)w.tiles);
-                if (r.unit < kWhole) r.unit = fit_unit(a, r.unit, w.tiles * key_ranges(a, (int)w.last, r.unit));
-            }
-            if (!whole) {
-                g -= a.solo;
-                r.range = r.apart > 0 ? g / r.apart : 0;
-                g -= r.range * r.apart;
-            }
-            r.part = g;
-            g += a.solo;
+            r.apart = w.tiles * a.kv_heads - a.solo;
+            r.unit = one_seq_unit(a, w);
+            place_item(a, w, whole ? i : i - a.solo, 0, whole, r);
+        } else {
+            const int q = i / a.kv_heads;
+            r.kvh = i - q * a.kv_heads;
+            r.t = w.tiles - 1 - q;
         }
-        const int q = g / a.kv_heads;
-        r.kvh = g - q * a.kv_heads;
-        t = w.tiles - 1 - q;
-        if (t >= 0) r.b = 0;
+        if (r.t >= 0) r.b = 0;
     } else {
         // the first 64 sequences stay in registers
         const Seq mine = lane < a.seqs.n_seqs ? seq_of(a.seqs, lane) : Seq{};
         const SeqWork work = seq_work(a, mine, group);
         if (a.splits > 1) {
-            float total = work.total, reach = (float)work.tiles * work.last, longest = work.last;
-            int tiles = work.tiles;
-            for (int b = 64 + lane; b < a.seqs.n_seqs; b += 64) {
-                const SeqWork w = seq_work(a, seq_of(a.seqs, b), group);
-                total += w.total;
-                reach += (float)w.tiles * w.last;
-                longest = fmaxf(longest, w.last);
-                tiles += w.tiles;
-            }
+            CallWork c = call_work(work);
+            for (int b = 64 + lane; b < a.seqs.n_seqs; b += 64)
+                add_work(c, call_work(seq_work(a, seq_of(a.seqs, b), group)));
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) {
-                total += __shfl_xor(total, o);
-                reach += __shfl_xor(reach, o);
-                longest = fmaxf(longest, __shfl_xor(longest, o));
-            }
-            tiles = wave_sum(tiles);
-            r.unit = tile_unit(a, total, reach, longest, (float)tiles);
+            for (int o = 32; o >= 1; o >>= 1)
+                add_work(c, CallWork{__shfl_xor(c.total, o), __shfl_xor(c.reach, o), __shfl_xor(c.longest, o),
+                                     __shfl_xor(c.tiles, o)});
+            r.unit = tile_unit(a, c);
             for (int k = 0; k < 2 && r.unit < kWhole && a.seqs.n_seqs <= 64; ++k)
-                r.unit = fit_unit(a, r.unit, wave_sum(work.tiles * key_ranges(a, (int)work.last, r.unit)));
+                r.unit = fit_unit(a, r.unit, wave_sum(work.tiles * key_ranges(a, work.most, r.unit)));
         }
         int l = -1;
         Seq s = mine;
@@ -386,7 +415,7 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
                 const bool it = here && __popcll(at & ((1ull << lane) - 1)) == q - above;
                 l = __builtin_ctzll(__ballot(it));
                 r.b = l;
-                t = __shfl(low - off, l);
+                r.t = __shfl(low - off, l);
             }
         } else {
             int tiles0 = 0, items0 = 0;
@@ -396,7 +425,7 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
                     s = b0 + lane < a.seqs.n_seqs ? seq_of(a.seqs, b0 + lane) : Seq{};
                     w = seq_work(a, s, group);
                 }
-                const int n = w.tiles * a.kv_heads, c = key_ranges(a, (int)w.last, r.unit);
+                const int n = w.tiles * a.kv_heads, c = key_ranges(a, w.most, r.unit);
                 int tiles = n, items = n * c;
 #pragma unroll
                 for (int o = 1; o < 64; o <<= 1) {
@@ -409,15 +438,8 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
                     r.b = b0 + l;
                     r.apart = __shfl(n, l);
                     const int base = items0 + __shfl(items - n * c, l);
-                    int g = i - (whole ? tiles0 + __shfl(tiles - n, l) : base);
-                    if (!whole) {
-                        r.range = g / r.apart;
-                        g -= r.range * r.apart;
-                    }
-                    r.part = base + g;
-                    const int q = g / a.kv_heads;
-                    r.kvh = g - q * a.kv_heads;
-                    t = __shfl(w.tiles, l) - 1 - q;
+                    w.tiles = __shfl(w.tiles, l);
+                    place_item(a, w, i - (whole ? tiles0 + __shfl(tiles - n, l) : base), base, whole, r);
                 }
                 tiles0 += __shfl(tiles, 63);
                 items0 += __shfl(items, 63);
@@ -438,7 +460,7 @@ __device__ __forceinline__ TileItem find_item(const AttnArgs &a, int group, int 
     r.s.kv0 = uniform(r.s.kv0);
     r.s.nk = uniform(r.s.nk);
     r.kvh = uniform(r.kvh);
-    r.t = uniform(t);
+    r.t = uniform(r.t);
     r.range = uniform(r.range);
     r.part = uniform(r.part);
     r.apart = uniform(r.apart);
@@ -450,7 +472,7 @@ struct TileRange {
     int t0, t1, ranges;
 };
 template <int D>
-__device__ __forceinline__ TileRange tile_range(const AttnArgs &a, const TileKeys &k, const TileItem &it) {
+__host__ __device__ __forceinline__ TileRange tile_range(const AttnArgs &a, const TileKeys &k, const TileItem &it) {
     constexpr int KK = TileShapeOf<D>::keys;
     const int first = k.k0 / KK, last = (k.k1 + KK - 1) / KK, n = last - first;
     TileRange r;
@@ -1288,6 +1310,67 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     return p;
 }
 
+// For a call's launch: where the kernels get what the plan says.
+void set_plan(AttnArgs *a, const AttnPlan &p, int num_cus) {
+    a->splits = p.splits;
+    a->target = p.target;
+    a->solo = p.solo;
+    a->cus = num_cus;
+    a->items = (int)(p.grid - p.solo);
+    // x / group by a multiplication (x < 2^31): s = ceil(log2 group), m =
+    // floor(2^32 (2^s - group) / group) + 1, x / group = (hi(x m) + x) >> s
+    const uint32_t group = (uint32_t)(a->heads / a->kv_heads);
+    a->div_s = 0;
+    while ((1u << a->div_s) < group) ++a->div_s;
+    a->div_m = (uint32_t)(((((uint64_t)1 << a->div_s) - group) << 32) / group) + 1;
+}
+
+// find_item of a split call on the host, from the sequences themselves.
+TileItem find_split_item(const AttnArgs &a, const Seq *seqs, int i, bool whole) {
+    const int group = a.heads / a.kv_heads, n_seqs = a.seqs.n_seqs;
+    TileItem r{};
+    r.b = -1;
+    r.unit = kWhole;
+    r.apart = 1;
+    if (n_seqs == 1) {
+        const SeqWork w = seq_work(a, seqs[0], group);
+        r.s = seqs[0];
+        r.apart = w.tiles * a.kv_heads - a.solo;
+        r.unit = one_seq_unit(a, w);
+        place_item(a, w, whole ? i : i - a.solo, 0, whole, r);
+        if (r.t >= 0) r.b = 0;
+        return r;
+    }
+    CallWork c[64] = {};
+    for (int b = 0; b < n_seqs; ++b) add_work(c[b % 64], call_work(seq_work(a, seqs[b], group)));
+    for (int o = 32; o >= 1; o >>= 1)
+        for (int l = 0; l < o; ++l) add_work(c[l], c[l + o]);
+    r.unit = tile_unit(a, c[0]);
+    for (int k = 0; k < 2 && r.unit < kWhole && n_seqs <= 64; ++k) {
+        int items = 0;
+        for (int b = 0; b < n_seqs; ++b) {
+            const SeqWork w = seq_work(a, seqs[b], group);
+            items += w.tiles * key_ranges(a, w.most, r.unit);
+        }
+        r.unit = fit_unit(a, r.unit, items);
+    }
+    int tiles = 0, items = 0;
+    for (int b = 0; b < n_seqs; ++b) {
+        const SeqWork w = seq_work(a, seqs[b], group);
+        const int n = w.tiles * a.kv_heads, all = n * key_ranges(a, w.most, r.unit);
+        if ((whole ? tiles + n : items + all) > i) {
+            r.b = b;
+            r.s = seqs[b];
+            r.apart = n;
+            place_item(a, w, i - (whole ? tiles : items), items, whole, r);
+            return r;
+        }
+        tiles += n;
+        items += all;
+    }
+    return r;
+}
+
 size_t round_256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Partial results of a plan: their rows, and bytes of the three areas (sums
@@ -1338,22 +1421,52 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
 
 } // namespace
 
+extern "C" int64_t b1_attention_items(const int32_t *q_len, const int32_t *kv_len, int n_seqs, int most, int heads,
+                                      int kv_heads, int head_dim, int causal, int window, int num_cus, int join,
+                                      int32_t *items, int64_t room, int64_t *rows) {
+    AttnArgs a{};
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.causal = causal;
+    a.window = window;
+    a.seqs.n_seqs = n_seqs;
+    a.seqs.kv_tokens = most;
+    std::vector<Seq> seqs(n_seqs);
+    int64_t kv0 = 0;
+    for (int b = 0; b < n_seqs; ++b) {
+        seqs[b] = Seq{a.seqs.tokens, q_len[b], (int)kv0, kv_len[b], false};
+        a.seqs.tokens += q_len[b];
+        kv0 += kv_len[b];
+    }
+    if (a.seqs.tokens == 0) return 0;
+    const AttnPlan p = attn_plan(a, num_cus, true);
+    if (p.few || p.splits <= 1) return 0;
+    set_plan(&a, p, num_cus);
+    *rows = part_rows(a, p);
+    const int group = heads / kv_heads;
+    const int64_t n = join ? p.tiles : p.grid - p.solo;
+    for (int64_t i = 0; i < std::min(n, room); ++i) {
+        const TileItem it = find_split_item(a, seqs.data(), (int)(join ? i : p.solo + i), join != 0);
+        TileRange r{};
+        if (it.b >= 0) {
+            const TileKeys k = tile_keys(a, it.s, group, it.t);
+            r = head_dim == 64 ? tile_range<64>(a, k, it) : head_dim == 128 ? tile_range<128>(a, k, it)
+                                                                            : tile_range<256>(a, k, it);
+        }
+        const int32_t row[] = {it.b, it.kvh, it.t, it.range, r.ranges, r.t0, r.t1, it.part, it.apart};
+        std::copy(row, row + 9, items + 9 * i);
+    }
+    return n;
+}
+
 size_t attn_workspace_bytes(const AttnArgs &a, int num_cus) { return part_bytes(a, attn_plan(a, num_cus, true)); }
 
 hipError_t launch_attn(const AttnArgs &args, int num_cus, void *ws, size_t ws_bytes, hipStream_t s) {
     AttnArgs a = args;
     AttnPlan p = attn_plan(a, num_cus, true);
     if (p.splits > 1 && (!ws || ws_bytes < part_bytes(a, p))) p = attn_plan(a, num_cus, false);
-    a.splits = p.splits;
-    a.target = p.target;
-    a.solo = p.solo;
-    a.cus = num_cus;
-    a.items = (int)(p.grid - p.solo);
-    // x / group by a multiplication (x < 2^31): s = ceil(log2 group), m =
-    // floor(2^32 (2^s - group) / group) + 1, x / group = (hi(x m) + x) >> s
-    const uint32_t group = (uint32_t)(a.heads / a.kv_heads);
-    while ((1u << a.div_s) < group) ++a.div_s;
-    a.div_m = (uint32_t)(((((uint64_t)1 << a.div_s) - group) << 32) / group) + 1;
+    set_plan(&a, p, num_cus);
     if (p.splits > 1) {
         const size_t rows = (size_t)part_rows(a, p);
         uint8_t *at = static_cast<uint8_t *>(ws);

@@ -247,6 +247,17 @@ struct AttnArgs {
 size_t attn_workspace_bytes(const AttnArgs &a, int num_cus);
 // Runs without a workspace too (ws NULL or too small), its keys unsplit.
 hipError_t launch_attn(const AttnArgs &a, int num_cus, void *ws, size_t ws_bytes, hipStream_t s);
+// The work items of a call whose tiles' keys are split (0: none), as the
+// kernels find them: of sequences of the given lengths, `most` keys at most by
+// what the host knows.  Items of the launch behind its whole tiles, or (join)
+// of its join; nine values each: sequence (-1: none), key head, tile, range,
+// the tile's ranges, the range's first stage and the one behind its last,
+// number of the partial sums of the tile's first range, and how far apart
+// those of its ranges are.  *rows: rows of partial sums there is room for.
+// For the tests; no part of the C ABI.
+extern "C" int64_t b1_attention_items(const int32_t *q_len, const int32_t *kv_len, int n_seqs, int most, int heads,
+                                      int kv_heads, int head_dim, int causal, int window, int num_cus, int join,
+                                      int32_t *items, int64_t room, int64_t *rows);
 
 // fp32 q, k, v rows of a linear -> head norm (weights or NULL), rotary
 // embedding (table rows of rope_dim: cos then sin; or NULL), 16 bits; k and
