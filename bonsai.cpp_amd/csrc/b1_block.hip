@@ -216,39 +216,58 @@ __global__ __launch_bounds__(256) void b1_qkv_kernel(QkvArgs a, int per) {
     if (bad && a.bad && threadIdx.x == 0 && blockIdx.y == 0) atomicAdd(a.bad, 1);
 }
 
+// Calls f(kernel, its threads a work-group, its rows a work-group) for rows
+// of H values.
+//
+// Few units a thread and as many threads as that takes: all of a row's
+// loads are on their way at once, with few registers held.  Measured (us
+// of a norm of x + add into h and packed): 32768 x 512 40.7 (256 threads
+// a row 47.3), 8192 x 2048 41.2 (a wave a row 50.8), 8192 x 4096 86.4
+// (256 threads 93.8), 4096 x 8192 88.0 (512 threads 94.9, 256 98.3),
+// 2048 x 16384 96.8 = 4.9 TB/s (256 threads 117), 2048 x 32768 188 (row
+// read twice 303).
+template <class F>
+auto with_rms_kernel(int H, F f) {
+    if (H <= 512) return f(b1_rms_norm_kernel<64, 1>, 256, 4);
+    if (H <= 2048) return f(b1_rms_norm_kernel<256, 1>, 256, 1);
+    if (H <= 4096) return f(b1_rms_norm_kernel<512, 1>, 512, 1);
+    if (H <= 8192) return f(b1_rms_norm_kernel<1024, 1>, 1024, 1);
+    if (H <= 16384) return f(b1_rms_norm_kernel<1024, 2>, 1024, 1);
+    if (H <= 32768) return f(b1_rms_norm_kernel<1024, 4>, 1024, 1);
+    return f(b1_rms_norm_kernel<1024, 0>, 1024, 1);
+}
+
+// The rows of a launch: work-groups of 2^31 threads (a launch has less than
+// 2^32).
+int64_t rms_launch_rows(int threads, int per) { return ((int64_t)1 << 31) / threads * per; }
+
 } // namespace
+
+extern "C" int64_t b1_rms_norm_launch(int H, int *threads, int *per) {
+    return with_rms_kernel(H, [&](auto, int t, int p) {
+        *threads = t;
+        *per = p;
+        return rms_launch_rows(t, p);
+    });
+}
 
 hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_t lda, int H, int rows,
                            const float *w, float eps, float *h, int64_t ldh, float *y, int64_t ldy, void *packed,
                            hipStream_t s) {
     uint32_t *pk = static_cast<uint32_t *>(packed);
-    // a launch has less than 2^32 threads
-    constexpr int most = 1 << 23;
-    auto run = [&](auto kernel, int per, int threads) {
+    return with_rms_kernel(H, [&](auto kernel, int threads, int per) {
+        const int64_t most = rms_launch_rows(threads, per);
         for (int64_t r0 = 0; r0 < rows; r0 += most) {
             const int n = (int)std::min<int64_t>(most, rows - r0);
-            hipLaunchKernelGGL(kernel, dim3((n + per - 1) / per), dim3(threads), 0, s, x + r0 * ldx, ldx,
-                               add ? add + r0 * lda : nullptr, lda, H, n, w, eps, h ? h + r0 * ldh : nullptr, ldh,
-                               y ? y + r0 * ldy : nullptr, ldy, pk ? pk + r0 * (H / 2) : nullptr);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)n + per - 1) / per)), dim3(threads), 0, s,
+                               x + r0 * ldx, ldx, add ? add + r0 * lda : nullptr, lda, H, n, w, eps,
+                               h ? h + r0 * ldh : nullptr, ldh, y ? y + r0 * ldy : nullptr, ldy,
+                               pk ? pk + r0 * (H / 2) : nullptr);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
         return hipSuccess;
-    };
-    // Few units a thread and as many threads as that takes: all of a row's
-    // loads are on their way at once, with few registers held.  Measured (us
-    // of a norm of x + add into h and packed): 32768 x 512 40.7 (256 threads
-    // a row 47.3), 8192 x 2048 41.2 (a wave a row 50.8), 8192 x 4096 86.4
-    // (256 threads 93.8), 4096 x 8192 88.0 (512 threads 94.9, 256 98.3),
-    // 2048 x 16384 96.8 = 4.9 TB/s (256 threads 117), 2048 x 32768 188 (row
-    // read twice 303).
-    if (H <= 512) return run(b1_rms_norm_kernel<64, 1>, 4, 256);
-    if (H <= 2048) return run(b1_rms_norm_kernel<256, 1>, 1, 256);
-    if (H <= 4096) return run(b1_rms_norm_kernel<512, 1>, 1, 512);
-    if (H <= 8192) return run(b1_rms_norm_kernel<1024, 1>, 1, 1024);
-    if (H <= 16384) return run(b1_rms_norm_kernel<1024, 2>, 1, 1024);
-    if (H <= 32768) return run(b1_rms_norm_kernel<1024, 4>, 1, 1024);
-    return run(b1_rms_norm_kernel<1024, 0>, 1, 1024);
+    });
 }
 
 hipError_t launch_qkv(const QkvArgs &a, hipStream_t s) {

@@ -202,6 +202,9 @@ hipError_t launch_swiglu_pack(const float *act, int64_t lda, int M, int H, void 
 hipError_t launch_rms_norm(const float *x, int64_t ldx, const float *add, int64_t lda, int H, int rows,
                            const float *w, float eps, float *h, int64_t ldh, float *y, int64_t ldy, void *packed,
                            hipStream_t s);
+// Rows of H values that a launch of it takes at most, and its work-groups'
+// threads and rows.  For the tests; no part of the C ABI.
+extern "C" int64_t b1_rms_norm_launch(int H, int *threads, int *per);
 
 // Sequences and their keys, as every attention kernel sees them.  Tokens of
 // sequence b are rows q_start[b] .. q_start[b + 1] (NULL: one sequence of

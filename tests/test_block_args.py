@@ -128,3 +128,14 @@ def test_python_refuses_what_is_no_cuda_tensor():
         bonsai_b1.attention(h, h, h)
     with pytest.raises(ValueError):
         bonsai_b1.attention_paged(h, h[None], h[None], None, x, x)
+
+
+@pytest.mark.parametrize("h", [32, 512, 544, 2048, 2080, 4096, 4128, 8192, 8224, 16384, 16416, 32768, 32800, 70016])
+def test_rms_norm_launches_fit(lib, h):
+    """The rows of a launch keep its threads below the launch limit of 2^32,
+    and cover a call of any number of rows in a few launches."""
+    lib.b1_rms_norm_launch.restype = ctypes.c_int64
+    threads, per = ctypes.c_int(0), ctypes.c_int(0)
+    rows = lib.b1_rms_norm_launch(h, ctypes.byref(threads), ctypes.byref(per))
+    assert rows % per.value == 0 and 1 << 21 <= rows < 1 << 31
+    assert rows // per.value * threads.value < 1 << 32

@@ -378,3 +378,23 @@ def test_captured_decode_step(torch, b1):
     # the shared pages are as they were, the steps' places are not
     assert torch.equal(kg[:prefix], kc[:prefix]) and not torch.equal(kg[prefix:], kc[prefix:])
     del graph
+
+
+def test_rms_norm_of_more_wide_rows_than_a_launch(torch, b1):
+    """Rows of 1024 threads: 2^22 of them would be 2^32 threads at once."""
+    rows, h = (1 << 22) + 3, 4128
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < rows * h * 6 + (4 << 30):
+        pytest.skip("needs 108 GB of free device memory")
+    x = torch.empty((rows, h), dtype=torch.float32, device="cuda")
+    some = torch.tensor([0, 1, (1 << 21) - 1, 1 << 21, (1 << 21) + 1, rows - 4, rows - 1], device="cuda")
+    x.fill_(1.0)
+    x[some] = normal(torch, 40, len(some), h)
+    packed = b1.rms_norm(x, None, 1e-6, packed=True)
+    want, off = norm_ref(torch, x[some], None, 1e-6)
+    del x
+    got = packed.view(torch.float16).view(rows, h)[some].contiguous().view(torch.uint8).flatten()
+    ref.check(ref.unpack(got, len(some), h), want, off, torch.float16, "rows")
+    del packed, got
+    torch.cuda.empty_cache()
