@@ -553,6 +553,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     const TileKeys tk = tile_keys(a, s, group, it.t);
     const TileRange tr = tile_range<D>(a, tk, it);
     const int ranges = uniform(tr.ranges), t0 = uniform(tr.t0), t1 = uniform(tr.t1);
+    const int first_key = uniform(tk.k0);
     if (it.range >= ranges) return;
 
     // this lane's row; rows past the tile's last repeat it and store nothing
@@ -598,7 +599,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
         }
         return p;
     };
-    auto load = [&](int kb, const Pages &page, int to) __attribute__((always_inline)) {
+    auto load = [&](int kb, const Pages &page, int to, bool begin) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int at = wave * NI + i, row0 = at * NR;
@@ -609,9 +610,12 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
                 const int size = 1 << a.seqs.page_shift, bytes = (int)kr.row * 2;
                 const uint32_t off = (uint32_t)((kb + row) & (size - 1)) * (uint32_t)bytes;
                 auto copy = [&](int id, int j) __attribute__((always_inline)) {
+                    // keys of the page up to the sequence's last; none of a
+                    // page that a window leaves behind, whose entry may be
+                    // anything (only in a tile's first stage)
+                    int keys = min(size, s.nk - (j & -size));
+                    if (begin && (j | (size - 1)) < first_key) keys = 0, id = 0;
                     if ((unsigned)id >= (unsigned)a.seqs.n_pages) bad = true, id = 0;
-                    // keys of the page up to the sequence's last
-                    const int keys = min(size, s.nk - (j & -size));
                     copy_to_lds(key_buffer(kr.base + id * kr.page, keys * bytes), ks, off + ck);
                     copy_to_lds(key_buffer(vr.base + id * vr.page, keys * bytes), vs, off + cv);
                 };
@@ -661,7 +665,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
     if (t0 < t1) {
 #pragma unroll
         for (int i = 0; i < S - 1; ++i)
-            if (t0 + i < t1) load((t0 + i) * KK, pages((t0 + i) * KK), i);
+            if (t0 + i < t1) load((t0 + i) * KK, pages((t0 + i) * KK), i, i == 0);
         next = pages((t0 + S - 1) * KK);
         // the queries too, so that no wait for them remains in the loop
         wait_vmcnt<0>();
@@ -678,7 +682,7 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
         wait_lgkmcnt0();
         lds_barrier();
         if (tt + S - 1 < t1) {
-            load(kb + (S - 1) * KK, next, (at + S - 1) % S);
+            load(kb + (S - 1) * KK, next, (at + S - 1) % S, false);
             next = pages(kb + S * KK);
         }
         if (!wave_on || kb > last_hi || kb + KK - 1 < first_lo) return;

@@ -596,8 +596,9 @@ enum { BONSAI_B1_F16 = 0, BONSAI_B1_BF16 = 1 };
  * 16-byte aligned; rows, heads and pages apart from one another by at least
  * head_dim.  Sequence b has kv_len[b] keys, its new tokens among them (they
  * are its last ones).  Table entries behind a sequence's last page are not
- * read; sequences may share pages that a call only reads.  max_pages *
- * page_size < 2^30, page_size * row_stride < 2^30.
+ * used, nor are those of pages that attention's window leaves before the
+ * first key any token of the call sees; sequences may share pages that a call
+ * only reads.  max_pages * page_size < 2^30, page_size * row_stride < 2^30.
  */
 typedef struct bonsai_b1_kv_pages {
     void *k, *v;          /* device */

@@ -51,3 +51,27 @@ def test_split_windows(torch, b1, case):
     b1.attention_paged(q, kc, vc, starts, i32(torch, kl), table, window=window, out=out, bad=bad)
     ref.check(out, want, off, dtype, "paged")
     assert int(bad) == 0
+
+
+@pytest.mark.parametrize("ql,kl,heads,kv_heads,d,window,page", [
+    ([130, 40], [400, 150], 4, 2, 128, 50, 16), ([200], [333], 2, 2, 64, 33, 4), ([90, 70], [300, 90], 4, 1, 64, 77, 1),
+    ([150], [2100], 2, 1, 256, 300, 2), ([129, 60], [5000, 4000], 8, 8, 128, 2000, 16), ([3, 1], [500, 90], 8, 2, 128, 45, 16),
+    ([1], [3000], 4, 4, 64, 1030, 1)])
+def test_pages_that_a_window_left(torch, b1, ql, kl, heads, kv_heads, d, window, page):
+    """Pages before the first key that any of a call's tokens sees may be gone:
+    their table entries are anything, what they held too."""
+    say(f"pages left {ql} {kl} {d} {window} {page}")
+    q, k, v = make(torch, 52, ql, kl, heads, kv_heads, d, torch.float16)
+    want, off = expect(torch, q, k, v, ql, kl, d ** -0.5, window)
+    kc, vc, table = paged(torch, 8, k, v, kl, page, "head")
+    gone = 0
+    for b, (n, m) in enumerate(zip(ql, kl)):
+        for j in range(max(0, m - n - window + 1) // page):  # all keys before the first token's window
+            kc[table[b, j]], vc[table[b, j]] = float("nan"), float("nan")
+            table[b, j] = (-1, 1 << 30)[j % 2]
+            gone += 1
+    assert gone > 0
+    bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = b1.attention_paged(q, kc, vc, i32(torch, ref.starts(ql)), i32(torch, kl), table, window=window, bad=bad)
+    ref.check(out, want, off, torch.float16, "rows")
+    assert int(bad) == 0
