@@ -716,6 +716,15 @@ def _counter(t):
     return t.data_ptr()
 
 
+def _workspace(t):
+    """Pointer and bytes of a workspace (None: none)."""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():  # an expanded one has more elements than memory
+        raise ValueError("workspace must be contiguous")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
 def _packed_rows(packed, ldp, rows, cols, stream, device):
     """A packed output (True: a new one) and its row stride in fp16 elements."""
     if packed is True:
@@ -920,8 +929,7 @@ def _attention(q, k, v, pages, kv_heads, q_start, kv_start, n_seqs, causal, wind
                          heads, kv_heads, d, tokens, kv_tokens, n_seqs, _i32_vector(q_start, None, "q_start"),
                          _i32_vector(kv_start, n_seqs + 1, "kv_start"), kv_p, 1 if causal else 0, min(window, 1 << 30),
                          scale if scale is not None else d ** -0.5, y.data_ptr(), ldo, form, _counter(bad))
-    ws, wsb = (workspace.data_ptr(), workspace.numel() * workspace.element_size()) if workspace is not None \
-        else (None, 0)
+    ws, wsb = _workspace(workspace)
     st = _lib.bonsai_b1_attention(ctypes.byref(args), ws, wsb, _raw_stream(stream, dev))
     if st != OK:
         raise B1Error(st, "bonsai_b1_attention")

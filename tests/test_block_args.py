@@ -139,3 +139,14 @@ def test_rms_norm_launches_fit(lib, h):
     rows = lib.b1_rms_norm_launch(h, ctypes.byref(threads), ctypes.byref(per))
     assert rows % per.value == 0 and 1 << 21 <= rows < 1 << 31
     assert rows // per.value * threads.value < 1 << 32
+
+
+def test_python_refuses_workspaces_smaller_than_their_elements():
+    import torch
+    buf = torch.zeros(64, dtype=torch.uint8)
+    assert capi._workspace(None) == (None, 0)
+    assert capi._workspace(buf[8:40]) == (buf.data_ptr() + 8, 32)
+    assert capi._workspace(buf.float().view(8, 8)[2:4])[1] == 64
+    for t in (buf[:1].expand(1 << 20), buf[::2], buf.view(8, 8).t()):
+        with pytest.raises(ValueError):
+            capi._workspace(t)
