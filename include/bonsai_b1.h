@@ -675,8 +675,9 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * of those; a token that sees none, or whose scores are all -inf, gets
  * zeros.  Masked and absent keys do not reach the output, whatever they hold.  Rows of no sequence are left as
  * they were.
- * Scores and sums are fp32; softmax weights are rounded to the inputs' type
- * for the product with v.  out: rows of heads * head_dim in the inputs' type
+ * Scores and sums are fp32 (a row with a scaled score past its range comes
+ * out NaN); softmax weights are rounded to the inputs' type for the product
+ * with v.  out: rows of heads * head_dim in the inputs' type
  * (packed = 0), or the packed fp16 activations of the next B1_0 linear
  * (packed = 1: bonsai_b1_pack_act_f16_ld's layout with row stride ldo, so
  * that `out` may be a column range of wider activations), as the attention

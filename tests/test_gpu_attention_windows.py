@@ -75,3 +75,30 @@ def test_pages_that_a_window_left(torch, b1, ql, kl, heads, kv_heads, d, window,
     out = b1.attention_paged(q, kc, vc, i32(torch, ref.starts(ql)), i32(torch, kl), table, window=window, bad=bad)
     ref.check(out, want, off, torch.float16, "rows")
     assert int(bad) == 0
+
+
+@pytest.mark.parametrize("ql,kl", [([40], [40]), ([90, 33], [3000, 2000]), ([2, 1], [30, 3000])])
+def test_scores_past_fp32(torch, b1, ql, kl):
+    """A score that only its scale takes past fp32's range gives NaN, never
+    the zeros of a row that sees nothing; rows that do not see it are right."""
+    say(f"scores past fp32 {ql} {kl}")
+    heads, d = 2, 64
+    q, k, v = make(torch, 53, ql, kl, heads, heads, d, torch.bfloat16)
+    q[..., 1:] *= 2.0 ** -6
+    q[..., 0], k[..., 0] = 2.0 ** 60, 0.0
+    last = ref.starts(kl)[1] - 1
+    k[last, 0, 0] = 2.0 ** 66  # seen by the first sequence's last token: 2^126, times 16 log2(e)
+    out = b1.attention(q, k, v, i32(torch, ref.starts(ql)), i32(torch, ref.starts(kl)), causal=True, scale=16.0)
+    row = ql[0] - 1
+    assert bool(out[row, 0].isnan().all())
+    rest = torch.ones(out.shape[:2], dtype=torch.bool)
+    rest[row, 0] = False
+    assert bool(out.cpu()[rest].isfinite().all())
+    k[last, 0, 0] = 0.0
+    want, off = [], []
+    for a, b, n, m in zip(ref.starts(ql), ref.starts(kl), ql, kl):
+        o, e = ref.attention(q[a:a + n].cpu(), k[b:b + m].cpu(), v[b:b + m].cpu(), 16.0, True)
+        want.append(o)
+        off.append(e)
+    want, off = torch.cat(want), torch.cat(off)
+    ref.check(out.cpu()[rest], want[rest], off[rest], torch.bfloat16, "rows that do not see it")
