@@ -692,9 +692,12 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * aligned) for calls whose keys are split over work-groups, or NULL for the
  * library's per-stream workspace, with the rules of bonsai_b1_linear_f32's
  * for captures.  Without one (a capture never allocates), or with one too
- * small, the call runs unsplit: the same values up to the order of fp32 sums, slower for few rows
- * over many keys.  A workspace serves one call at a time: give graphs that
- * may be replayed at once one each.
+ * small, the call runs unsplit, slower for few rows over many keys.  A
+ * range's softmax weights are rounded relative to the largest score it has
+ * seen, so that split and unsplit calls agree within that rounding (half a
+ * step of the inputs' type relative to each weight), not bit for bit.  A
+ * workspace serves one call at a time: give graphs that may be replayed at
+ * once one each.
  */
 typedef struct bonsai_b1_attention_args {
     const void *q, *k, *v; /* k, v unused with pages */
