@@ -117,11 +117,6 @@ __host__ __device__ __forceinline__ void visible(const AttnArgs &a, const Seq &s
     }
 }
 
-// l, or NaN where a scaled score is past fp32's range: its weight is exp2 of
-// the product less the maximum, in one instruction that does not round the
-// product, and so 0 in place of infinity less infinity.
-__device__ __forceinline__ float nan_past_fp32(float m, float l) { return m == kInf ? __builtin_nanf("") : l; }
-
 // One row in fp32 over the visible keys of [j0, j1), without matrix
 // instructions: what a tile falls back to for a row that came out
 // non-finite.  There a product of weight 0 and a masked key's infinity or NaN
@@ -144,13 +139,14 @@ __device__ void row_fp32(const AttnArgs &a, const KeyRows &kr, const KeyRows &vr
                 s += to_f32<BF>((uint16_t)(x[e] >> 16)) * to_f32<BF>((uint16_t)(y[e] >> 16));
             }
         }
-        return s * scale2;
+        s *= scale2;
+        asm("" : "+v"(s)); // rounded: past fp32's range infinity, whose weight is NaN
+        return s;
     };
     m = kLowest;
     l = 0.f;
     for (int j = j0; j < j1; ++j) m = fmaxf(m, score(j));
     for (int j = j0; j < j1; ++j) l += __builtin_amdgcn_exp2f(score(j) - m);
-    l = nan_past_fp32(m, l);
     if (l == 0.f) return;
     const float inv = 1.0f / l;
     for (int j = j0; j < j1; ++j)
@@ -758,7 +754,11 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
         for (int i = 0; i < S; ++i)
             if (tt + i < t1) stage(tt + i, i);
     }
-    l = nan_past_fp32(m, halves_sum(l));
+    l = halves_sum(l);
+    // A scaled score past fp32's range: its weight is exp2 of the product less
+    // the maximum, in one instruction that does not round the product, and so
+    // 0 in place of infinity less infinity.
+    if (m == kInf) l = __builtin_nanf("");
 
     if (__syncthreads_or(bad)) {
         bad = true;
@@ -1015,6 +1015,8 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int j = kb + 16 * kt + 4 * g + i;
+                    // (a product past fp32's range is infinity and its weight
+                    // NaN: the choice keeps it apart from the difference below)
                     sc[kt][i] = j <= hi && j >= lo && j < j1 ? sc[kt][i] * scale2 : -kInf;
                     mx = fmaxf(mx, sc[kt][i]);
                 }
@@ -1054,7 +1056,6 @@ __global__ __launch_bounds__(256) void b1_attn_few_kernel(AttnArgs a) {
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        l = nan_past_fp32(m, l);
         // the four waves' shares; register i of product e: column E (4 g + i) + e
         if (r0 > 0) __syncthreads(); // the last rows' are read
 #pragma unroll
