@@ -726,8 +726,9 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
-        // weights, rounded to the inputs' type for the product and summed as
-        // rounded; o (transposed) += v (transposed) p, 16 keys a product, in
+        // weights, rounded to the inputs' type for the product (another for
+        // what that leaves would be half as many matrix instructions again, of
+        // a kernel bound by them) and summed as rounded; o (transposed) += v (transposed) p, 16 keys a product, in
         // the order the scores' registers hold them
 #pragma unroll
         for (int x = 0; x < 2 * KT; ++x) {
@@ -830,8 +831,10 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 // matrix operand needs (values are put together from two keys' words), so
 // that a wave's 32 keys of both are in flight together.  The weights of bf16
 // inputs are two products' worth of bf16 (the value and what its rounding
-// left): 2^-16 in place of 2^-8, for a product that costs nothing beside the
-// reads.  Bound by HBM: 64 bf16 caches of 60 to 8100 keys, 1.04 GB, 210 us,
+// left): 2^-17 in place of 2^-9, for a product that costs nothing beside the
+// reads; those of fp16 inputs are rounded once, 2^-12 (two products: no time
+// at D = 64 and 128, 3 to 6 % at 256; the output's own rounding is as large).
+// Bound by HBM: 64 bf16 caches of 60 to 8100 keys, 1.04 GB, 210 us,
 // 4.9 TB/s (the rate of a large copy); one of 32700 keys, 134 MB, 27 us and a
 // join of 5.6, latency at both ends.
 constexpr int kFewRows = 16, kFewKeys = 32, kWaves = 4;
@@ -1269,7 +1272,9 @@ struct AttnPlan {
 // Calls whose sequences have up to 16 rows a key head on average run the
 // few-rows kernel, others tiles (8 sequences over 3000 keys, 8 key heads, us:
 // 16 rows 27.3, as tiles 32.0; 24 rows 42.1, 32.8; 32 sequences over 2000: 16
-// rows 52.0, 50.0; 24 rows 89.8, 50.5).  Tiles of few rounds of the device are split
+// rows 52.0, 50.0; 24 rows 89.8, 50.5; all of equal sequences: a long chunk
+// among single tokens is far from both, 63 tokens and one of 190 over 6000
+// keys 4105, apart 282 and 49).  Tiles of few rounds of the device are split
 // where that pays; of more equal ones (one sequence, every key seen) the part
 // of the last round that would leave most of the device idle.
 AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
@@ -1281,8 +1286,9 @@ AttnPlan attn_plan(const AttnArgs &a, int num_cus, bool split) {
     p.few = rows <= kFewRows * n;
     p.splits = 1;
     if (p.few) {
-        // Two work-groups a CU fit.  Where the sequences themselves make few,
-        // exactly those (32 heads over 32700 keys: 38 us, 45 with 4 a CU);
+        // Two work-groups a CU fit (one at D = 256, whose second round runs
+        // after the first).  Where the sequences themselves make few, exactly
+        // two (32 heads over 32700 keys: 38 us, 45 with 4 a CU);
         // else small pieces, so that none outlasts the rest (64 sequences of
         // 60 to 8100 keys: 215 us, 245 with 2).  Four rounds of whole sequences
         // even out by themselves (256 of 60 to 4000 keys, 8 key heads: 379 us,
