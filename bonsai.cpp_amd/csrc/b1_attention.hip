@@ -12,6 +12,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "b1_seqs.h"
@@ -510,17 +511,18 @@ __device__ __forceinline__ void copy_to_lds(u32x4 rsrc, uint8_t *lds, uint32_t o
                  : "memory");
 }
 
-// Order for the scheduler: the LDS reads (PER each) of AHEAD products, then N
-// products with a read PER each behind them while there are any.
-template <int AHEAD, int PER, int N>
+// Order for the scheduler: the LDS reads (PER each) of AHEAD products (USES
+// instructions each), then N products with a read PER each behind them while
+// there are any.
+template <int AHEAD, int PER, int N, int USES = 1>
 __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * PER, 0); // LDS reads
 #pragma unroll
     for (int i = 0; i < N - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); // matrix instructions
+        __builtin_amdgcn_sched_group_barrier(0x8, USES, 0); // matrix instructions
         __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, AHEAD * USES, 0);
 }
 
 // One pass over the keys: S^T = K Q^T by 32x32x16 products leaves a lane the
@@ -537,7 +539,15 @@ __device__ __forceinline__ void reads_ahead() {
 // %, reads of values 9 %; matrix units busy 63 % of the cycles, no bank
 // conflicts.  0.96 PFLOP/s at 4608 tokens x 24 heads of 128, 0.8 at 8191
 // causal tokens x 16 heads of 64.
-template <bool BF, int D, bool PAGED>
+//
+// FINE, for bf16 inputs and fp16 output (packed): the weights are two products'
+// worth of bf16, 2^-16 in place of 2^-8, which is eight times as coarse as the
+// output (error against 64 bits 1.00 of that of fp32 weights, 3.5 to 5 times
+// with one product).  Half as many matrix instructions again: 6000 causal
+// tokens x 16 heads of 128 241 us, with one product 178; of 64 147, 116; of
+// 256 503, 422.  fp16 weights are as fine as the output, and bf16 output as
+// coarse as the weights: one product (1.07 to 1.29 times).
+template <bool BF, int D, bool PAGED, bool FINE>
 __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kernel(AttnArgs a) {
     constexpr int ST = D / 16, DT = D / 32, CH = D / 8, KK = TileShapeOf<D>::keys, KT = KK / 32,
                   S = TileShapeOf<D>::stages, SB = KK * D * 2;
@@ -726,29 +736,36 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= alpha;
         }
-        // weights, rounded to the inputs' type for the product (another for
-        // what that leaves would be half as many matrix instructions again, of
-        // a kernel bound by them) and summed as rounded; o (transposed) += v (transposed) p, 16 keys a product, in
+        // weights, rounded to the inputs' type for the product and summed as
+        // rounded, or (FINE) with another product for what the rounding left;
+        // o (transposed) += v (transposed) p, 16 keys a product, in
         // the order the scores' registers hold them
 #pragma unroll
         for (int x = 0; x < 2 * KT; ++x) {
-            u32x4 pf;
+            u32x4 pf, pr;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 8 * (x & 1) + 2 * e;
                 const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x / 2][i], scale2, -m));
                 const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[x / 2][i + 1], scale2, -m));
                 pf[e] = pack_16<BF>(p0, p1);
-                l = add_pair<BF>(pf[e], l);
+                if constexpr (FINE) {
+                    l += p0 + p1;
+                    pr[e] = pack_16<BF>(p0 - to_f32<BF>((uint16_t)pf[e]), p1 - to_f32<BF>((uint16_t)(pf[e] >> 16)));
+                } else {
+                    l = add_pair<BF>(pf[e], l);
+                }
             }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const uint8_t *at = vs + 16 * x * (D * 2) + va[dt];
                 const u32x2 y = read_columns(at), z = read_columns(at + 8 * (D * 2));
-                o[dt] = mfma32<BF>(u32x4{y[0], y[1], z[0], z[1]}, pf, o[dt]);
+                const u32x4 vf = {y[0], y[1], z[0], z[1]};
+                o[dt] = mfma32<BF>(vf, pf, o[dt]);
+                if constexpr (FINE) o[dt] = mfma32<BF>(vf, pr, o[dt]);
             }
         }
-        reads_ahead<2, 2, 2 * KT * DT>();
+        reads_ahead<2, 2, 2 * KT * DT, FINE ? 2 : 1>();
     };
     for (int tt = t0; tt < t1; tt += S) {
 #pragma unroll
@@ -831,8 +848,8 @@ __global__ __launch_bounds__(256, TileShapeOf<D>::waves) void b1_attn_tile_kerne
 // matrix operand needs (values are put together from two keys' words), so
 // that a wave's 32 keys of both are in flight together.  The weights of bf16
 // inputs are two products' worth of bf16 (the value and what its rounding
-// left): 2^-17 in place of 2^-9, for a product that costs nothing beside the
-// reads; those of fp16 inputs are rounded once, 2^-12 (two products: no time
+// left): 2^-16 in place of 2^-8, for a product that costs nothing beside the
+// reads; those of fp16 inputs are rounded once, 2^-11 (two products: no time
 // at D = 64 and 128, 3 to 6 % at 256; the output's own rounding is as large).
 // Bound by HBM: 64 bf16 caches of 60 to 8100 keys, 1.04 GB, 210 us,
 // 4.9 TB/s (the rate of a large copy); one of 32700 keys, 134 MB, 27 us and a
@@ -1412,10 +1429,17 @@ hipError_t launch(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
         else
             hipLaunchKernelGGL((b1_attn_few_kernel<BF, D, false>), grid, block, 0, s, a);
     } else {
-        if (a.seqs.pages)
-            hipLaunchKernelGGL((b1_attn_tile_kernel<BF, D, true>), grid, block, 0, s, a);
+        auto run = [&](auto fine) {
+            constexpr bool FINE = decltype(fine)::value;
+            if (a.seqs.pages)
+                hipLaunchKernelGGL((b1_attn_tile_kernel<BF, D, true, FINE>), grid, block, 0, s, a);
+            else
+                hipLaunchKernelGGL((b1_attn_tile_kernel<BF, D, false, FINE>), grid, block, 0, s, a);
+        };
+        if (BF && a.packed)
+            run(std::bool_constant<BF>());
         else
-            hipLaunchKernelGGL((b1_attn_tile_kernel<BF, D, false>), grid, block, 0, s, a);
+            run(std::false_type());
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;

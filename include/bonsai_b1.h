@@ -680,7 +680,7 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * sequence are left as they were.
  * Scores and sums are fp32 (a row with a scaled score past its range comes
  * out NaN); softmax weights are rounded to the inputs' type for the product
- * with v.  out: rows of heads * head_dim in the inputs' type
+ * with v, those of bf16 inputs to twice its bits where out is packed (fp16).  out: rows of heads * head_dim in the inputs' type
  * (packed = 0), or the packed fp16 activations of the next B1_0 linear
  * (packed = 1: bonsai_b1_pack_act_f16_ld's layout with row stride ldo, so
  * that `out` may be a column range of wider activations), as the attention
@@ -703,8 +703,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * for captures.  Without one (a capture never allocates), or with one too
  * small, the call runs unsplit, slower for few rows over many keys.  A
  * range's softmax weights are rounded relative to the largest score it has
- * seen, so that split and unsplit calls agree within that rounding (half a
- * step of the inputs' type relative to each weight), not bit for bit.  A
+ * seen, so that split and unsplit calls agree within that rounding, not bit
+ * for bit.  A
  * workspace serves one call at a time: give graphs that may be replayed at
  * once one each.
  */
