@@ -704,9 +704,8 @@ int bonsai_b1_qkv_rope(const bonsai_b1_qkv_args *args, hipStream_t stream);
  * small, the call runs unsplit, slower for few rows over many keys.  A
  * range's softmax weights are rounded relative to the largest score it has
  * seen, so that split and unsplit calls agree within that rounding, not bit
- * for bit.  A
- * workspace serves one call at a time: give graphs that may be replayed at
- * once one each.
+ * for bit.  A workspace serves one call at a time: give graphs that may be
+ * replayed at once one each.
  */
 typedef struct bonsai_b1_attention_args {
     const void *q, *k, *v; /* k, v unused with pages */
