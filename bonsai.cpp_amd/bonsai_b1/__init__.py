@@ -8,16 +8,19 @@ device is not gfx950, calls raise.
 from .capi import (  # noqa: F401
     B1Error,
     MODES,
+    Routes,
     SafetensorsFile,
     Weights,
     attention,
     attention_paged,
+    combine_experts,
     weights_free,
     declared_symbols,
     device_weights,
     linear_batch,
     linear_batch_workspace_bytes,
     linear_epi,
+    linear_experts,
     linear_epi_workspace_bytes,
     norm_mod,
     linear_packed_f16_epi,
@@ -40,6 +43,7 @@ from .capi import (  # noqa: F401
     qkv_rope_paged,
     quantize_f32,
     rms_norm,
+    route,
     swiglu_pack_f16,
     workspace_bytes,
 )

@@ -98,6 +98,29 @@ class AttentionArgs(ctypes.Structure):
                 ("packed", ctypes.c_int), ("bad", ctypes.c_void_p)]
 
 
+F32 = 2
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class RoutesC(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int), ("experts", ctypes.c_int), ("top_k", ctypes.c_int),
+                ("expert", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("start", ctypes.c_void_p),
+                ("order", ctypes.c_void_p), ("place", ctypes.c_void_p)]
+
+
+class RouteArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("dtype", ctypes.c_int), ("score", ctypes.c_int),
+                ("bias", ctypes.c_void_p), ("renormalize", ctypes.c_int), ("scale", ctypes.c_float),
+                ("routes", RoutesC)]
+
+
+class ExpertsArgs(ctypes.Structure):
+    _fields_ = [("routes", RoutesC), ("act", ctypes.c_void_p), ("by_token", ctypes.c_int), ("w", ctypes.c_void_p),
+                ("in_dim", ctypes.c_int), ("out_dim", ctypes.c_int), ("act_fn", ctypes.c_int),
+                ("packed", ctypes.c_void_p), ("ldp", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("ldo", ctypes.c_int64), ("nonfinite", ctypes.c_void_p), ("bad", ctypes.c_void_p)]
+
+
 def library_path() -> Path:
     return _LIB
 
@@ -208,6 +231,14 @@ def load():
     L.bonsai_b1_attention.restype = i
     L.bonsai_b1_attention_workspace_bytes.argtypes = [ctypes.POINTER(AttentionArgs)]
     L.bonsai_b1_attention_workspace_bytes.restype = ctypes.c_size_t
+    L.bonsai_b1_route.argtypes = [ctypes.POINTER(RouteArgs), vp, ctypes.c_size_t, vp]
+    L.bonsai_b1_route.restype = i
+    L.bonsai_b1_route_workspace_bytes.argtypes = [ctypes.POINTER(RouteArgs)]
+    L.bonsai_b1_route_workspace_bytes.restype = ctypes.c_size_t
+    L.bonsai_b1_linear_experts.argtypes = [ctypes.POINTER(ExpertsArgs), vp]
+    L.bonsai_b1_linear_experts.restype = i
+    L.bonsai_b1_combine_experts.argtypes = [ctypes.POINTER(RoutesC), vp, i64, i, vp, i64, vp, i64, vp, vp]
+    L.bonsai_b1_combine_experts.restype = i
     L.bonsai_b1_safetensors_open.argtypes = [ctypes.c_char_p, ctypes.POINTER(vp)]
     L.bonsai_b1_safetensors_open.restype = i
     L.bonsai_b1_safetensors_close.argtypes = [vp]
@@ -774,12 +805,12 @@ def rms_norm(x, weight=None, eps: float = 1e-6, add=None, residual=None, out=Non
     return y if residual is None else (residual, y)
 
 
-def _dtype_code(dtype):
+def _dtype_code(dtype, what="queries, keys and values are fp16 or bf16"):
     if dtype is _torch.float16:
         return F16
     if dtype is _torch.bfloat16:
         return BF16
-    raise ValueError("queries, keys and values are fp16 or bf16")
+    raise ValueError(what)
 
 
 def _kv_pages(k_cache, v_cache, kv_len, pages, n_seqs):
@@ -980,6 +1011,156 @@ def attention_paged(q, k_cache, v_cache, q_start, kv_len, pages, causal: bool = 
     kv = _kv_pages(k_cache, v_cache, kv_len, pages, n)
     return _attention(q, None, None, kv, k_cache.shape[1], q_start, None, n, causal, window, scale, out, packed, ldp,
                       bad, workspace, stream, dev)
+
+
+class Routes:
+    """The routes of a call's tokens through their experts, in device memory:
+    expert and weight [tokens, top_k] (int32, -1: no route; fp32), start
+    [experts + 1], order [tokens * top_k] (the rows' slots token * top_k + j,
+    expert by expert) and place [tokens, top_k] (the slots' rows), int32.
+    route() makes one; linear_experts() and combine_experts() read it."""
+
+    __slots__ = ("expert", "weight", "start", "order", "place")
+
+    def __init__(self, expert, weight, start, order, place):
+        self.expert, self.weight, self.start, self.order, self.place = expert, weight, start, order, place
+
+    @property
+    def tokens(self):
+        return self.expert.shape[0]
+
+    @property
+    def top_k(self):
+        return self.expert.shape[1]
+
+    @property
+    def experts(self):
+        return self.start.shape[0] - 1
+
+
+def _routes_c(r):
+    """The bonsai_b1_routes of a Routes."""
+    if r.expert.dim() != 2 or r.start.dim() != 1 or r.order.dim() != 1:
+        raise ValueError("expert must be [tokens, top_k], start and order vectors")
+    tokens, k = r.expert.shape
+    for t, shape, dtype, what in ((r.expert, (tokens, k), _torch.int32, "expert"),
+                                  (r.weight, (tokens, k), _torch.float32, "weight"),
+                                  (r.place, (tokens, k), _torch.int32, "place"),
+                                  (r.order, (tokens * k,), _torch.int32, "order"),
+                                  (r.start, r.start.shape, _torch.int32, "start")):
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"routes: {what} must be contiguous {dtype} {list(shape)}")
+    # (ctypes cuts integers to the field's width: the limits of the C entries)
+    if (tokens | k | r.start.numel()) >> 24:
+        raise ValueError("tokens * top_k is limited to 2^24, experts to 1024")
+    return RoutesC(tokens, r.start.numel() - 1, k, r.expert.data_ptr(), r.weight.data_ptr(), r.start.data_ptr(),
+                   r.order.data_ptr(), r.place.data_ptr())
+
+
+def route(logits, top_k: int, score: str = "softmax", bias=None, renormalize: bool = True, scale: float = 1.0,
+          out=None, workspace=None, stream=None):
+    """The router's choice (bonsai_b1_route): logits [tokens, experts] fp32,
+    fp16 or bf16 -> Routes with each token's top_k experts and weights and the
+    experts' rows.  score: "softmax" over all experts or "sigmoid"; bias fp32
+    [experts] is added to the scores for the choice alone; renormalize
+    divides by the sum of the chosen scores.  Experts whose logit is -inf are
+    never chosen.  out: the Routes to write."""
+    lib = _lib or load()
+    if logits.dim() != 2:
+        raise ValueError("logits must be [tokens, experts]")
+    tokens, experts = logits.shape
+    if not 1 <= top_k <= experts or tokens * top_k >> 24 or experts > 1024:
+        raise ValueError("top_k is 1 to the experts, tokens * top_k below 2^24, experts at most 1024")
+    code = F32 if logits.dtype is _torch.float32 else _dtype_code(logits.dtype, "logits are fp32, fp16 or bf16")
+    dev = _on_current_device(logits, bias, workspace,
+                             *((out.expert, out.weight, out.start, out.order, out.place) if out is not None else ()))
+    ld, unit = logits.stride()
+    if unit != 1 and experts > 1:
+        raise ValueError("logits must have unit column stride")
+    if out is None:
+        i32 = _torch.int32
+        out = Routes(_empty(stream, (tokens, top_k), i32, dev), _empty(stream, (tokens, top_k), _torch.float32, dev),
+                     _empty(stream, (experts + 1,), i32, dev), _empty(stream, (tokens * top_k,), i32, dev),
+                     _empty(stream, (tokens, top_k), i32, dev))
+    routes = _routes_c(out)
+    if (routes.tokens, routes.experts, routes.top_k) != (tokens, experts, top_k):
+        raise ValueError("out is of other tokens, experts or top_k")
+    args = RouteArgs(logits.data_ptr(), ld if tokens > 1 else experts, code, SCORES[score],
+                     _f32_vector(bias, experts, "bias"), 1 if renormalize else 0, scale, routes)
+    ws, wsb = _workspace(workspace)
+    st = lib.bonsai_b1_route(ctypes.byref(args), ws, wsb, _raw_stream(stream, dev))
+    if st != OK:
+        raise B1Error(st, "bonsai_b1_route")
+    return out
+
+
+def linear_experts(packed_act, w_packed, routes, in_dim: int, out_dim: int, act: str = "none", rows: str = "tokens",
+                   out=None, packed=None, ldp=None, nonfinite=None, bad=None, stream=None):
+    """The B1_0 linear of each route's expert (bonsai_b1_linear_experts):
+    packed_act holds packed fp16 activations of in_dim, a row a token
+    (rows="tokens", the up projections) or a row a route in the experts'
+    order (rows="routes", the down projections); w_packed the experts' weight
+    rows back to back, out_dim each.  Returns y [tokens * top_k, out_dim] fp32
+    in the experts' order, or, with packed=True or a uint8 tensor (with ldp a
+    view at the target columns), the packed fp16 activations of act(y)
+    ("none", "gelu_tanh", or "swiglu" over [gate | value])."""
+    lib = _lib or load()
+    if packed is False:
+        packed = None
+    if rows not in ("tokens", "routes"):
+        raise ValueError('rows is "tokens" or "routes"')
+    dev = _on_current_device(packed_act, w_packed, routes.expert, routes.weight, routes.start, routes.order,
+                             routes.place, out, packed if packed is not True else None, nonfinite, bad)
+    c = _routes_c(routes)
+    n = c.tokens * c.top_k
+    if in_dim <= 0 or out_dim <= 0 or (in_dim | out_dim) >> 31:
+        raise ValueError("in_dim and out_dim are positive")
+    if not packed_act.is_contiguous() or packed_act.numel() * packed_act.element_size() < \
+            (c.tokens if rows == "tokens" else n) * in_dim * 2:
+        raise ValueError("packed_act must hold the rows' in_dim fp16 elements, contiguous")
+    if w_packed.dtype is not _torch.uint8 or not w_packed.is_contiguous() or \
+            w_packed.numel() != c.experts * out_dim * (in_dim // BLOCK_SIZE) * BLOCK_BYTES:
+        raise ValueError("w_packed must be contiguous uint8 of experts * out_dim * in_dim/32 * 6 bytes")
+    cols = out_dim // 2 if act == "swiglu" else out_dim
+    p = o = None
+    ldo = 0
+    if packed is not None:
+        if out is not None:
+            raise ValueError("one of out and packed")
+        y, ldp = _packed_rows(packed, ldp, n, cols, stream, dev)
+        p = y.data_ptr()
+    else:
+        y = out if out is not None else _empty(stream, (n, out_dim), _torch.float32, dev)
+        o, ldo, ldp = y.data_ptr(), _f32_rows(y, n, out_dim, "out"), 0
+    args = ExpertsArgs(c, packed_act.data_ptr(), 1 if rows == "tokens" else 0, w_packed.data_ptr(), in_dim, out_dim,
+                       ACTS[act], p, ldp, o, ldo, _counter(nonfinite), _counter(bad))
+    st = lib.bonsai_b1_linear_experts(ctypes.byref(args), _raw_stream(stream, dev))
+    if st != OK:
+        raise B1Error(st, "bonsai_b1_linear_experts")
+    return y
+
+
+def combine_experts(y, routes, residual=None, out=None, bad=None, stream=None):
+    """residual + the weighted sum of each token's rows of y
+    (bonsai_b1_combine_experts): y [tokens * top_k, H] fp32 in the experts'
+    order, as linear_experts gives it; residual [tokens, H] fp32 or None; out
+    may be residual.  Returns out [tokens, H]."""
+    lib = _lib or load()
+    dev = _on_current_device(y, routes.expert, routes.weight, routes.start, routes.order, routes.place, residual, out,
+                             bad)
+    c = _routes_c(routes)
+    if y.dim() != 2:
+        raise ValueError("y must be [tokens * top_k, H]")
+    h = y.shape[1]
+    ldy = _f32_rows(y, c.tokens * c.top_k, h, "y")
+    r_p, ldr = (residual.data_ptr(), _f32_rows(residual, c.tokens, h, "residual")) if residual is not None else (None, 0)
+    if out is None:
+        out = _empty(stream, (c.tokens, h), _torch.float32, dev)
+    st = lib.bonsai_b1_combine_experts(ctypes.byref(c), y.data_ptr(), ldy, h, r_p, ldr, out.data_ptr(),
+                                       _f32_rows(out, c.tokens, h, "out"), _counter(bad), _raw_stream(stream, dev))
+    if st != OK:
+        raise B1Error(st, "bonsai_b1_combine_experts")
+    return out
 
 
 class SafetensorsFile:

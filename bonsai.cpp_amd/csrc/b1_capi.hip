@@ -690,6 +690,158 @@ int bonsai_b1_attention(const bonsai_b1_attention_args *args, void *workspace, s
                                                                                              : BONSAI_B1_ERR_HIP;
 }
 
+// ---- a mixture of experts ----
+
+// Counts shared by the three entries: every index of a row in 32 bits, every
+// grid within the launch limits.
+static bool routes_ok(const bonsai_b1_routes *r) {
+    if (r->tokens < 0 || r->experts <= 0 || r->experts > 1024 || r->top_k <= 0 || r->top_k > 64 ||
+        r->top_k > r->experts)
+        return false;
+    return (int64_t)r->tokens * r->top_k < (1 << 24);
+}
+
+static bool al4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+static int route_args(const bonsai_b1_route_args *g, b1::RouteArgs *a) {
+    if (!g || !routes_ok(&g->routes)) return BONSAI_B1_ERR_ARG;
+    const bonsai_b1_routes &r = g->routes;
+    if (g->dtype != BONSAI_B1_F16 && g->dtype != BONSAI_B1_BF16 && g->dtype != BONSAI_B1_F32)
+        return BONSAI_B1_ERR_ARG;
+    if (g->score != BONSAI_B1_SCORE_SOFTMAX && g->score != BONSAI_B1_SCORE_SIGMOID) return BONSAI_B1_ERR_ARG;
+    if (!(g->scale >= -3.4e38f && g->scale <= 3.4e38f)) return BONSAI_B1_ERR_ARG;
+    if (!r.start || !al4(r.start) || !al4(g->bias)) return BONSAI_B1_ERR_ARG;
+    if (r.tokens > 0) {
+        const uintptr_t unit = g->dtype == BONSAI_B1_F32 ? 3 : 1;
+        if (!g->logits || (reinterpret_cast<uintptr_t>(g->logits) & unit) || g->ld < r.experts ||
+            g->ld >= ((int64_t)1 << 38))
+            return BONSAI_B1_ERR_ARG;
+        if (!r.expert || !r.weight || !r.order || !r.place || !al4(r.expert) || !al4(r.weight) || !al4(r.order) ||
+            !al4(r.place))
+            return BONSAI_B1_ERR_ARG;
+    }
+    *a = b1::RouteArgs{};
+    a->logits = g->logits;
+    a->ld = g->ld;
+    a->type = g->dtype;
+    a->tokens = r.tokens;
+    a->experts = r.experts;
+    a->top_k = r.top_k;
+    a->sigmoid = g->score == BONSAI_B1_SCORE_SIGMOID;
+    a->renormalize = g->renormalize != 0;
+    a->bias = g->bias;
+    a->scale = g->scale;
+    a->expert = r.expert;
+    a->weight = r.weight;
+    a->start = r.start;
+    a->order = r.order;
+    a->place = r.place;
+    return BONSAI_B1_OK;
+}
+
+size_t bonsai_b1_route_workspace_bytes(const bonsai_b1_route_args *args) {
+    b1::RouteArgs a;
+    return route_args(args, &a) == BONSAI_B1_OK ? b1::route_workspace_bytes(a) : 0;
+}
+
+int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace, size_t workspace_bytes, hipStream_t stream) {
+    b1::RouteArgs a;
+    const int st = route_args(args, &a);
+    if (st != BONSAI_B1_OK) return st;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u) return BONSAI_B1_ERR_ARG;
+    DeviceInfo *dev = current_device(nullptr);
+    if (!dev) return BONSAI_B1_ERR_DEVICE;
+    WsLease lease;
+    if (!workspace) {
+        workspace_bytes = b1::route_workspace_bytes(a);
+        if (workspace_bytes > 0) {
+            lease.acquire(dev, stream, workspace_bytes);
+            workspace = lease.ptr();
+        }
+    }
+    // (no tokens: the starts are still written)
+    return b1::launch_route(a, workspace, workspace_bytes, stream) == hipSuccess ? BONSAI_B1_OK : BONSAI_B1_ERR_HIP;
+}
+
+int bonsai_b1_linear_experts(const bonsai_b1_experts_args *g, hipStream_t stream) {
+    if (!g || !routes_ok(&g->routes)) return BONSAI_B1_ERR_ARG;
+    const bonsai_b1_routes &r = g->routes;
+    if (g->in_dim <= 0 || g->in_dim % 64 || g->in_dim > b1::kExpertsMaxK || g->out_dim <= 0 ||
+        (int64_t)(g->in_dim / 32) * 6 * g->out_dim >= ((int64_t)1 << 31))
+        return BONSAI_B1_ERR_ARG;
+    if (!al4(g->nonfinite) || !al4(g->bad) || !al4(r.start) || !al4(r.order)) return BONSAI_B1_ERR_ARG;
+    b1::ExpertArgs a{};
+    const int routes = r.tokens * r.top_k;
+    if (g->packed) {
+        if (g->out) return BONSAI_B1_ERR_ARG;
+        const bool glu = g->act_fn == BONSAI_B1_ACT_SWIGLU;
+        if (!glu && g->act_fn != BONSAI_B1_ACT_NONE && g->act_fn != BONSAI_B1_ACT_GELU_TANH) return BONSAI_B1_ERR_ARG;
+        if (g->out_dim % (glu ? 64 : 32)) return BONSAI_B1_ERR_ARG;
+        if (!rows_ok(g->packed, g->ldp, glu ? g->out_dim / 2 : g->out_dim, 8) || !stride_ok(g->ldp))
+            return BONSAI_B1_ERR_ARG;
+        a.kind = glu ? 3 : g->act_fn == BONSAI_B1_ACT_GELU_TANH ? 2 : 1;
+        a.glu_h = glu ? g->out_dim / 2 : 0;
+        a.pk = static_cast<uint32_t *>(g->packed);
+        a.ldpw = g->ldp / 2;
+    } else {
+        if (g->act_fn != BONSAI_B1_ACT_NONE) return BONSAI_B1_ERR_ARG;
+        if (routes > 0 && (!g->out || !al4(g->out))) return BONSAI_B1_ERR_ARG;
+        if (g->ldo < g->out_dim || g->ldo >= ((int64_t)1 << 38)) return BONSAI_B1_ERR_ARG;
+        a.out = g->out;
+        a.ldo = g->ldo;
+        a.vec = !(reinterpret_cast<uintptr_t>(g->out) & 15u) && g->ldo % 4 == 0;
+    }
+    if (routes > 0 && (!r.start || (g->by_token && !r.order) || !rows_ok(g->act, g->in_dim, g->in_dim, 8) || !g->w ||
+                       !al4(g->w)))
+        return BONSAI_B1_ERR_ARG;
+    DeviceInfo *dev = current_device(nullptr);
+    if (!dev) return BONSAI_B1_ERR_DEVICE;
+    if (routes == 0) return BONSAI_B1_OK;
+    a.act = static_cast<const uint16_t *>(g->act);
+    a.w = static_cast<const uint8_t *>(g->w);
+    a.K = g->in_dim;
+    a.N = g->out_dim;
+    a.experts = r.experts;
+    a.routes = routes;
+    a.top_k = r.top_k;
+    a.start = r.start;
+    a.order = g->by_token ? r.order : nullptr;
+    a.nonfinite = g->nonfinite;
+    a.bad = g->bad;
+    return b1::launch_experts(a, dev->num_cus, stream) == hipSuccess ? BONSAI_B1_OK : BONSAI_B1_ERR_HIP;
+}
+
+int bonsai_b1_combine_experts(const bonsai_b1_routes *r, const float *y, int64_t ldy, int H, const float *residual,
+                              int64_t ldr, float *out, int64_t ldo, int32_t *bad, hipStream_t stream) {
+    if (!r || !routes_ok(r) || H <= 0 || H % 4 || !al4(bad)) return BONSAI_B1_ERR_ARG;
+    if (r->tokens > 0) {
+        const int64_t most = (int64_t)1 << 38;
+        if (!rows_ok(y, ldy, H, 4) || !rows_ok(out, ldo, H, 4) || ldy >= most || ldo >= most)
+            return BONSAI_B1_ERR_ARG;
+        if (residual && (!rows_ok(residual, ldr, H, 4) || ldr >= most)) return BONSAI_B1_ERR_ARG;
+        // in place: a value is read before it is written
+        if (residual == out && ldr != ldo) return BONSAI_B1_ERR_ARG;
+        if (!r->weight || !r->place || !al4(r->weight) || !al4(r->place)) return BONSAI_B1_ERR_ARG;
+    }
+    if (!current_device(nullptr)) return BONSAI_B1_ERR_DEVICE;
+    if (r->tokens == 0) return BONSAI_B1_OK;
+    b1::CombineArgs a{};
+    a.y = y;
+    a.ldy = ldy;
+    a.tokens = r->tokens;
+    a.top_k = r->top_k;
+    a.routes = r->tokens * r->top_k;
+    a.H = H;
+    a.weight = r->weight;
+    a.place = r->place;
+    a.residual = residual;
+    a.ldr = ldr;
+    a.out = out;
+    a.ldo = ldo;
+    a.bad = bad;
+    return b1::launch_combine(a, stream) == hipSuccess ? BONSAI_B1_OK : BONSAI_B1_ERR_HIP;
+}
+
 int bonsai_b1_quantize_f32(const float *w, int64_t ldw, int in_dim, int out_dim, void *packed, int order,
                            hipStream_t stream) {
     if (in_dim <= 0 || out_dim < 0 || in_dim % BONSAI_B1_BLOCK_SIZE || ldw < in_dim) return BONSAI_B1_ERR_ARG;

@@ -282,6 +282,59 @@ struct QkvArgs {
 };
 hipError_t launch_qkv(const QkvArgs &a, hipStream_t s);
 
+// The router: logits [tokens][ld] (type 0 fp16, 1 bf16, 2 fp32) -> every
+// token's experts (-1: none) and weights [tokens][top_k], the experts' first
+// rows start [experts + 1], the slots (token * top_k + j) in the experts'
+// order (-1 behind the last), and each slot's row there (-1: none).
+struct RouteArgs {
+    const void *logits;
+    int64_t ld;
+    int type, tokens, experts, top_k, sigmoid, renormalize;
+    const float *bias; // [experts] or NULL
+    float scale;
+    int32_t *expert;
+    float *weight;
+    int32_t *start, *order, *place;
+};
+size_t route_workspace_bytes(const RouteArgs &a);
+// Without a workspace (NULL or too small) by one work-group.
+hipError_t launch_route(const RouteArgs &a, void *ws, size_t ws_bytes, hipStream_t s);
+
+// The linears of `experts` experts over their rows start[e] .. start[e + 1];
+// weights [experts][N][K/32*6].
+struct ExpertArgs {
+    const uint16_t *act;  // packed fp16 rows of K
+    const uint8_t *w;
+    int K, N, experts, routes, top_k;
+    const int32_t *start; // [experts + 1]
+    const int32_t *order; // row r reads activations order[r] / top_k; NULL: r
+    int kind;             // 0 fp32 rows, 1 packed, 2 packed GELU, 3 packed SwiGLU
+    float *out;
+    int64_t ldo;
+    int vec;              // out's rows are 16-byte aligned
+    uint32_t *pk;
+    int64_t ldpw;         // in dwords
+    int glu_h;            // kind 3: N / 2
+    int32_t *nonfinite, *bad;
+};
+constexpr int kExpertsMaxK = 8192;
+hipError_t launch_experts(const ExpertArgs &a, int num_cus, hipStream_t s);
+
+// out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]], rows of H.
+struct CombineArgs {
+    const float *y;
+    int64_t ldy;
+    int tokens, top_k, routes, H;
+    const float *weight;
+    const int32_t *place;
+    const float *residual; // or NULL
+    int64_t ldr;
+    float *out;
+    int64_t ldo;
+    int32_t *bad;
+};
+hipError_t launch_combine(const CombineArgs &a, hipStream_t s);
+
 // Packed B1_0 writer over device fp32 weights [N][ldw]; order 0 = numpy's
 // np.mean summation, 1 = left to right.
 hipError_t launch_quantize(const float *w, int64_t ldw, int K, int N, void *packed, int order, hipStream_t s);

@@ -728,6 +728,128 @@ int bonsai_b1_attention(const bonsai_b1_attention_args *args, void *workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * A mixture of 1-bit experts: of a block's `experts` MLPs each token goes
+ * through top_k, its routes.  Three calls around the experts' own linears:
+ *   bonsai_b1_route            router logits -> each token's experts, and the
+ *                              rows of each expert side by side
+ *   bonsai_b1_linear_experts   the B1_0 linear of each row's expert (up
+ *                              projections, then down projections)
+ *   bonsai_b1_combine_experts  each token's rows, weighted and added to the
+ *                              residual stream
+ * Slot t * top_k + j is token t's j-th route.  Nothing of the routes is
+ * needed on the host: the calls can be captured in a graph and replayed over
+ * other routes.  No reference counterpart.
+ *
+ * The arrays of a call's routes (device memory, 4-byte aligned):
+ *   expert [tokens][top_k]  the slots' experts, best first; -1: no route
+ *   weight [tokens][top_k]  their weights (0 where there is no route)
+ *   start  [experts + 1]    expert e's rows are start[e] .. start[e + 1]
+ *   order  [tokens * top_k] the rows' slots: by expert, within one by slot;
+ *                           -1 behind the last row, start[experts]
+ *   place  [tokens][top_k]  the slots' rows; -1: no route
+ * tokens * top_k < 2^24, experts <= 1024, top_k <= 64 and <= experts.
+ */
+typedef struct bonsai_b1_routes {
+    int tokens, experts, top_k;
+    int32_t *expert;
+    float *weight;
+    int32_t *start, *order, *place;
+} bonsai_b1_routes;
+
+/* The type of router logits besides BONSAI_B1_F16 and _BF16. */
+enum { BONSAI_B1_F32 = 2 };
+enum { BONSAI_B1_SCORE_SOFTMAX = 0, BONSAI_B1_SCORE_SIGMOID = 1 };
+
+/*
+ * The router's choice, from logits [tokens][ld] (of `dtype`, aligned to it).
+ * Chosen are the top_k largest logits or, with `bias` (fp32 [experts]: the
+ * correction that balances the experts' loads), the largest score + bias,
+ * computed in 64 bits; ties go to the lowest expert.  An expert whose logit
+ * (or bias) is -inf is off: never chosen, so that a token may have fewer than
+ * top_k routes, or none.  The score is the softmax over all the token's
+ * experts or the sigmoid of the logit; the weight is the chosen one's score,
+ * divided with `renormalize` by the sum of the token's chosen ones (0 where
+ * that is 0), times `scale`.  The bias is no part of it.
+ * A NaN among a token's logits or scores, or with softmax +inf, makes its weights NaN (NaN
+ * is chosen behind every number).
+ * Writes all arrays of `routes`, the same on every call with the same logits.
+ * workspace: bonsai_b1_route_workspace_bytes(args) bytes (16-byte aligned),
+ * or NULL for the library's per-stream workspace, with the rules of
+ * bonsai_b1_linear_f32's for captures.  Without one, or with one too small,
+ * one work-group routes all tokens, with the same results, slower (8192
+ * tokens of 128 experts: tens of times).  A workspace serves one call at a time: give
+ * graphs that may be replayed at once one each.
+ */
+typedef struct bonsai_b1_route_args {
+    const void *logits;
+    int64_t ld; /* >= experts */
+    int dtype;  /* BONSAI_B1_F16 / _BF16 / _F32 */
+    int score;  /* BONSAI_B1_SCORE_* */
+    const float *bias; /* [experts] or NULL */
+    int renormalize;
+    float scale; /* finite */
+    bonsai_b1_routes routes;
+} bonsai_b1_route_args;
+size_t bonsai_b1_route_workspace_bytes(const bonsai_b1_route_args *args);
+int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
+                    size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * y[r] = W_e a for every row r of every expert e.
+ *   act     packed fp16 activations (bonsai_b1_pack_act_f16's layout, row
+ *           stride in_dim).  by_token: a row reads its token's, order[r] /
+ *           top_k (the up projections over a norm's packed output; of
+ *           [tokens] rows), else row r (the down projections; of
+ *           tokens * top_k rows)
+ *   w       B1_0 rows of all experts back to back, [experts][out_dim]
+ *           [in_dim / 32 * 6] (bonsai_b1_weights_concat, or one tensor), 4-byte
+ *           aligned; SwiGLU: an expert's gate rows, then its value rows
+ * Output, rows in the experts' order, rows from start[experts] on left as
+ * they were: with `packed` the packed fp16 activations of `act_fn` of y
+ * (BONSAI_B1_ACT_*; row stride ldp fp16 elements, ldp >= the columns, a
+ * multiple of 8; 16-byte aligned; out_dim % 32 == 0, SwiGLU % 64), the input
+ * of the down projections; else y as fp32 in out (row stride ldo >= out_dim,
+ * 4-byte aligned; act_fn NONE).
+ * Of `routes` only start and (by_token) order are read, and tokens, experts,
+ * top_k.  in_dim % 64 == 0, in_dim <= 8192; an expert's weights below 2^31
+ * bytes.  Outputs apart from the inputs.
+ * Numbers are those of FAST mode: products of fp16 in fp32 sums, in an order
+ * that depends on tokens, experts, top_k and the widths, not on the routes.
+ * The non-finite counter counts y.  Starts out of order or range make every
+ * row of the call NaN, an order entry out of range its row; `bad` grows by at
+ * least 1 then, and nothing out of range is read or written.
+ */
+typedef struct bonsai_b1_experts_args {
+    bonsai_b1_routes routes;
+    const void *act;
+    int by_token;
+    const void *w;
+    int in_dim, out_dim;
+    int act_fn;
+    void *packed; /* or NULL */
+    int64_t ldp;
+    float *out; /* or NULL; one of packed and out */
+    int64_t ldo;
+    int32_t *nonfinite; /* device counter or NULL */
+    int32_t *bad;       /* device counter or NULL */
+} bonsai_b1_experts_args;
+int bonsai_b1_linear_experts(const bonsai_b1_experts_args *args,
+                             hipStream_t stream);
+
+/*
+ * out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]] over the token's
+ * routes, in fp32, added in the order of j: the block's output from the down
+ * projections' rows y (fp32, row stride ldy).  residual may be NULL (0) or out itself
+ * (same row stride); out is apart from y.  A place out of range makes the
+ * token's row NaN and adds to `bad`.  Of `routes` weight and place are read.
+ * H % 4 == 0; pointers 16-byte aligned, row strides multiples of 4, >= H.
+ */
+int bonsai_b1_combine_experts(const bonsai_b1_routes *routes, const float *y,
+                              int64_t ldy, int H, const float *residual,
+                              int64_t ldr, float *out, int64_t ldo,
+                              int32_t *bad, hipStream_t stream);
+
+/*
  * The B1_0 writer on the device; replaces quantize_b1_0 of
  * convert_to_b1_0_packed.py:21-43 and of tests/c_ops/test_b1_linear.cpp:
  * 129-163.  w: fp32 [out_dim][ldw] device weights (ldw >= in_dim,
