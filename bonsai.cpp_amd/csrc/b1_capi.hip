@@ -766,9 +766,11 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace, size_t wo
 int bonsai_b1_linear_experts(const bonsai_b1_experts_args *g, hipStream_t stream) {
     if (!g || !routes_ok(&g->routes)) return BONSAI_B1_ERR_ARG;
     const bonsai_b1_routes &r = g->routes;
-    if (g->in_dim <= 0 || g->in_dim % 64 || g->in_dim > b1::kExpertsMaxK || g->out_dim <= 0 ||
+    if (g->in_dim <= 0 || g->in_dim % 64 || g->in_dim > (1 << 16) || g->out_dim <= 0 || g->out_dim > (1 << 17) ||
         (int64_t)(g->in_dim / 32) * 6 * g->out_dim >= ((int64_t)1 << 31))
         return BONSAI_B1_ERR_ARG;
+    // tokens' rows by 32-bit byte offsets
+    if (g->by_token && (int64_t)r.tokens * g->in_dim >= ((int64_t)1 << 31)) return BONSAI_B1_ERR_ARG;
     if (!al4(g->nonfinite) || !al4(g->bad) || !al4(r.start) || !al4(r.order)) return BONSAI_B1_ERR_ARG;
     b1::ExpertArgs a{};
     const int routes = r.tokens * r.top_k;
@@ -798,6 +800,7 @@ int bonsai_b1_linear_experts(const bonsai_b1_experts_args *g, hipStream_t stream
     if (!dev) return BONSAI_B1_ERR_DEVICE;
     if (routes == 0) return BONSAI_B1_OK;
     a.act = static_cast<const uint16_t *>(g->act);
+    a.act_rows = g->by_token ? r.tokens : routes;
     a.w = static_cast<const uint8_t *>(g->w);
     a.K = g->in_dim;
     a.N = g->out_dim;

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "b1_device.h"
@@ -336,48 +337,113 @@ __global__ __launch_bounds__(kRouteThreads) void b1_route_place_kernel(RouteArgs
 
 // ------------------------------------------------------ groups of rows ----
 
-// Rows of an expert: up to `most` of them from row0 on.
+// How many groups of up to BM rows of one expert there are, counting through
+// the experts in order, and lane l's share: experts l * each .. of them, the
+// first's rows from edge[0] on and its groups `before` the next lane's.  By a
+// whole wave.  Starts are brought into range and order first, so that any
+// contents of `start` give groups within the rows, apart from one another, and
+// no more of them than group_bound() says.  Up to 256 experts a lane keeps its
+// experts' edges (its loads all on their way at once), with more it reads them
+// again in find_group().
+constexpr int kEdges = 4;
+struct Groups {
+    uint32_t edge[kEdges + 1], before, total;
+    int each;
+    bool bad; // starts out of order or of range
+};
+template <int BM>
+__device__ __forceinline__ Groups count_groups(const int32_t *start, int experts, int routes) {
+    const int lane = threadIdx.x & 63;
+    Groups g;
+    g.each = (experts + 63) / 64;
+    const int e0 = min(lane * g.each, experts), e1 = min(e0 + g.each, experts);
+    auto within = [&](int v) { return (uint32_t)min(max(v, 0), routes); };
+    auto groups = [&](uint32_t rows) { return (rows + BM - 1) / BM; };
+    bool bad;
+    uint32_t top, n = 0;
+    if (g.each <= kEdges) {
+        int v[kEdges + 1];
+#pragma unroll
+        for (int i = 0; i <= kEdges; ++i) v[i] = start[min(e0 + i, e1)];
+        bad = v[0] < 0 || v[kEdges] > routes;
+#pragma unroll
+        for (int i = 0; i < kEdges; ++i) bad |= v[i + 1] < v[i];
+        g.edge[0] = within(v[0]);
+#pragma unroll
+        for (int i = 1; i <= kEdges; ++i) g.edge[i] = max(g.edge[i - 1], within(v[i]));
+        top = g.edge[kEdges];
+    } else {
+        int last = start[e0];
+        bad = last < 0;
+        top = g.edge[0] = within(last);
+        for (int e = e0; e < e1; ++e) {
+            const int v = start[e + 1];
+            bad |= v < last;
+            last = v;
+            top = max(top, within(v));
+        }
+        bad |= last > routes;
+    }
+    g.bad = __ballot(bad) != 0;
+    if (g.bad) { // no start before an earlier one
+        const uint32_t floor = __shfl_up(scan_max(top), 1);
+        if (lane) g.edge[0] = max(g.edge[0], floor);
+#pragma unroll
+        for (int i = 1; i <= kEdges; ++i) g.edge[i] = max(g.edge[i], g.edge[0]);
+    }
+    if (g.each <= kEdges) {
+#pragma unroll
+        for (int i = 0; i < kEdges; ++i) n += groups(g.edge[i + 1] - g.edge[i]);
+    } else {
+        uint32_t row = g.edge[0];
+        for (int e = e0; e < e1; ++e) {
+            const uint32_t end = max(row, within(start[e + 1]));
+            n += groups(end - row);
+            row = end;
+        }
+    }
+    g.before = scan_add(n);
+    g.total = lane_value(g.before, 63);
+    g.before -= n;
+    return g;
+}
+
+// The t-th of them (t < total).
 struct Group {
     int expert, row0, rows;
-    bool bad; // the starts of the experts' rows are out of order or of range
 };
-
-// The t-th group of up to BM rows of one expert, counting through the experts
-// in order, and how many groups there are (*groups); by a whole wave.  Starts
-// are brought into range and order first, so that any contents of `start` give
-// groups within the rows, apart from one another, and no more of them than
-// group_bound() says.
 template <int BM>
-__device__ __forceinline__ Group find_group(const int32_t *start, int experts, int routes, int t, int *groups) {
-    const int lane = threadIdx.x & 63;
-    Group found = {0, 0, 0, false};
-    uint32_t before = 0, floor = 0;
-    for (int e0 = 0; e0 < experts; e0 += 64) {
-        const int e = min(e0 + lane, experts - 1);
-        const int a = start[e], b = start[e + 1];
-        const bool there = e0 + lane < experts;
-        found.bad |= __ballot(a < 0 || b < a || b > routes) != 0;
-        uint32_t s0 = (uint32_t)min(max(a, 0), routes), s1 = (uint32_t)min(max(b, 0), routes);
-        if (found.bad) { // no start before an earlier one
-            s0 = scan_max(max(s0, floor));
-            s1 = scan_max(max(s1, s0));
-            floor = lane_value(s1, 63);
+__device__ __forceinline__ Group find_group(const Groups &g, const int32_t *start, int experts, int routes, int t) {
+    // the last lane with no more groups before it that has some itself
+    const uint64_t who = __ballot(g.before <= (uint32_t)t);
+    const int l = 63 - __builtin_clzll(who);
+    uint32_t left = (uint32_t)t - lane_value(g.before, l), row = lane_value(g.edge[0], l), end = row;
+    int e = l * g.each;
+    if (g.each <= kEdges) {
+#pragma unroll
+        for (int i = 0; i < kEdges; ++i) {
+            const uint32_t to = lane_value(g.edge[i + 1], l), n = (to - row + BM - 1) / BM;
+            if (left < n) {
+                end = to;
+                break;
+            }
+            left -= n;
+            row = to;
+            ++e;
         }
-        const uint32_t rows = there ? s1 - s0 : 0u, n = (rows + BM - 1) / BM;
-        const uint32_t end = before + scan_add(n);
-        const uint64_t who = __ballot((uint32_t)t >= end - n && (uint32_t)t < end);
-        if (who) {
-            const int l = __builtin_ctzll(who);
-            const uint32_t first = lane_value(end - n, l);
-            const uint32_t at = ((uint32_t)t - first) * BM;
-            found.expert = e0 + l;
-            found.row0 = (int)(lane_value(s0, l) + at);
-            found.rows = (int)min(lane_value(rows, l) - at, (uint32_t)BM);
+    } else {
+        for (;; ++e) {
+            end = max(row, (uint32_t)min(max(start[e + 1], 0), routes));
+            const uint32_t n = (end - row + BM - 1) / BM;
+            if (left < n || e + 1 >= experts) break;
+            left -= n;
+            row = end;
         }
-        before = lane_value(end, 63);
     }
-    *groups = (int)before;
-    return found;
+    row += left * BM;
+    // (wave-uniform: scalar registers)
+    return Group{__builtin_amdgcn_readfirstlane(e), __builtin_amdgcn_readfirstlane((int)row),
+                 __builtin_amdgcn_readfirstlane((int)min(end - row, (uint32_t)BM))};
 }
 
 // Groups of up to bm rows that `routes` rows of `experts` experts can have.
@@ -399,6 +465,23 @@ __device__ __forceinline__ floatx4 nan4() {
 // A buffer offset past any buffer: reads zeros.
 constexpr uint32_t kNowhere = 0x80000000u;
 
+// silu(x) = x / (1 + 2^(-x log2 e)) by the hardware's exponential and
+// reciprocal, which feed an fp16 rounding: within (|x| + 4) half steps of fp32.
+__device__ __forceinline__ float silu_fast(float x) {
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+}
+
+// The scheduler's order: M times an MFMA, D LDS reads and V vector operations.
+template <int M, int V, int D>
+__device__ __forceinline__ void interleave() {
+    if constexpr (M > 0) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if constexpr (D > 0) __builtin_amdgcn_sched_group_barrier(0x100, D, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, V, 0);
+        interleave<M - 1, V, D>();
+    }
+}
+
 // ------------------------------------------------ few rows an expert ----
 
 // y = W a for up to 16 rows of one expert and `per` steps of 64 weight rows.
@@ -418,11 +501,40 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
     const int bid = blockIdx.x;
-    int groups;
     const int slot = bid / parts, part = bid - slot * parts;
-    const Group gr = find_group<BM>(a.start, a.experts, a.routes, slot, &groups);
-    if (bid == 0 && threadIdx.x == 0 && gr.bad && a.bad) atomicAdd(a.bad, 1);
-    if (slot >= groups) return;
+    const Groups all = count_groups<BM>(a.start, a.experts, a.routes);
+    if (bid == 0 && threadIdx.x == 0 && all.bad && a.bad) atomicAdd(a.bad, 1);
+    if (slot >= (int)all.total) return;
+    const Group gr = find_group<BM>(all, a.start, a.experts, a.routes, slot);
+
+    const uint32_t rs = (uint32_t)(a.K / 32) * 6;
+    const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(a.w) + (size_t)gr.expert * a.N * rs, (short)0, (int)((uint32_t)a.N * rs), kBufferFlags);
+    const __amdgpu_buffer_rsrc_t none = __builtin_amdgcn_make_buffer_rsrc(nullptr, (short)0, 0, kBufferFlags);
+    const int pairs = a.K / 64; // of blocks, 12 bytes of a weight row
+    uint32_t woff[U]; // of this lane's pair within a weight row
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pair = (wave * U + u) * 4 + g;
+        woff[u] = pair < pairs ? 12u * (uint32_t)pair : kNowhere;
+    }
+    // weight rows of group nt of step s: 64 s + 16 nt, or 32 gates, then their 32 values
+    auto weight_row = [&](int s, int nt) {
+        if constexpr (OUT == 3) return 32 * s + 16 * (nt & 1) + (nt >> 1) * a.glu_h + li;
+        return 64 * s + 16 * nt + li;
+    };
+    const int s0 = part * per, s1 = min(s0 + per, OUT == 3 ? a.glu_h / 32 : (a.N + 63) / 64);
+    // (rows past the last read that again; behind the last step nothing is read)
+    auto load = [&](int s, int u, int nt) {
+        const uint32_t off = __umul24((uint32_t)min(weight_row(s, nt), a.N - 1), rs) + woff[u];
+        return __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(s < s1 ? wrs : none, (int)off, 0, 0));
+    };
+    // a step's weights, each replaced by the next step's once it is expanded
+    u32x3 w[4][U];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[nt][u] = load(s0, u, nt);
 
     // the row's activations
     int64_t src = gr.row0 + li;
@@ -432,16 +544,13 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
         wrong = s < 0 || s >= a.routes;
         src = wrong ? 0 : s / a.top_k;
     }
-    const uint32_t wrong_rows = gr.bad ? 0xffffu : (uint32_t)__ballot(wrong) & 0xffffu;
-    if (wrong_rows && !gr.bad && a.bad && part == 0 && threadIdx.x == 0) atomicAdd(a.bad, __popc(wrong_rows));
+    const uint32_t wrong_rows = all.bad ? 0xffffu : (uint32_t)__ballot(wrong) & 0xffffu;
+    if (wrong_rows && !all.bad && a.bad && part == 0 && threadIdx.x == 0) atomicAdd(a.bad, __popc(wrong_rows));
     there = there && !wrong;
-    const int pairs = a.K / 64; // of blocks, 12 bytes of a weight row
     half8 af[U][2][4];
-    uint32_t woff[U]; // of this lane's pair within a weight row
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int pair = (wave * U + u) * 4 + g;
-        woff[u] = pair < pairs ? 12u * (uint32_t)pair : kNowhere;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -452,30 +561,15 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
                 af[u][b][c] = v;
             }
     }
-    const uint32_t rs = (uint32_t)(a.K / 32) * 6;
-    const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t *>(a.w) + (size_t)gr.expert * a.N * rs, (short)0, (int)((uint32_t)a.N * rs), kBufferFlags);
-    // weight rows of group nt of step s: 64 s + 16 nt, or 32 gates, then their 32 values
-    auto weight_row = [&](int s, int nt) {
-        if constexpr (OUT == 3) return 32 * s + 16 * (nt & 1) + (nt >> 1) * a.glu_h + li;
-        return 64 * s + 16 * nt + li;
-    };
-    const int s0 = part * per, s1 = min(s0 + per, OUT == 3 ? a.glu_h / 32 : (a.N + 63) / 64);
-    u32x3 w[U][4], next[U][4];
-    auto load = [&](u32x3 (&to)[U][4], int s) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const int row = weight_row(s, nt);
-                const uint32_t off = row < a.N && woff[u] != kNowhere ? (uint32_t)row * rs + woff[u] : kNowhere;
-                to[u][nt] = __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(wrs, (int)off, 0, 0));
-            }
-    };
     int bad = 0;
-    if (s0 < s1) load(w, s0);
+    // block b of a pair's words as the operands of its four chunks
+    auto expand = [&](const u32x3 &d, int b, u32x4 (&c)[4]) {
+        const uint32_t sc = b ? dup_hi16(d[1]) : dup_lo16(d[0]);
+        const uint32_t sign = b ? d[2] : __builtin_amdgcn_alignbit(d[1], d[0], 16);
+        wpair_quads<0>(sign, sign >> 8, sc, c[0], c[2]);
+        wpair_quads<1>(sign, sign >> 8, sc, c[1], c[3]);
+    };
     for (int s = s0; s < s1; ++s) {
-        if (s + 1 < s1) load(next, s + 1);
         floatx4 acc[4];
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
@@ -484,12 +578,9 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    const u32x3 d = w[u][nt];
-                    const uint32_t sc = b ? dup_hi16(d[1]) : dup_lo16(d[0]);
-                    const uint32_t sign = b ? d[2] : __builtin_amdgcn_alignbit(d[1], d[0], 16);
                     u32x4 c[4];
-                    wpair_quads<0>(sign, sign >> 8, sc, c[0], c[2]);
-                    wpair_quads<1>(sign, sign >> 8, sc, c[1], c[3]);
+                    expand(w[nt][u], b, c);
+                    if (b == 1) w[nt][u] = load(s + 1, u, nt);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         acc[nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, c[k]), af[u][b][k],
@@ -517,8 +608,11 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
             for (int i = 0; i < 4; ++i) bad += !__builtin_isfinite(v[i]);
         };
         const bool cnt = a.nonfinite != nullptr;
+        // another wave first at each step: few rows are one wave's work, and
+        // the others go on with the next step meanwhile
+        const int item0 = (int)(threadIdx.x + 64 * (NW - (s - s0) % NW)) % (NW * 64);
         if constexpr (OUT == 0) {
-            for (int i = threadIdx.x; i < gr.rows * 16; i += NW * 64) {
+            for (int i = item0; i < gr.rows * 16; i += NW * 64) {
                 const int row = i >> 4, col = 64 * s + 4 * (i & 15);
                 if (col >= a.N) continue;
                 const floatx4 v = sum4(row, 4 * (i & 15));
@@ -538,7 +632,7 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
         } else {
             // (row, 32-column block, quad of 4 dwords)
             constexpr int Q = OUT == 3 ? 4 : 8;
-            for (int i = threadIdx.x; i < gr.rows * Q; i += NW * 64) {
+            for (int i = item0; i < gr.rows * Q; i += NW * 64) {
                 const int row = i / Q, q = i % Q, dq = (q & 3) * 4, blk = q >> 2;
                 const int col = (OUT == 3 ? 32 * s : 64 * s + 32 * blk);
                 if (OUT != 3 && col >= a.N) continue;
@@ -555,8 +649,8 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        lo[k] = mul_f32(silu_f32(lo[k]), vlo[k]);
-                        hi[k] = mul_f32(silu_f32(hi[k]), vhi[k]);
+                        lo[k] = mul_f32(silu_fast(lo[k]), vlo[k]);
+                        hi[k] = mul_f32(silu_fast(hi[k]), vhi[k]);
                     }
                 } else if constexpr (OUT == 2) {
 #pragma unroll
@@ -571,10 +665,387 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
                 *reinterpret_cast<u32x4 *>(a.pk + (size_t)(gr.row0 + row) * a.ldpw + col / 2 + dq) = v;
             }
         }
+    }
+    count_nonfinite(a.nonfinite, bad);
+}
+
+// ----------------------------------------------- many rows an expert ----
+
+// Tiles of BM rows of one expert and BN = NWN * WN weight rows.
+//
+// MFMA 16x16x32, 16 weight rows as the A operand, rows of activations as the
+// B operand.  A stage is 64 of K: BM rows of 128 bytes, shared by the waves,
+// their 16-byte chunks at c ^ row / 2 so that the 16 rows of a fragment read
+// cover all banks; and a wave's own WN columns of weights, 12 bytes a column
+// and stage, loaded L stages at once so that L lanes take adjacent bytes of a
+// row (a slice of WN / L columns a stage, a group of L stages ahead).  R
+// stages of activations in a ring, copied straight to LDS.
+template <int BM_, int WN_, int NWN_, int R_, int L_, int OCC_, int SETS_>
+struct ExpertTile {
+    static constexpr int BM = BM_, WN = WN_, NWN = NWN_, R = R_, L = L_, OCC = OCC_, SETS = SETS_;
+    static constexpr int NT = NWN * 64, BN = WN * NWN, MT = BM / 16, NTL = WN / 16;
+    static constexpr int ASZ = BM * 128;                 // bytes of a stage's activations
+    static constexpr int AW = ASZ / 1024 / NWN;          // loads of them a wave
+    static constexpr int WSL = WN * 16, WGRP = L * WSL;  // a slice, a group (16 bytes a lane's 12)
+    // groups kept: stage s + R's loads fill a slice of group (s + R) / L + 1
+    // while stage s + 1 of this and every later group is still to be read
+    static constexpr int groups() {
+        int g = 0;
+        for (int s = 0; s < 4 * L; ++s) g = (s + R) / L + 1 - (s + 1) / L > g ? (s + R) / L + 1 - (s + 1) / L : g;
+        return g + 1;
+    }
+    static constexpr int RW = groups();
+    static constexpr int WBASE = R * ASZ, LDS = WBASE + NWN * RW * WGRP;
+    static constexpr int LOADS = AW + 1;                 // a wave and stage
+    static constexpr int TOK = (BM + 63) / 64;           // of a lane
+    static_assert(ASZ % (1024 * NWN) == 0 && WN % 64 == 0 && WN % L == 0 && WN / L * L <= 64, "loads of whole waves");
+    static_assert(LDS <= 160 * 1024 && (R - 1) * LOADS < 64, "gfx950 LDS, vmcnt");
+};
+
+// Waits until at most `later` stages' loads are outstanding (later <= MAXL).
+template <int LOADS, int MAXL>
+__device__ __forceinline__ void wait_stages(int later) {
+    if constexpr (MAXL == 0) {
+        wait_vmcnt<0>();
+    } else {
+        if (later >= MAXL)
+            wait_vmcnt<LOADS * MAXL>();
+        else
+            wait_stages<LOADS, MAXL - 1>(later);
+    }
+}
+
+template <class C, int OUT>
+__global__ __launch_bounds__(C::NT, C::OCC) void b1_experts_tile_kernel(ExpertArgs a, int tiles_n) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wn = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, g = lane >> 4;
+    const Groups all = count_groups<C::BM>(a.start, a.experts, a.routes);
+    if (blockIdx.x == 0 && tid == 0 && all.bad && a.bad) atomicAdd(a.bad, 1);
+    // contiguous tiles an XCD, its work-groups taking them in turn
+    const int tiles = (int)all.total * tiles_n;
+    const int xcd = blockIdx.x & 7, each = gridDim.x >> 3;
+    const int share = tiles >> 3, more = tiles & 7;
+    const int first = xcd * share + min(xcd, more) + ((int)blockIdx.x >> 3);
+    const int last = xcd * share + min(xcd, more) + share + (xcd < more ? 1 : 0);
+    if (first >= last) return;
+
+    const int K = a.K, n = K / 64;
+    const uint32_t rs = (uint32_t)(K / 32) * 6;
+    const __amdgpu_buffer_rsrc_t none = __builtin_amdgcn_make_buffer_rsrc(nullptr, (short)0, 0, kBufferFlags);
+    __amdgpu_buffer_rsrc_t ars = none, wrs = none;
+    uint32_t aoff[C::AW], boff[C::L];
+    int expert, row0, rows, n0; // of the tile
+    uint64_t wrong[C::TOK];
+
+    // slots of a tile's rows, on their way while the one before is computed
+    int slots[C::TOK];
+    int expert_next = 0, row0_next = 0, rows_next = 0, n0_next = 0;
+    auto look_up = [&](int t) {
+        const int GM = 8, tg = t / (GM * tiles_n), first_m = tg * GM;
+        const int size = min(GM, (int)all.total - first_m), in = t - first_m * tiles_n;
+        const Group gr = find_group<C::BM>(all, a.start, a.experts, a.routes, first_m + in % size);
+        expert_next = gr.expert;
+        row0_next = gr.row0;
+        rows_next = gr.rows;
+        n0_next = in / size * C::BN;
+        if (a.order)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int i = 0; i < C::TOK; ++i) slots[i] = a.order[row0_next + min(64 * i + lane, rows_next - 1)];
+    };
+    auto swz = [](int row) { return (row >> 1) & 7; };
+    auto swl = [](int c) { return C::L == 4 ? (c >> 2) & 3 : C::L == 2 ? (c >> 3) & 1 : 0; };
+    // the weight row of a tile column
+    auto weight_row = [&](int tc) {
+        const int c = n0 + tc;
+        if constexpr (OUT == 3) {
+            // 32 gates, then their 32 values
+            const int j = min(c >> 6, a.glu_h / 32 - 1) * 32 + (c & 31);
+            return (c & 32 ? a.glu_h : 0) + j;
+        }
+        return min(c, a.N - 1);
+    };
+    // the addresses of the tile that was looked up
+    auto aim = [&]() {
+        expert = expert_next;
+        row0 = row0_next;
+        rows = rows_next;
+        n0 = n0_next;
+        int token[C::TOK];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) w[u][nt] = next[u][nt];
+        for (int i = 0; i < C::TOK; ++i) {
+            token[i] = min(64 * i + lane, rows - 1);
+            bool is = false;
+            if (a.order) {
+                is = slots[i] < 0 || slots[i] >= a.routes;
+                token[i] = is ? 0 : slots[i] / a.top_k;
+            }
+            wrong[i] = __ballot(is && 64 * i + lane < rows);
+        }
+        const uint16_t *act = a.act;
+        uint32_t bytes = (uint32_t)a.act_rows * (uint32_t)K * 2u;
+        if (!a.order) {
+            act += (size_t)row0 * K;
+            bytes = (uint32_t)rows * (uint32_t)K * 2u;
+        }
+        ars = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(act), (short)0, (int)bytes, kBufferFlags);
+        wrs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.w) + (size_t)expert * a.N * rs, (short)0,
+                                                (int)((uint32_t)a.N * rs), kBufferFlags);
+#pragma unroll
+        for (int i = 0; i < C::AW; ++i) {
+            const int row = 8 * (wn * C::AW + i) + lane / 8;
+            int tok = __shfl(token[0], row & 63);
+            if constexpr (C::TOK == 2) tok = row < 64 ? tok : __shfl(token[1], row & 63);
+            aoff[i] = ((uint32_t)tok * (uint32_t)K + (uint32_t)((lane % 8) ^ swz(row)) * 8) * 2;
+        }
+#pragma unroll
+        for (int i = 0; i < C::L; ++i) {
+            const int c = i * (C::WN / C::L) + lane / C::L;
+            boff[i] = (uint32_t)weight_row(wn * C::WN + c) * rs + 12u * (uint32_t)((lane % C::L) ^ swl(c));
+        }
+    };
+    const int last_group = (n - 1) / C::L;
+    uint8_t *const sw0 = smem + C::WBASE + wn * (C::RW * C::WGRP);
+    int wfill;
+    auto load_slice = [&](int at, int group) {
+        // (a group's stages past K: zeros past the buffer or the next row's, never used)
+        dma_buf_lds12s(wrs, sw0 + at, boff[0], (uint32_t)(min(group, last_group) * C::L * 12));
+        const uint32_t b0 = boff[0];
+#pragma unroll
+        for (int i = 0; i + 1 < C::L; ++i) boff[i] = boff[i + 1];
+        boff[C::L - 1] = b0;
+    };
+    auto issue = [&](int s, int slot) {
+        uint8_t *sa = smem + slot + wn * C::AW * 1024;
+#pragma unroll
+        for (int i = 0; i < C::AW; ++i) dma_buf_lds16s(ars, sa + i * 1024, aoff[i], (uint32_t)s * 128u);
+        load_slice(wfill, s / C::L + 1);
+        wfill = wfill + C::WSL == C::RW * C::WGRP ? 0 : wfill + C::WSL;
+    };
+    // the first stages of a tile
+    auto begin = [&]() {
+#pragma unroll
+        for (int i = 0; i < C::L; ++i) load_slice(i * C::WSL, 0);
+        wfill = C::WGRP;
+#pragma unroll
+        for (int s = 0; s < C::R; ++s)
+            if (s < n) issue(s, s * C::ASZ);
+    };
+
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+    typedef const __attribute__((address_space(3))) uint32_t lds_u32;
+    typedef __attribute__((address_space(3))) half8 lds_half8;
+    lds_u8 *const lbase = (lds_u8 *)smem;
+    lds_u8 *fa[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fa[j] = lbase + li * 128 + (((4 * j + g) ^ swz(li)) * 16);
+    lds_u8 *const qw = lbase + C::WBASE + wn * (C::RW * C::WGRP) + li * (C::L * 16);
+    const int qsw = swl(li) * 16;
+    int rgrp, rsub;
+    floatx4 acc[C::MT][C::NTL];
+    uint32_t d[C::NTL][3], s2[C::NTL], wg[C::NTL];
+    half8 af[C::SETS][C::MT];
+    auto read_weights = [&]() {
+        lds_u8 *const qp = qw + rgrp + (rsub ^ qsw);
+        rsub += 16;
+        if (rsub == 16 * C::L) {
+            rsub = 0;
+            rgrp = rgrp + C::WGRP == C::RW * C::WGRP ? 0 : rgrp + C::WGRP;
+        }
+#pragma unroll
+        for (int nt = 0; nt < C::NTL; ++nt) {
+            lds_u32 *q = (lds_u32 *)(qp + nt * (C::L * 256));
+            d[nt][0] = q[0];
+            d[nt][1] = q[1];
+            d[nt][2] = q[2];
+        }
+    };
+    auto read_rows = [&](int slot, int j) {
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) af[j][mt] = *(const lds_half8 *)(fa[j] + slot + mt * 16 * 128);
+    };
+    // the scale pairs of block j and its sign words, the lane's last pair at
+    // the sign bits, from the stage's words
+    auto scales = [&](int j) {
+#pragma unroll
+        for (int nt = 0; nt < C::NTL; ++nt) {
+            if (j == 0) {
+                s2[nt] = dup_lo16(d[nt][0]);
+                wg[nt] = __builtin_amdgcn_alignbit(d[nt][1], d[nt][0], 4 + 4 * g);
+            } else {
+                s2[nt] = dup_hi16(d[nt][1]);
+                wg[nt] = d[nt][2] << (12 - 4 * g);
+            }
+        }
+    };
+    // Every wave's part of the next stage is in LDS (its loads waited for
+    // before) and this one's reads are done, so that its slot can be filled.
+    auto publish = [&]() {
+        wait_lgkmcnt0();
+        __builtin_amdgcn_sched_barrier(0);
+        lds_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto next = [&](int slot) { return slot + C::ASZ == C::R * C::ASZ ? 0 : slot + C::ASZ; };
+    // A stage: its two blocks, 16 weight rows at a time.  What the next MFMAs
+    // need (fragments, packed words, the next 16 rows as fp16) is read and
+    // expanded while the MFMAs at hand run, a few vector operations behind
+    // each: an MFMA holds its SIMD's matrix unit for 16 cycles and the issue
+    // for 4, and what stands behind a row of MFMAs waits for all of them.
+    u32x4 bo;
+    auto stage = [&](int slot, auto &&advance) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (j == 1) { // (behind the last stage reads what is not used)
+                advance();
+                read_weights();
+            }
+            const int slot_ahead = j == 0 ? slot : next(slot);
+            if (C::SETS == 2) read_rows(slot_ahead, 1 - j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int nt = 0; nt < C::NTL; ++nt) {
+                u32x4 ahead = bo;
+                if (nt + 1 < C::NTL) {
+                    ahead = wpair4(wg[nt + 1], s2[nt + 1]);
+                } else {
+                    scales(1 - j);
+                    ahead = wpair4(wg[0], s2[0]);
+                }
+#pragma unroll
+                for (int mt = 0; mt < C::MT; ++mt) {
+                    acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(half8, bo), af[C::SETS == 2 ? j : 0][mt], acc[mt][nt], 0, 0, 0);
+                    // each fragment makes room for the next block's
+                    if (C::SETS == 1 && nt + 1 == C::NTL)
+                        af[0][mt] = *(const lds_half8 *)(fa[1 - j] + slot_ahead + mt * 16 * 128);
+                }
+                constexpr int V = (8 + C::MT - 1) / C::MT;
+                if (nt + 1 < C::NTL)
+                    interleave<C::MT, V, 0>();
+                else
+                    interleave<C::MT, 2 * V, C::SETS == 1>();
+                __builtin_amdgcn_sched_barrier(0);
+                bo = ahead;
+            }
+        }
+    };
+
+    look_up(first);
+    aim();
+    begin();
+    int bad = 0;
+    for (int t = first; t < last; t += each) {
+        if (t + each < last) look_up(t + each);
+        wait_stages<C::LOADS, C::R - 1>(n - 1);
+        publish();
+        rgrp = rsub = 0;
+        read_weights();
+        read_rows(0, 0);
+        scales(0);
+        bo = wpair4(wg[0], s2[0]);
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < C::NTL; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+        int slot = 0;
+        for (int s = 0; s < n; ++s) {
+            stage(slot, [&]() {
+                if (s + C::R < n) {
+                    wait_vmcnt<(C::R - 2) * C::LOADS>();
+                    publish();
+                    issue(s + C::R, slot);
+                } else if (s + 1 < n) {
+                    wait_stages<C::LOADS, C::R - 2>(n - 2 - s);
+                    publish();
+                }
+            });
+            slot = next(slot);
+        }
+
+        // the next tile's first loads, then what this one leaves
+        const int my_row0 = row0, my_rows = rows;
+        const int c0 = n0 + wn * C::WN;
+        uint64_t nans[C::TOK];
+#pragma unroll
+        for (int i = 0; i < C::TOK; ++i) nans[i] = all.bad ? ~0ull : wrong[i];
+        if (n0 == 0 && wn == 0 && lane == 0 && a.bad && !all.bad) {
+            int bad_rows = 0;
+#pragma unroll
+            for (int i = 0; i < C::TOK; ++i) bad_rows += __popcll(wrong[i]);
+            if (bad_rows) atomicAdd(a.bad, bad_rows);
+        }
+        if (t + each < last) {
+            aim();
+            publish(); // no wave reads the stages any more
+            begin();
+        }
+        const bool cnt = a.nonfinite != nullptr;
+        auto count4 = [&](const floatx4 &v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad += !__builtin_isfinite(v[e]);
+        };
+#pragma unroll
+        for (int mt = 0; mt < C::MT; ++mt) {
+            const int row = 16 * mt + li;
+            if (row >= my_rows) continue;
+            if ((nans[mt / 4] >> (row & 63)) & 1)
+#pragma unroll
+                for (int nt = 0; nt < C::NTL; ++nt) acc[mt][nt] = nan4();
+            if constexpr (OUT == 0) {
+                float *const o = a.out + (size_t)(my_row0 + row) * a.ldo;
+#pragma unroll
+                for (int nt = 0; nt < C::NTL; ++nt) {
+                    const int col = c0 + 16 * nt + 4 * g;
+                    const floatx4 v = acc[mt][nt];
+                    if (a.vec && col + 4 <= a.N) {
+                        if (cnt) count4(v);
+                        *reinterpret_cast<floatx4 *>(o + col) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (col + e < a.N) {
+                                bad += cnt && !__builtin_isfinite(v[e]);
+                                o[col + e] = v[e];
+                            }
+                    }
+                }
+            } else {
+                uint32_t *const o = a.pk + (size_t)(my_row0 + row) * a.ldpw + 4 * g;
+#pragma unroll
+                for (int nt = 0; nt < C::NTL; nt += OUT == 3 ? 4 : 2) {
+                    const int col = c0 + 16 * nt; // of the weight rows
+                    if (col >= a.N) continue;
+                    floatx4 lo = acc[mt][nt], hi = acc[mt][nt + 1];
+                    if (cnt) {
+                        count4(lo);
+                        count4(hi);
+                    }
+                    if constexpr (OUT == 3) {
+                        const floatx4 vlo = acc[mt][nt + 2], vhi = acc[mt][nt + 3];
+                        if (cnt) {
+                            count4(vlo);
+                            count4(vhi);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            lo[e] = mul_f32(silu_fast(lo[e]), vlo[e]);
+                            hi[e] = mul_f32(silu_fast(hi[e]), vhi[e]);
+                        }
+                    } else if constexpr (OUT == 2) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            lo[e] = gelu_tanh(lo[e]);
+                            hi[e] = gelu_tanh(hi[e]);
+                        }
+                    }
+                    u32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = pack_f16_rounded(lo[e], hi[e]);
+                    *reinterpret_cast<u32x4 *>(o + col / (OUT == 3 ? 4 : 2)) = v;
+                }
+            }
+        }
     }
     count_nonfinite(a.nonfinite, bad);
 }
@@ -592,7 +1063,6 @@ __global__ __launch_bounds__(256) void b1_combine_kernel(CombineArgs a) {
     if (wrong && a.bad && threadIdx.x == 0 && blockIdx.y == 0) atomicAdd(a.bad, 1);
     if (col >= a.H) return;
     floatx4 v = {0.f, 0.f, 0.f, 0.f};
-    if (a.residual) v = *reinterpret_cast<const floatx4 *>(a.residual + (int64_t)token * a.ldr + col);
     for (int j = 0; j < a.top_k; ++j) {
         const int p = place[j];
         if (p < 0 || p >= a.routes) continue;
@@ -601,6 +1071,7 @@ __global__ __launch_bounds__(256) void b1_combine_kernel(CombineArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(w, x[i], v[i]);
     }
+    if (a.residual) v += *reinterpret_cast<const floatx4 *>(a.residual + (int64_t)token * a.ldr + col);
     if (wrong) v = nan4();
     *reinterpret_cast<floatx4 *>(a.out + (int64_t)token * a.ldo + col) = v;
 }
@@ -667,17 +1138,91 @@ hipError_t launch_route(const RouteArgs &a, void *ws, size_t ws_bytes, hipStream
     return hipGetLastError();
 }
 
+// ------------------------------------------------ the experts' linears ----
+
 namespace {
 
-template <int NW, int U>
-hipError_t launch_few(const ExpertArgs &a, int num_cus, hipStream_t s) {
+// Groups of up to bm rows of one expert that evenly spread routes make.
+double likely_groups(const ExpertArgs &a, int bm) {
+    const double mean = (double)a.routes / a.experts;
+    return a.experts * (1.0 - std::exp(-mean) + std::max(0.0, mean / bm - 0.5));
+}
+
+// Which kernel a call takes, by models of their microseconds.  They are fitted
+// to 4563 shapes of 2 to 256 experts, 0.5 to 600 rows an expert, K 128 to 8192
+// and N 512 to 8192 on 256 CUs, each run with all four (the median shape within
+// 4 %; the kernel chosen takes 1.4 % more than the fastest of them on average,
+// 10 % at the 95th percentile, where one kernel by rows an expert alone takes
+// 18 % and 90 %): a fixed time, and for tiles the longer of what the rounds of
+// a CU's resident work-groups take one after another and what all its tiles take of its
+// matrix units, for few rows a work-group's steps beside the others on its CU.
+struct FewPlan {
+    int waves, units, parts, per; // 256s of K a wave; work-groups a group of rows, steps each
+    double us;
+};
+
+FewPlan plan_few(const ExpertArgs &a, int num_cus) {
+    const int units = (a.K + 255) / 256;
+    FewPlan f = {};
+    f.waves = units <= 3 || (units > 4 && units <= 6) ? 3 : units <= 8 ? 4 : 8;
+    f.units = units <= 4 ? 1 : units <= 16 ? 2 : 4;
     const int steps = a.kind == 3 ? a.glu_h / 32 : (a.N + 63) / 64;
-    const int64_t slots = group_bound(a.routes, a.experts, 16);
-    // two work-groups a CU at a time, some rounds of them
-    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)num_cus / slots);
-    const int per = (int)std::max<int64_t>(1, (steps + want - 1) / want), parts = (steps + per - 1) / per;
+    const int resident = (f.units == 1 ? 16 : f.units == 2 ? 12 : 8) / f.waves; // work-groups a CU, by their registers
+    const double groups = likely_groups(a, 16);
+    double best = 1e30;
+    for (int p = 1; p <= steps; ++p) {
+        const int per = (steps + p - 1) / p;
+        if ((steps + per - 1) / per != p) continue; // fewer parts of as many steps
+        const double wgs = std::ceil(groups * p / num_cus), beside = std::min(wgs, (double)resident);
+        const double rounds = std::ceil(wgs / resident), cost = rounds * (3.0 + per * (beside + 1.0));
+        if (cost < best) {
+            best = cost;
+            f.parts = p;
+            f.per = per;
+            const double wave = f.units * f.waves / 4.0;
+            f.us = a.kind == 0 ? 4.9 + rounds * (per * (0.85 * wave * beside + 0.12 * f.units) - 1.3)
+                               : 5.7 + rounds * (per * (0.80 * wave * beside + 0.20 * f.units) - 1.7);
+        }
+    }
+    return f;
+}
+
+//                      BM  WN NWN R  L OCC SETS
+using E32 = ExpertTile<32, 64, 4, 3, 2, 4, 2>;
+using E64 = ExpertTile<64, 64, 4, 3, 2, 3, 1>;
+using E128 = ExpertTile<128, 64, 4, 2, 4, 2, 1>;
+
+struct TileTimes {
+    double fixed, round, round_k, tile, tile_k; // us; _k: a stage
+};
+template <class C>
+double tile_us(const ExpertArgs &a, int num_cus, const TileTimes &packed, const TileTimes &rows) {
+    const TileTimes &t = a.kind == 0 ? rows : packed;
+    const double tiles = likely_groups(a, C::BM) * ((a.N + C::BN - 1) / C::BN) / num_cus, n = a.K / 64;
+    return t.fixed + std::max(std::ceil(tiles / C::OCC) * (t.round + t.round_k * n),
+                              std::ceil(tiles) * (t.tile + t.tile_k * n));
+}
+
+// 0: few rows; else the tiles' rows
+int plan_experts(const ExpertArgs &a, int num_cus, FewPlan *few) {
+    const double us[3] = {
+        tile_us<E32>(a, num_cus, {3.9, 0.48, 0.42, 0.51, 0.30}, {3.7, 0.63, 0.43, 0.91, 0.31}),
+        tile_us<E64>(a, num_cus, {3.5, 1.1, 0.53, 0.82, 0.42}, {2.7, 2.1, 0.53, 1.8, 0.43}),
+        tile_us<E128>(a, num_cus, {3.8, 1.7, 0.76, 1.4, 0.68}, {3.5, 0.0, 0.35, 2.2, 0.76})};
+    const int best = (int)(std::min_element(us, us + 3) - us);
+    if (a.K <= kFewMaxK) {
+        *few = plan_few(a, num_cus);
+        const int64_t threads = group_bound(a.routes, a.experts, 16) * few->parts * few->waves * 64;
+        if (few->us < us[best] && threads < ((int64_t)1 << 31)) return 0;
+    }
+    return 32 << best;
+}
+
+template <int NW, int U>
+hipError_t launch_few(const ExpertArgs &a, const FewPlan &f, hipStream_t s) {
+    const dim3 grid((unsigned)(group_bound(a.routes, a.experts, 16) * f.parts));
     auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(slots * parts)), dim3(NW * 64), 0, s, a, parts, per);
+        hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), 0, s, a, f.parts, f.per);
         return hipGetLastError();
     };
     switch (a.kind) {
@@ -688,14 +1233,55 @@ hipError_t launch_few(const ExpertArgs &a, int num_cus, hipStream_t s) {
     }
 }
 
+template <class C>
+hipError_t launch_tiles(const ExpertArgs &a, int num_cus, hipStream_t s) {
+    const int tiles_n = (a.N + C::BN - 1) / C::BN;
+    const int64_t tiles = group_bound(a.routes, a.experts, C::BM) * tiles_n;
+    // a multiple of the XCDs
+    const unsigned grid = (unsigned)(std::min<int64_t>((int64_t)num_cus * C::OCC, tiles + 7) / 8 * 8);
+    auto run = [&](auto kernel) {
+        const hipError_t e = allow_lds(kernel, C::LDS);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(kernel, dim3(std::max(grid, 8u)), dim3(C::NT), C::LDS, s, a, tiles_n);
+        return hipGetLastError();
+    };
+    switch (a.kind) {
+    case 0: return run(&b1_experts_tile_kernel<C, 0>);
+    case 1: return run(&b1_experts_tile_kernel<C, 1>);
+    case 2: return run(&b1_experts_tile_kernel<C, 2>);
+    default: return run(&b1_experts_tile_kernel<C, 3>);
+    }
+}
+
 } // namespace
 
+extern "C" int b1_experts_plan(int routes, int experts, int K, int N, int kind, int num_cus, int *waves, int *units) {
+    ExpertArgs a{};
+    a.routes = routes;
+    a.experts = experts;
+    a.K = K;
+    a.N = N;
+    a.kind = kind;
+    a.glu_h = N / 2;
+    FewPlan f = {};
+    const int rows = plan_experts(a, num_cus, &f);
+    *waves = rows ? 0 : f.waves;
+    *units = rows ? 0 : f.units;
+    return rows;
+}
+
 hipError_t launch_experts(const ExpertArgs &a, int num_cus, hipStream_t s) {
-    const int units = (a.K + 255) / 256;
-    if (units <= 4) return launch_few<4, 1>(a, num_cus, s);
-    if (units <= 8) return launch_few<8, 1>(a, num_cus, s);
-    if (units <= 16) return launch_few<8, 2>(a, num_cus, s);
-    return launch_few<8, 4>(a, num_cus, s);
+    FewPlan f = {};
+    switch (plan_experts(a, num_cus, &f)) {
+    case 0: break;
+    case 32: return launch_tiles<E32>(a, num_cus, s);
+    case 64: return launch_tiles<E64>(a, num_cus, s);
+    default: return launch_tiles<E128>(a, num_cus, s);
+    }
+    if (f.units == 1) return f.waves == 3 ? launch_few<3, 1>(a, f, s) : launch_few<4, 1>(a, f, s);
+    if (f.units == 2 && f.waves == 3) return launch_few<3, 2>(a, f, s);
+    if (f.units == 2) return f.waves == 4 ? launch_few<4, 2>(a, f, s) : launch_few<8, 2>(a, f, s);
+    return launch_few<8, 4>(a, f, s);
 }
 
 hipError_t launch_combine(const CombineArgs &a, hipStream_t s) {

@@ -304,6 +304,7 @@ hipError_t launch_route(const RouteArgs &a, void *ws, size_t ws_bytes, hipStream
 // weights [experts][N][K/32*6].
 struct ExpertArgs {
     const uint16_t *act;  // packed fp16 rows of K
+    int act_rows;         // how many; with `order` below 2^32 bytes
     const uint8_t *w;
     int K, N, experts, routes, top_k;
     const int32_t *start; // [experts + 1]
@@ -317,8 +318,12 @@ struct ExpertArgs {
     int glu_h;            // kind 3: N / 2
     int32_t *nonfinite, *bad;
 };
-constexpr int kExpertsMaxK = 8192;
+constexpr int kFewMaxK = 8192; // of the few-rows kernel
 hipError_t launch_experts(const ExpertArgs &a, int num_cus, hipStream_t s);
+// What it runs for a shape (its `kind`, N weight rows): the rows of a tile, or
+// 0 for the few-rows kernel with *waves waves of *units times 256 of K.  For
+// the tests; no part of the C ABI.
+extern "C" int b1_experts_plan(int routes, int experts, int K, int N, int kind, int num_cus, int *waves, int *units);
 
 // out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]], rows of H.
 struct CombineArgs {

@@ -811,8 +811,9 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
  * of the down projections; else y as fp32 in out (row stride ldo >= out_dim,
  * 4-byte aligned; act_fn NONE).
  * Of `routes` only start and (by_token) order are read, and tokens, experts,
- * top_k.  in_dim % 64 == 0, in_dim <= 8192; an expert's weights below 2^31
- * bytes.  Outputs apart from the inputs.
+ * top_k.  in_dim % 64 == 0, in_dim <= 2^16, out_dim <= 2^17, an expert's weights
+ * below 2^31 bytes; by_token: tokens * in_dim < 2^31.  Outputs apart from the
+ * inputs.
  * Numbers are those of FAST mode: products of fp16 in fp32 sums, in an order
  * that depends on tokens, experts, top_k and the widths, not on the routes.
  * The non-finite counter counts y.  Starts out of order or range make every
@@ -838,7 +839,7 @@ int bonsai_b1_linear_experts(const bonsai_b1_experts_args *args,
 
 /*
  * out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]] over the token's
- * routes, in fp32, added in the order of j: the block's output from the down
+ * routes, in fp32, summed in the order of j, the residual last: the block's output from the down
  * projections' rows y (fp32, row stride ldy).  residual may be NULL (0) or out itself
  * (same row stride); out is apart from y.  A place out of range makes the
  * token's row NaN and adds to `bad`.  Of `routes` weight and place are read.
