@@ -1038,23 +1038,25 @@ class Routes:
         return self.start.shape[0] - 1
 
 
-def _routes_c(r):
-    """The bonsai_b1_routes of a Routes."""
-    if r.expert.dim() != 2 or r.start.dim() != 1 or r.order.dim() != 1:
-        raise ValueError("expert must be [tokens, top_k], start and order vectors")
-    tokens, k = r.expert.shape
-    for t, shape, dtype, what in ((r.expert, (tokens, k), _torch.int32, "expert"),
-                                  (r.weight, (tokens, k), _torch.float32, "weight"),
-                                  (r.place, (tokens, k), _torch.int32, "place"),
-                                  (r.order, (tokens * k,), _torch.int32, "order"),
-                                  (r.start, r.start.shape, _torch.int32, "start")):
-        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"routes: {what} must be contiguous {dtype} {list(shape)}")
+_ROUTES = ("expert", "weight", "start", "order", "place")
+
+
+def _routes_c(r, used=_ROUTES):
+    """The bonsai_b1_routes of a Routes, with the arrays that a call uses."""
+    if r.expert.dim() != 2 or r.start.dim() != 1:
+        raise ValueError("expert must be [tokens, top_k], start a vector")
+    (tokens, k), n = r.expert.shape, r.start.numel()
     # (ctypes cuts integers to the field's width: the limits of the C entries)
-    if (tokens | k | r.start.numel()) >> 24:
+    if (tokens | k | n) >> 24:
         raise ValueError("tokens * top_k is limited to 2^24, experts to 1024")
-    return RoutesC(tokens, r.start.numel() - 1, k, r.expert.data_ptr(), r.weight.data_ptr(), r.start.data_ptr(),
-                   r.order.data_ptr(), r.place.data_ptr())
+    c = RoutesC(tokens, n - 1, k)
+    for name in used:
+        t = getattr(r, name)
+        if t.dtype is not (_torch.float32 if name == "weight" else _torch.int32) or not t.is_contiguous() or \
+                t.numel() != (n if name == "start" else tokens * k):
+            raise ValueError(f"routes: {name} must be contiguous, int32 (weight fp32), a value a slot (start: experts + 1)")
+        setattr(c, name, t.data_ptr())
+    return c
 
 
 def route(logits, top_k: int, score: str = "softmax", bias=None, renormalize: bool = True, scale: float = 1.0,
@@ -1078,11 +1080,16 @@ def route(logits, top_k: int, score: str = "softmax", bias=None, renormalize: bo
     if unit != 1 and experts > 1:
         raise ValueError("logits must have unit column stride")
     if out is None:
-        i32 = _torch.int32
-        out = Routes(_empty(stream, (tokens, top_k), i32, dev), _empty(stream, (tokens, top_k), _torch.float32, dev),
-                     _empty(stream, (experts + 1,), i32, dev), _empty(stream, (tokens * top_k,), i32, dev),
-                     _empty(stream, (tokens, top_k), i32, dev))
-    routes = _routes_c(out)
+        # one allocation: five cost 3 us more
+        n, shape, step = tokens * top_k, (tokens, top_k), (top_k, 1)
+        buf = _empty(stream, (4 * n + experts + 1,), _torch.int32, dev)
+        out = Routes(buf.as_strided(shape, step, 0), buf.as_strided(shape, step, n).view(_torch.float32),
+                     buf.as_strided((experts + 1,), (1,), 4 * n), buf.as_strided((n,), (1,), 2 * n),
+                     buf.as_strided(shape, step, 3 * n))
+        at = buf.data_ptr()
+        routes = RoutesC(tokens, experts, top_k, at, at + 4 * n, at + 16 * n, at + 8 * n, at + 12 * n)
+    else:
+        routes = _routes_c(out)
     if (routes.tokens, routes.experts, routes.top_k) != (tokens, experts, top_k):
         raise ValueError("out is of other tokens, experts or top_k")
     args = RouteArgs(logits.data_ptr(), ld if tokens > 1 else experts, code, SCORES[score],
@@ -1109,9 +1116,9 @@ def linear_experts(packed_act, w_packed, routes, in_dim: int, out_dim: int, act:
         packed = None
     if rows not in ("tokens", "routes"):
         raise ValueError('rows is "tokens" or "routes"')
-    dev = _on_current_device(packed_act, w_packed, routes.expert, routes.weight, routes.start, routes.order,
-                             routes.place, out, packed if packed is not True else None, nonfinite, bad)
-    c = _routes_c(routes)
+    dev = _on_current_device(packed_act, w_packed, routes.start, routes.order, out,
+                             packed if packed is not True else None, nonfinite, bad)
+    c = _routes_c(routes, ("start", "order") if rows == "tokens" else ("start",))
     n = c.tokens * c.top_k
     if in_dim <= 0 or out_dim <= 0 or (in_dim | out_dim) >> 31:
         raise ValueError("in_dim and out_dim are positive")
@@ -1146,9 +1153,8 @@ def combine_experts(y, routes, residual=None, out=None, bad=None, stream=None):
     order, as linear_experts gives it; residual [tokens, H] fp32 or None; out
     may be residual.  Returns out [tokens, H]."""
     lib = _lib or load()
-    dev = _on_current_device(y, routes.expert, routes.weight, routes.start, routes.order, routes.place, residual, out,
-                             bad)
-    c = _routes_c(routes)
+    dev = _on_current_device(y, routes.weight, routes.place, residual, out, bad)
+    c = _routes_c(routes, ("weight", "place"))
     if y.dim() != 2:
         raise ValueError("y must be [tokens * top_k, H]")
     h = y.shape[1]

@@ -12,6 +12,7 @@
 namespace b1 {
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 
 // ------------------------------------------------- scans over a wave ----
@@ -65,18 +66,22 @@ __device__ __forceinline__ float logit_at(const RouteArgs &a, int64_t i) {
 // A token's experts and weights, by one wave; lane j < top_k returns the j-th
 // expert (-1: none) and writes it and its weight.
 //
-// Lane l holds logits l, l + 64, ...  (EL of them).  A choice is the largest
-// key of all lanes, ties to the lowest expert: keys are the logits as
-// integers of the same order, or, where a bias makes a score's rounding count
-// (WIDE), the 64-bit scores + bias, compared by their high words first.  Key
-// 0 is never chosen: -inf and what is chosen already.  NaN comes behind every
-// number (and makes the row's weights NaN).
+// Lane l holds logits EL * l .. EL * l + EL - 1.  A choice is the largest key
+// of all lanes (a scan of six steps), ties to the lowest lane, which holds the
+// lowest experts.  Keys are the logits as integers of the same order, or,
+// where a bias makes a score's rounding count (WIDE), the 64-bit scores +
+// bias, compared by their high words first.  Key 0 is never chosen: -inf and
+// what is chosen already.  NaN comes behind every number (and makes the row's
+// weights NaN).  Up to four experts a lane are sorted once, so that a choice
+// only moves the lane's next one up.
 constexpr uint32_t kNanKey = 1;
 template <int EL, bool WIDE>
 __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
+    constexpr bool SORTED = EL > 1 && EL <= 4;
     const int lane = threadIdx.x & 63;
     float x[EL];
     uint32_t hi[EL], lo[WIDE ? EL : 1];
+    int id[EL];
     const int64_t row = (int64_t)token * a.ld;
     uint32_t top = 0; // the largest logit, as a key
     bool nan = false;
@@ -86,14 +91,24 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
     };
 #pragma unroll
     for (int i = 0; i < EL; ++i) {
-        const int e = lane + 64 * i;
+        const int e = lane * EL + i;
+        id[i] = e;
         x[i] = e < a.experts ? logit_at(a, row + e) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < EL; ++i) {
         nan |= x[i] != x[i];
         hi[i] = x[i] > -INFINITY ? key_of(x[i]) : x[i] != x[i] ? kNanKey : 0u;
         top = max(top, hi[i]);
     }
     top = wave_max(top);
     const float peak = __builtin_bit_cast(float, top ^ ((top >> 31) ? 0x80000000u : 0xffffffffu));
+    float all = 0.f; // softmax over all experts
+    if (!a.sigmoid && !a.renormalize) {
+#pragma unroll
+        for (int i = 0; i < EL; ++i) all += x[i] > -INFINITY ? expf(x[i] - peak) : 0.f;
+        all = wave_sum(all);
+    }
     if constexpr (WIDE) {
         double z[EL], sum = 0.0;
 #pragma unroll
@@ -107,59 +122,84 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         }
         if (!a.sigmoid) sum = wave_sum(sum);
         // an infinite logit: weights NaN, chosen by the logits
-        if (a.sigmoid || sum < (double)INFINITY) {
+        const bool by_score = a.sigmoid || sum < (double)INFINITY;
 #pragma unroll
-            for (int i = 0; i < EL; ++i) {
-                const int e = lane + 64 * i;
-                if (e >= a.experts || hi[i] <= kNanKey) {
-                    lo[i] = 0;
-                    continue;
-                }
-                const double k = (a.sigmoid ? z[i] : z[i] / sum) + (double)a.bias[e] + 0.0;
-                const uint64_t b = __builtin_bit_cast(uint64_t, k);
-                const uint64_t key = b ^ ((b >> 63) ? ~0ull : 1ull << 63);
-                nan |= k != k;
-                hi[i] = k > -(double)INFINITY ? (uint32_t)(key >> 32) : k != k ? kNanKey : 0u;
-                lo[i] = k == k ? (uint32_t)key : 0u;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < EL; ++i) lo[i] = 0;
+        for (int i = 0; i < EL; ++i) {
+            lo[i] = 0;
+            if (!by_score || id[i] >= a.experts || hi[i] <= kNanKey) continue;
+            const double k = (a.sigmoid ? z[i] : z[i] / sum) + (double)a.bias[id[i]] + 0.0;
+            const uint64_t b = __builtin_bit_cast(uint64_t, k);
+            const uint64_t key = b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+            nan |= k != k;
+            hi[i] = k > -(double)INFINITY ? (uint32_t)(key >> 32) : k != k ? kNanKey : 0u;
+            lo[i] = k == k ? (uint32_t)key : 0u;
         }
     }
     const bool any_nan = __ballot(nan) != 0;
-    int mine = -1;
-    float mine_x = -INFINITY;
-    for (int j = 0; j < a.top_k; ++j) {
-        uint32_t m = 0;
+    auto above = [&](int i, int j) { // i's key is larger than j's
+        if constexpr (WIDE) return hi[i] > hi[j] || (hi[i] == hi[j] && lo[i] > lo[j]);
+        return hi[i] > hi[j];
+    };
+    if constexpr (SORTED) {
 #pragma unroll
-        for (int i = 0; i < EL; ++i) m = max(m, hi[i]);
-        m = wave_max(m);
-        if (m == 0) break;
-        uint32_t ml = 0;
-        if constexpr (WIDE) {
+        for (int n = 1; n < EL; ++n)
 #pragma unroll
-            for (int i = 0; i < EL; ++i) ml = max(ml, hi[i] == m ? lo[i] : 0u);
-            ml = wave_max(ml);
-        }
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < EL; ++i) {
-            bool same = hi[i] == m;
-            if constexpr (WIDE) same = same && lo[i] == ml;
-            const uint64_t who = __ballot(same);
-            if (!found && who) { // wave-uniform
-                found = true;
-                const int l = __builtin_ctzll(who);
-                const float v = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, x[i]), l));
-                if (lane == l) hi[i] = 0;
-                if (lane == j) {
-                    mine = l + 64 * i;
-                    mine_x = v;
+            for (int i = n; i > 0; --i) {
+                const bool swap = above(i, i - 1);
+                const uint32_t h = hi[i];
+                hi[i] = swap ? hi[i - 1] : h;
+                hi[i - 1] = swap ? h : hi[i - 1];
+                const int e = id[i];
+                id[i] = swap ? id[i - 1] : e;
+                id[i - 1] = swap ? e : id[i - 1];
+                if constexpr (WIDE) {
+                    const uint32_t l = lo[i];
+                    lo[i] = swap ? lo[i - 1] : l;
+                    lo[i - 1] = swap ? l : lo[i - 1];
                 }
+            }
+    }
+    int mine = -1;
+    for (int j = 0; j < a.top_k; ++j) {
+        uint32_t m = hi[0], ml = 0;
+        int e = id[0];
+        if constexpr (WIDE) ml = lo[0];
+        if constexpr (!SORTED) { // the lane's largest, the first of equals
+#pragma unroll
+            for (int i = 1; i < EL; ++i) {
+                bool more = hi[i] > m;
+                if constexpr (WIDE) more = more || (hi[i] == m && lo[i] > ml);
+                m = more ? hi[i] : m;
+                e = more ? id[i] : e;
+                if constexpr (WIDE) ml = more ? lo[i] : ml;
+            }
+        }
+        const uint32_t best = wave_max(m);
+        if (best == 0) break;
+        bool same = m == best;
+        if constexpr (WIDE) {
+            const uint32_t best_lo = wave_max(same ? ml : 0u);
+            same = same && ml == best_lo;
+        }
+        const int l = __builtin_ctzll(__ballot(same));
+        const int chosen = __builtin_amdgcn_readlane(e, l);
+        if (lane == j) mine = chosen;
+        if (lane == l) {
+            if constexpr (SORTED) {
+#pragma unroll
+                for (int i = 0; i + 1 < EL; ++i) {
+                    hi[i] = hi[i + 1];
+                    id[i] = id[i + 1];
+                    if constexpr (WIDE) lo[i] = lo[i + 1];
+                }
+                hi[EL - 1] = 0;
+            } else {
+#pragma unroll
+                for (int i = 0; i < EL; ++i) hi[i] = id[i] == chosen ? 0u : hi[i];
             }
         }
     }
+    const float mine_x = mine >= 0 ? logit_at(a, row + mine) : -INFINITY;
     float weight;
     if (a.sigmoid) {
         // in 64 bits: scores of far logits stay apart from zero
@@ -171,13 +211,7 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         weight = (float)(s * (double)a.scale);
     } else {
         const float p = mine >= 0 ? expf(mine_x - peak) : 0.f;
-        float sum = p;
-        if (!a.renormalize) {
-            sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < EL; ++i) sum += x[i] > -INFINITY ? expf(x[i] - peak) : 0.f;
-        }
-        weight = p / wave_sum(sum) * a.scale;
+        weight = p / (a.renormalize ? wave_sum(p) : all) * a.scale;
     }
     if (any_nan) weight = __builtin_nanf("");
     if (mine < 0) weight = 0.f;
@@ -275,12 +309,14 @@ __global__ __launch_bounds__(kRouteThreads) void b1_route_kernel(RouteArgs a) {
 }
 
 // Many tokens, in two launches: each work-group chooses for `per` tokens and
-// counts their experts; then each finds its first row of every expert from
-// all the counts and places its slots.
+// counts their experts (16 bits: a token has an expert once; rows of a multiple of 4 counts); then each finds its
+// first row of every expert from all the counts and places its slots.
+__host__ __device__ constexpr int count_row(int experts) { return (experts + 3) / 4 * 4; }
+
 template <int EL, bool WIDE>
-__global__ __launch_bounds__(kRouteThreads) void b1_route_choose_kernel(RouteArgs a, int per, uint32_t *counts) {
+__global__ __launch_bounds__(kRouteThreads) void b1_route_choose_kernel(RouteArgs a, int per, uint16_t *counts) {
     extern __shared__ uint32_t route_lds[];
-    const int wave = threadIdx.x >> 6, E = a.experts;
+    const int wave = threadIdx.x >> 6, E = count_row(a.experts);
     for (int e = threadIdx.x; e < E; e += kRouteThreads) route_lds[e] = 0;
     __syncthreads();
     const int t1 = min((int)(blockIdx.x + 1) * per, a.tokens);
@@ -289,43 +325,47 @@ __global__ __launch_bounds__(kRouteThreads) void b1_route_choose_kernel(RouteArg
         if (e >= 0) atomicAdd(&route_lds[e], 1u);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) counts[(size_t)blockIdx.x * E + e] = route_lds[e];
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) counts[(size_t)blockIdx.x * E + e] = (uint16_t)route_lds[e];
 }
 
-__global__ __launch_bounds__(kRouteThreads) void b1_route_place_kernel(RouteArgs a, int per, const uint32_t *counts) {
+__global__ __launch_bounds__(kRouteThreads) void b1_route_place_kernel(RouteArgs a, int per, const uint16_t *counts) {
     extern __shared__ uint32_t route_lds[];
-    uint32_t *base = route_lds, *total = route_lds + a.experts, *parts = route_lds + 2 * a.experts;
+    const int E = count_row(a.experts), quads = E / 4, lane = threadIdx.x & 63;
+    uint32_t *base = route_lds, *total = route_lds + E, *parts = route_lds + 2 * E;
     __shared__ uint32_t all;
-    const int E = a.experts, lane = threadIdx.x & 63;
     for (int e = threadIdx.x; e < E; e += kRouteThreads) base[e] = total[e] = 0;
     __syncthreads();
-    // threads e, e + E', ... of an expert take the work-groups in turn
-    const int groups = max(1, kRouteThreads / E);
-    const int g = threadIdx.x / E;
+    // a thread takes four experts of every `groups`-th work-group
+    const int groups = kRouteThreads / quads, g = threadIdx.x / quads, q = threadIdx.x - g * quads;
     if (g < groups) {
-        for (int e = threadIdx.x - g * E; e < E; e += kRouteThreads) {
-            uint32_t before = 0, sum = 0;
+        uint32_t before[4] = {}, sum[4] = {};
 #pragma unroll 8
-            for (int w = g; w < (int)gridDim.x; w += groups) {
-                const uint32_t n = counts[(size_t)w * E + e];
-                sum += n;
-                before += w < (int)blockIdx.x ? n : 0u;
+        for (int w = g; w < (int)gridDim.x; w += groups) {
+            const u32x2 n = *reinterpret_cast<const u32x2 *>(counts + (size_t)w * E + 4 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t c = (n[i / 2] >> (16 * (i & 1))) & 0xffffu;
+                sum[i] += c;
+                before[i] += w < (int)blockIdx.x ? c : 0u;
             }
-            if (before) atomicAdd(&base[e], before);
-            if (sum) atomicAdd(&total[e], sum);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (before[i]) atomicAdd(&base[4 * q + i], before[i]);
+            if (sum[i]) atomicAdd(&total[4 * q + i], sum[i]);
         }
     }
     __syncthreads();
     if (threadIdx.x < 64) {
-        const uint32_t n = lds_prefix(total, E);
+        const uint32_t n = lds_prefix(total, a.experts);
         if (lane == 0) all = n;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
         base[e] += total[e];
         if (blockIdx.x == 0) a.start[e] = (int)total[e];
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.start[E] = (int)all;
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.start[a.experts] = (int)all;
     __syncthreads();
     const int64_t slots = (int64_t)a.tokens * a.top_k;
     const int64_t s0 = (int64_t)blockIdx.x * per * a.top_k;
@@ -1078,10 +1118,12 @@ __global__ __launch_bounds__(256) void b1_combine_kernel(CombineArgs a) {
 
 // ---------------------------------------------------------- launchers ----
 
-constexpr int kRouteOneGroup = 64; // tokens
+// Tokens of a single work-group (128 experts: 16 tokens 5.9 us, 32 8.3, 64 12.6;
+// two launches 9.0).
+constexpr int kRouteOneGroup = 32;
 
-// Tokens a work-group of the two-launch router: at most 256 work-groups.
-int route_per(int tokens) { return std::max(kRouteWaves, (tokens + 255) / 256); }
+// Tokens a work-group of the two-launch router: 256 work-groups and one at most.
+int route_per(int tokens) { return std::min(std::max(kRouteWaves, (tokens + 255) / 256), 65535); }
 
 template <class F>
 hipError_t with_route(const RouteArgs &a, F f) {
@@ -1100,7 +1142,7 @@ hipError_t with_route(const RouteArgs &a, F f) {
 size_t route_workspace_bytes(const RouteArgs &a) {
     if (a.tokens <= kRouteOneGroup) return 0;
     const int per = route_per(a.tokens);
-    return (size_t)((a.tokens + per - 1) / per) * a.experts * 4;
+    return (size_t)((a.tokens + per - 1) / per) * count_row(a.experts) * 2;
 }
 
 // More than 64 KB of LDS is for the asking.
@@ -1113,7 +1155,7 @@ static hipError_t allow_lds(K kernel, size_t bytes) {
 
 hipError_t launch_route(const RouteArgs &a, void *ws, size_t ws_bytes, hipStream_t s) {
     const size_t need = route_workspace_bytes(a);
-    const size_t row = (size_t)a.experts * 4;
+    const size_t row = (size_t)count_row(a.experts) * 4;
     if (need == 0 || !ws || ws_bytes < need)
         return with_route(a, [&](auto el, auto wide) {
             auto kernel = &b1_route_kernel<decltype(el)::value, decltype(wide)::value>;
@@ -1124,7 +1166,7 @@ hipError_t launch_route(const RouteArgs &a, void *ws, size_t ws_bytes, hipStream
             return hipGetLastError();
         });
     const int per = route_per(a.tokens), groups = (a.tokens + per - 1) / per;
-    uint32_t *counts = static_cast<uint32_t *>(ws);
+    uint16_t *counts = static_cast<uint16_t *>(ws);
     const hipError_t e = with_route(a, [&](auto el, auto wide) {
         hipLaunchKernelGGL((b1_route_choose_kernel<decltype(el)::value, decltype(wide)::value>), dim3(groups),
                            dim3(kRouteThreads), row, s, a, per, counts);

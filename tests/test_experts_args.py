@@ -121,7 +121,7 @@ def test_python_refusals():
     c = capi._routes_c(good)
     assert (c.tokens, c.top_k, c.experts) == (3, 2, 8)
     for bad in (dict(expert=i.long()), dict(weight=torch.zeros(3, 2).double()), dict(weight=torch.zeros(3, 1)),
-                dict(place=i.flatten()), dict(order=i.flatten()[:5]), dict(start=torch.zeros(9)),
+                dict(place=i.flatten()[:4]), dict(order=i.flatten()[:5]), dict(start=torch.zeros(9)),
                 dict(expert=torch.zeros(2, 3, dtype=torch.int32).t()), dict(order=torch.zeros(12, dtype=torch.int32)[::2])):
         a = dict(expert=i, weight=torch.zeros(3, 2), start=good.start, order=good.order, place=i)
         with pytest.raises(ValueError):
