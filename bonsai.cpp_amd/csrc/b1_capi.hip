@@ -816,7 +816,7 @@ int bonsai_b1_linear_experts(const bonsai_b1_experts_args *g, hipStream_t stream
 
 int bonsai_b1_combine_experts(const bonsai_b1_routes *r, const float *y, int64_t ldy, int H, const float *residual,
                               int64_t ldr, float *out, int64_t ldo, int32_t *bad, hipStream_t stream) {
-    if (!r || !routes_ok(r) || H <= 0 || H % 4 || !al4(bad)) return BONSAI_B1_ERR_ARG;
+    if (!r || !routes_ok(r) || H <= 0 || H % 4 || H > (1 << 24) || !al4(bad)) return BONSAI_B1_ERR_ARG;
     if (r->tokens > 0) {
         const int64_t most = (int64_t)1 << 38;
         if (!rows_ok(y, ldy, H, 4) || !rows_ok(out, ldo, H, 4) || ldy >= most || ldo >= most)

@@ -770,15 +770,15 @@ enum { BONSAI_B1_SCORE_SOFTMAX = 0, BONSAI_B1_SCORE_SIGMOID = 1 };
  * experts or the sigmoid of the logit; the weight is the chosen one's score,
  * divided with `renormalize` by the sum of the token's chosen ones (0 where
  * that is 0), times `scale`.  The bias is no part of it.
- * A NaN among a token's logits or scores, or with softmax +inf, makes its weights NaN (NaN
- * is chosen behind every number).
+ * A NaN among a token's logits or scores, or with softmax +inf, makes its
+ * weights NaN (NaN is chosen behind every number).
  * Writes all arrays of `routes`, the same on every call with the same logits.
  * workspace: bonsai_b1_route_workspace_bytes(args) bytes (16-byte aligned),
  * or NULL for the library's per-stream workspace, with the rules of
  * bonsai_b1_linear_f32's for captures.  Without one, or with one too small,
  * one work-group routes all tokens, with the same results, slower (8192
- * tokens of 128 experts: tens of times).  A workspace serves one call at a time: give
- * graphs that may be replayed at once one each.
+ * tokens of 128 experts: ONEGROUP us, else 13).  A workspace serves one call
+ * at a time: give graphs that may be replayed at once one each.
  */
 typedef struct bonsai_b1_route_args {
     const void *logits;
@@ -815,7 +815,10 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
  * below 2^31 bytes; by_token: tokens * in_dim < 2^31.  Outputs apart from the
  * inputs.
  * Numbers are those of FAST mode: products of fp16 in fp32 sums, in an order
- * that depends on tokens, experts, top_k and the widths, not on the routes.
+ * that depends on tokens, experts, top_k, the widths and the output's kind
+ * (they choose the kernel), not on the routes: the same call gives the same
+ * bits.  SwiGLU uses the device's exponential and reciprocal instructions,
+ * within half a step of fp16 of the exact value like GELU's.
  * The non-finite counter counts y.  Starts out of order or range make every
  * row of the call NaN, an order entry out of range its row; `bad` grows by at
  * least 1 then, and nothing out of range is read or written.
@@ -839,11 +842,12 @@ int bonsai_b1_linear_experts(const bonsai_b1_experts_args *args,
 
 /*
  * out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]] over the token's
- * routes, in fp32, summed in the order of j, the residual last: the block's output from the down
- * projections' rows y (fp32, row stride ldy).  residual may be NULL (0) or out itself
- * (same row stride); out is apart from y.  A place out of range makes the
+ * routes, in fp32, summed in the order of j, the residual last: the block's
+ * output from the down projections' rows y (fp32, row stride ldy).  residual
+ * may be NULL (0) or out itself (same row stride); out is apart from y.  A place out of range makes the
  * token's row NaN and adds to `bad`.  Of `routes` weight and place are read.
- * H % 4 == 0; pointers 16-byte aligned, row strides multiples of 4, >= H.
+ * H % 4 == 0, H <= 2^24; pointers 16-byte aligned, row strides multiples of
+ * 4, >= H.
  */
 int bonsai_b1_combine_experts(const bonsai_b1_routes *routes, const float *y,
                               int64_t ldy, int H, const float *residual,

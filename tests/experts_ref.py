@@ -7,6 +7,17 @@ import torch
 
 from tests.attention_ref import U32
 
+# tokens, experts, top_k, in_dim, out_dim -> the kernel that runs it: rows of a
+# tile, or 0 and the few-rows kernel's waves and 256s of K a wave
+KERNELS = {
+    (40, 3, 2, 192, 256): (0, 3, 1), (33, 7, 2, 704, 320): (0, 3, 1), (20, 5, 2, 1024, 128): (0, 4, 1),
+    (9, 6, 3, 1344, 192): (0, 3, 2), (21, 4, 2, 2048, 192): (0, 4, 2), (13, 3, 1, 4096, 128): (0, 8, 2),
+    (30, 3, 2, 8192, 128): (0, 8, 4),
+    (20, 20, 2, 192, 2496): (32, 0, 0), (100, 20, 3, 1088, 2304): (32, 0, 0), (200, 33, 6, 128, 576): (32, 0, 0),
+    (7, 3, 2, 8256, 64): (32, 0, 0), (6, 2, 1, 16384, 320): (32, 0, 0),
+    (2721, 5, 3, 192, 128): (64, 0, 0), (512, 20, 1, 1088, 2368): (64, 0, 0), (4000, 2, 1, 128, 2048): (64, 0, 0),
+    (2829, 3, 3, 320, 320): (128, 0, 0), (2774, 20, 3, 832, 320): (128, 0, 0), (6000, 2, 1, 64, 2112): (128, 0, 0)}
+
 
 def layout(expert, experts):
     """start, order and place of expert ids [tokens, top_k] (-1: no route)."""

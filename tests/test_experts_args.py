@@ -75,7 +75,8 @@ PACKED = dict(out=None, ldo=0, packed=P, ldp=128)
     dict(act=None), dict(act=P + 8), dict(w=None), dict(w=P + 2), dict(in_dim=0), dict(in_dim=96), dict(in_dim=-64),
     dict(out_dim=0), dict(out_dim=-1), dict(act_fn=1), dict(act_fn=2), dict(act_fn=3), dict(out=None),
     dict(out=P + 2), dict(ldo=127), dict(ldo=1 << 40), dict(packed=P, ldp=128), dict(nonfinite=P + 1),
-    dict(bad=P + 2), dict(in_dim=8192, out_dim=1 << 21, ldo=1 << 21)])
+    dict(bad=P + 2), dict(in_dim=65536 + 64), dict(out_dim=(1 << 17) + 1, ldo=1 << 18),
+    dict(in_dim=65536, out_dim=1 << 17, ldo=1 << 17), dict(in_dim=65536, routes=routes(tokens=32768))])
 def test_linear_experts(lib, change):
     assert lib.bonsai_b1_linear_experts(ctypes.byref(experts(**change)), None) == capi.ERR_ARG
 
@@ -97,7 +98,8 @@ def test_linear_experts_routes(lib, change):
 @pytest.mark.parametrize("change", [
     dict(y=None), dict(y=P + 8), dict(ldy=60), dict(ldy=66), dict(H=0), dict(H=66), dict(H=-4), dict(residual=P + 4),
     dict(residual=P, ldr=32), dict(residual=P, ldr=65), dict(out=None), dict(out=P + 4), dict(ldo=63), dict(ldo=62),
-    dict(residual=P * 2, ldr=128), dict(bad=P + 2), dict(ldy=1 << 40)])
+    dict(residual=P * 2, ldr=128), dict(bad=P + 2), dict(ldy=1 << 40),
+    dict(H=(1 << 24) + 4, ldy=1 << 25, ldo=1 << 25)])
 def test_combine_experts(lib, change):
     a = dict(routes=ctypes.byref(routes()), y=P, ldy=64, H=64, residual=None, ldr=0, out=P * 2, ldo=64, bad=None)
     a.update(change)

@@ -225,6 +225,37 @@ def test_linear_experts(torch, b1, unpack, tokens, experts, k, in_dim, out_dim, 
                packed)
 
 
+@pytest.mark.parametrize("rows", ["tokens", "routes"])
+@pytest.mark.parametrize("act,packed", [("none", False), ("none", True), ("gelu_tanh", True), ("swiglu", True)])
+@pytest.mark.parametrize("shape", moe.KERNELS)
+def test_linear_experts_by_each_kernel(torch, b1, unpack, shape, rows, act, packed):
+    """Every kernel that the dispatch knows; the CPU tests hold its shapes."""
+    tokens, experts, k, in_dim, out_dim = shape
+    say(f"linear_experts kernel {shape} {rows} {act} {packed}")
+    run_linear(torch, b1, unpack, spread_out(torch, tokens, experts, k, tokens), experts, in_dim, out_dim, rows, act,
+               packed)
+
+
+@pytest.mark.parametrize("tokens,experts,k,in_dim,out_dim", [
+    (20, 20, 2, 192, 2497), (100, 20, 3, 1088, 2303), (2721, 5, 3, 192, 131), (512, 20, 1, 1088, 2345),
+    (2829, 3, 3, 320, 333), (6000, 2, 1, 64, 2111)])
+def test_linear_experts_by_tiles_of_odd_widths(torch, b1, unpack, tokens, experts, k, in_dim, out_dim):
+    say(f"linear_experts odd tiles {tokens} {experts} {k} {in_dim} {out_dim}")
+    run_linear(torch, b1, unpack, spread_out(torch, tokens, experts, k, 5), experts, in_dim, out_dim, "tokens", "none",
+               False)
+
+
+@pytest.mark.parametrize("counts", [
+    [1, 0, 0, 0, 0], [0, 0, 0, 0, 1], [0, 1, 0, 1, 0], [4000, 1, 1, 1, 1], [1, 1, 1, 1, 300]])
+@pytest.mark.parametrize("tokens,in_dim,out_dim", [(60, 192, 2496), (2721, 192, 128), (4243, 320, 320)])
+def test_linear_experts_by_tiles_of_uneven_groups(torch, b1, unpack, tokens, in_dim, out_dim, counts):
+    say(f"linear_experts uneven tiles {tokens} {in_dim} {out_dim} {counts}")
+    expert = spread_out(torch, tokens, 5, 1, 3, counts)
+    expert[5::97] = -1
+    run_linear(torch, b1, unpack, expert, 5, in_dim, out_dim, "tokens", "swiglu", True)
+    run_linear(torch, b1, unpack, expert, 5, in_dim, out_dim - 1, "routes", "none", False)
+
+
 @pytest.mark.parametrize("out_dim", [1, 2, 15, 63, 65, 100, 129, 191, 193, 257, 1003])
 @pytest.mark.parametrize("tokens", [2, 40, 400])
 def test_linear_experts_of_odd_widths(torch, b1, unpack, out_dim, tokens):
@@ -290,7 +321,7 @@ def bad_starts(torch, routes, experts):
     yield "extremes", [-(1 << 31)] + [(1 << 31) - 1] * experts
 
 
-@pytest.mark.parametrize("tokens,experts,k", [(5, 6, 2), (300, 3, 2), (40, 130, 3)])
+@pytest.mark.parametrize("tokens,experts,k", [(5, 6, 2), (300, 3, 2), (40, 130, 3), (9000, 2, 1), (3000, 300, 2)])
 def test_bad_indices(torch, b1, tokens, experts, k):
     """Starts out of order or range make the call's rows NaN, an order entry
     or a place out of range its row; nothing else is touched, and `bad` says
