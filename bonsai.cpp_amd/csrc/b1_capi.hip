@@ -766,8 +766,8 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace, size_t wo
 int bonsai_b1_linear_experts(const bonsai_b1_experts_args *g, hipStream_t stream) {
     if (!g || !routes_ok(&g->routes)) return BONSAI_B1_ERR_ARG;
     const bonsai_b1_routes &r = g->routes;
-    if (g->in_dim <= 0 || g->in_dim % 64 || g->in_dim > (1 << 16) || g->out_dim <= 0 || g->out_dim > (1 << 17) ||
-        (int64_t)(g->in_dim / 32) * 6 * g->out_dim >= ((int64_t)1 << 31))
+    // (an expert's weights below 2^31 bytes)
+    if (g->in_dim <= 0 || g->in_dim % 64 || g->in_dim > (1 << 16) || g->out_dim <= 0 || g->out_dim > (1 << 17))
         return BONSAI_B1_ERR_ARG;
     // tokens' rows by 32-bit byte offsets
     if (g->by_token && (int64_t)r.tokens * g->in_dim >= ((int64_t)1 << 31)) return BONSAI_B1_ERR_ARG;

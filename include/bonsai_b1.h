@@ -811,9 +811,8 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
  * of the down projections; else y as fp32 in out (row stride ldo >= out_dim,
  * 4-byte aligned; act_fn NONE).
  * Of `routes` only start and (by_token) order are read, and tokens, experts,
- * top_k.  in_dim % 64 == 0, in_dim <= 2^16, out_dim <= 2^17, an expert's weights
- * below 2^31 bytes; by_token: tokens * in_dim < 2^31.  Outputs apart from the
- * inputs.
+ * top_k.  in_dim % 64 == 0, in_dim <= 2^16, out_dim <= 2^17; by_token:
+ * tokens * in_dim < 2^31.  Outputs apart from the inputs.
  * Numbers are those of FAST mode: products of fp16 in fp32 sums, in an order
  * that depends on tokens, experts, top_k, the widths and the output's kind
  * (they choose the kernel), not on the routes: the same call gives the same

@@ -76,7 +76,7 @@ PACKED = dict(out=None, ldo=0, packed=P, ldp=128)
     dict(out_dim=0), dict(out_dim=-1), dict(act_fn=1), dict(act_fn=2), dict(act_fn=3), dict(out=None),
     dict(out=P + 2), dict(ldo=127), dict(ldo=1 << 40), dict(packed=P, ldp=128), dict(nonfinite=P + 1),
     dict(bad=P + 2), dict(in_dim=65536 + 64), dict(out_dim=(1 << 17) + 1, ldo=1 << 18),
-    dict(in_dim=65536, out_dim=1 << 17, ldo=1 << 17), dict(in_dim=65536, routes=routes(tokens=32768))])
+    dict(in_dim=65536, routes=routes(tokens=32768))])
 def test_linear_experts(lib, change):
     assert lib.bonsai_b1_linear_experts(ctypes.byref(experts(**change)), None) == capi.ERR_ARG
 
