@@ -309,8 +309,12 @@ __global__ __launch_bounds__(kRouteThreads) void b1_route_kernel(RouteArgs a) {
 }
 
 // Many tokens, in two launches: each work-group chooses for `per` tokens and
-// counts their experts (16 bits: a token has an expert once; rows of a multiple of 4 counts); then each finds its
-// first row of every expert from all the counts and places its slots.
+// counts their experts (16 bits: a token has an expert once; rows of a
+// multiple of 4 counts); then each finds its first row of every expert from
+// all the counts and places its slots.  Bound by the choice's chain of scans
+// and, in the second launch, by the round trips to the counts: 8192 tokens of
+// 128 experts 8.7 + 6.3 us traced, where the logits' bytes would take 1 (with
+// unsorted lanes and 32-bit counts 9.3 + 7.6; 13.4 in a graph).
 __host__ __device__ constexpr int count_row(int experts) { return (experts + 3) / 4 * 4; }
 
 template <int EL, bool WIDE>
@@ -506,7 +510,9 @@ __device__ __forceinline__ floatx4 nan4() {
 constexpr uint32_t kNowhere = 0x80000000u;
 
 // silu(x) = x / (1 + 2^(-x log2 e)) by the hardware's exponential and
-// reciprocal, which feed an fp16 rounding: within (|x| + 4) half steps of fp32.
+// reciprocal, which feed an fp16 rounding: the exponent is rounded once and so
+// is its factor, the instructions are off by a step each: within 1.5 |x| + 7
+// half steps of fp32.
 __device__ __forceinline__ float silu_fast(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
 }
@@ -526,8 +532,14 @@ __device__ __forceinline__ void interleave() {
 
 // y = W a for up to 16 rows of one expert and `per` steps of 64 weight rows.
 //
-// Bound by the weights, read once a group (6 bytes a block of 32), and by the
-// shifts and selects that make fp16 of them, about 7 a lane and 8 weights.
+// The weights are read once a group (6 bytes a block of 32); what bounds it is
+// making fp16 of them and multiplying, 27 vector operations and four MFMAs a
+// block that overlap little: 512 rows over 128 experts, K = 2048, 1536 weight
+// rows (75 MB) 24.5 us, the same loads and sums without expansion or MFMAs
+// 16.5, the arithmetic without the loads 22.6.  Expanding a block
+// beside the MFMAs of the one before in a fixed order, two MFMA chains, two
+// steps of loads ahead: no gain.  The sums of each step by another wave first:
+// spread over all of them it took 1.4 us more.
 // MFMA 16x16x32 with 16 weight rows as the A operand and the rows of
 // activations as the B operand.  A wave takes U * 256 of K and lane (li, g)
 // two blocks (12 bytes) of weight row li for every 256: MFMA (b, c) of the 256
@@ -711,9 +723,25 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
 
 // ----------------------------------------------- many rows an expert ----
 
-// Tiles of BM rows of one expert and BN = NWN * WN weight rows.
+// Tiles of BM rows of one expert and BN = NWN * WN weight rows, by work-groups
+// that stay and take tiles in turn: a tile's rows are looked up while the one
+// before is computed, and its first stages are on their way while that one is
+// stored.
 //
-// MFMA 16x16x32, 16 weight rows as the A operand, rows of activations as the
+// Bound by the matrix units: in the loop over K, 128-row tiles run at 1.4
+// PFLOP/s counting the rows they do not have (clock about 1.8 GHz at the
+// board's power limit, where a library product of 8192^3 runs at 1.29).  65536
+// rows over 128 experts, K = 2048, 1536 weight rows with SwiGLU: 361 to 381 us
+// by board = 1.08 to 1.14 PFLOP/s of rows there are; one work-group a tile with its
+// sums stored through LDS took 459.  Fp32 rows add their
+// bytes' time (K = 768, 2048 columns, 537 MB: 287 to 302 us): the stores
+// hold up the loads of the CU's other work-group, counted waits or not.
+// Branches that skip the upper 64 rows of tiles without any saved what they
+// cost.  One loop over all stages, the reads behind the last one wasted: with
+// the last stages apart the compiler copied the sums between loops and spilled
+// (405 us).
+//
+// MFMA, 16 weight rows as the A operand, rows of activations as the
 // B operand.  A stage is 64 of K: BM rows of 128 bytes, shared by the waves,
 // their 16-byte chunks at c ^ row / 2 so that the 16 rows of a fragment read
 // cover all banks; and a wave's own WN columns of weights, 12 bytes a column
@@ -1093,7 +1121,8 @@ __global__ __launch_bounds__(C::NT, C::OCC) void b1_experts_tile_kernel(ExpertAr
 // ------------------------------------------------------------ combine ----
 
 // out[t] = residual[t] + sum_j weight[t][j] y[place[t][j]], 4 columns a
-// thread; bound by HBM (4 bytes a value of y, the residual and out).
+// thread; bound by HBM (4 bytes a value of y, the residual and out: 8192
+// tokens of 8 rows of 2048 134 us, 5.0 TB/s, the rate of a large copy).
 __global__ __launch_bounds__(256) void b1_combine_kernel(CombineArgs a) {
     const int token = blockIdx.x, col = (blockIdx.y * 256 + threadIdx.x) * 4;
     const int32_t *place = a.place + (int64_t)token * a.top_k;
@@ -1196,8 +1225,9 @@ double likely_groups(const ExpertArgs &a, int bm) {
 // 4 %; the kernel chosen takes 1.4 % more than the fastest of them on average,
 // 10 % at the 95th percentile, where one kernel by rows an expert alone takes
 // 18 % and 90 %): a fixed time, and for tiles the longer of what the rounds of
-// a CU's resident work-groups take one after another and what all its tiles take of its
-// matrix units, for few rows a work-group's steps beside the others on its CU.
+// a CU's resident work-groups take one after another and what all its tiles
+// take of its matrix units, for few rows a work-group's steps beside the
+// others on its CU.
 struct FewPlan {
     int waves, units, parts, per; // 256s of K a wave; work-groups a group of rows, steps each
     double us;
@@ -1209,7 +1239,8 @@ FewPlan plan_few(const ExpertArgs &a, int num_cus) {
     f.waves = units <= 3 || (units > 4 && units <= 6) ? 3 : units <= 8 ? 4 : 8;
     f.units = units <= 4 ? 1 : units <= 16 ? 2 : 4;
     const int steps = a.kind == 3 ? a.glu_h / 32 : (a.N + 63) / 64;
-    const int resident = (f.units == 1 ? 16 : f.units == 2 ? 12 : 8) / f.waves; // work-groups a CU, by their registers
+    // work-groups a CU, by their registers
+    const int resident = (f.units == 1 ? 16 : f.units == 2 ? 12 : 8) / f.waves;
     const double groups = likely_groups(a, 16);
     double best = 1e30;
     for (int p = 1; p <= steps; ++p) {

@@ -89,14 +89,18 @@ def linear(a, w):
 
 def activation(y, off, act):
     """act(y) and its bound for y off by `off`: silu' stays below 1.1, the
-    tanh form of gelu's slope below 1.13; the fp32 steps of silu and the
-    product with the value are 8 at most, gelu's are within 3e-7 max(1, |y|)."""
+    tanh form of gelu's slope below 1.13.  silu(g) by 2^(-g log2 e): the
+    exponent |g| log2 e is off by half a step for its product and a quarter for
+    its factor, times ln 2 in the power, 0.75 |g| steps = 1.5 |g| U32; power and reciprocal
+    by a step each, the sum, the product and the one with the value by half a
+    step each, and the constant 1 more: 1.5 |g| + 8 half steps.  gelu's are
+    within 3e-7 max(1, |y|)."""
     if act == "swiglu":
         h = y.shape[1] // 2
         g, v, og, ov = y[:, :h], y[:, h:], off[:, :h], off[:, h:]
         silu = g * torch.sigmoid(g)
         out = silu * v
-        return out, 1.1 * og * v.abs() + silu.abs() * ov + 1.1 * og * ov + 8 * U32 * out.abs() + 2.0 ** -126
+        return out, 1.1 * og * v.abs() + silu.abs() * ov + 1.1 * og * ov + (1.5 * g.abs() + 8) * U32 * out.abs() + 2.0 ** -126
     if act == "gelu_tanh":
         out = 0.5 * y * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (y + 0.044715 * y ** 3)))
         return out, 1.13 * off + 3e-7 * y.abs().clamp(min=1.0)
