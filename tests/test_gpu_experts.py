@@ -518,6 +518,64 @@ def test_a_capture_without_a_workspace(torch, b1):
     del g
 
 
+def test_large_kernels_captured(torch, b1):
+    """Kernels with more than 64 KB of LDS ask for it at every call, a captured
+    one too: 128-row tiles, one work-group that routes over 1024 experts."""
+    from bonsai_b1 import synth
+    say("large kernels captured")
+    tokens, experts, k, in_dim, out_dim = 2829, 3, 3, 320, 320
+    logits, wide = normal(torch, 1, tokens, experts), normal(torch, 2, 20, 1024)
+    acts = b1.pack_act_f16(normal(torch, 3, tokens, in_dim))
+    w = synth.device_packed_weights(experts * out_dim, in_dim, 4)
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+
+    def step():
+        r = b1.route(logits, k, workspace=ws)
+        return r, b1.linear_experts(acts, w, r, in_dim, out_dim), b1.route(wide, 6)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            got = step()
+        for turn in range(3):
+            logits.copy_(normal(torch, 10 + turn, tokens, experts))
+            wide.copy_(normal(torch, 20 + turn, 20, 1024))
+            g.replay()
+            stream.synchronize()
+            want = step()
+            stream.synchronize()
+            same_routes(torch, got[0], want[0])
+            same_routes(torch, got[2], want[2])
+            assert torch.equal(got[1], want[1])
+    del g
+
+
+@pytest.mark.parametrize("tokens,real", [(8, 5), (200, 77), (64, 0)])
+def test_padded_batch(torch, b1, tokens, real):
+    """Tokens whose experts are all off have no rows and get their residual;
+    the others come out as without them."""
+    from bonsai_b1 import synth
+    say(f"padded batch {tokens} {real}")
+    experts, k, h, f = 6, 2, 256, 64
+    x, logits = normal(torch, 1, tokens, h), normal(torch, 2, tokens, experts)
+    logits[real:] = -math.inf
+    up_w, down_w = (synth.device_packed_weights(experts * n, d, s) for n, d, s in ((2 * f, h, 4), (h, f, 5)))
+    acts = b1.pack_act_f16(x)
+    r = b1.route(logits, k)
+    assert int(r.start[-1]) == real * k and bool((r.order[real * k:] == -1).all())
+    up = torch.full((tokens * k * f * 2 + 16,), 255, dtype=torch.uint8, device="cuda")  # NaN where nothing is written
+    b1.linear_experts(acts, up_w, r, h, 2 * f, act="swiglu", packed=up)
+    y = torch.full((tokens * k, h), math.nan, device="cuda")
+    b1.linear_experts(up, down_w, r, f, h, rows="routes", out=y)
+    out = b1.combine_experts(y, r, residual=x)
+    assert torch.equal(out[real:], x[real:]) and bool(out.isfinite().all())
+    assert bool(y[real * k:].isnan().all())
+
+
 def test_calls_on_another_stream(torch, b1):
     """stream=: results, and outputs that belong to that stream."""
     from bonsai_b1 import synth
