@@ -1038,25 +1038,31 @@ class Routes:
         return self.start.shape[0] - 1
 
 
-_ROUTES = ("expert", "weight", "start", "order", "place")
+def _route_array(t, dtype, n, what):
+    """Pointer of one of a Routes' arrays, n contiguous values."""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"routes: {what} must be {n} contiguous values of {dtype}")
+    return t.data_ptr()
 
 
-def _routes_c(r, used=_ROUTES):
-    """The bonsai_b1_routes of a Routes, with the arrays that a call uses."""
-    if r.expert.dim() != 2 or r.start.dim() != 1:
+def _routes_size(r):
+    """tokens, experts and top_k of a Routes."""
+    s, n = r.expert.shape, r.start.numel()
+    if len(s) != 2 or r.start.dim() != 1:
         raise ValueError("expert must be [tokens, top_k], start a vector")
-    (tokens, k), n = r.expert.shape, r.start.numel()
     # (ctypes cuts integers to the field's width: the limits of the C entries)
-    if (tokens | k | n) >> 24:
+    if (s[0] | s[1] | n) >> 24:
         raise ValueError("tokens * top_k is limited to 2^24, experts to 1024")
-    c = RoutesC(tokens, n - 1, k)
-    for name in used:
-        t = getattr(r, name)
-        if t.dtype is not (_torch.float32 if name == "weight" else _torch.int32) or not t.is_contiguous() or \
-                t.numel() != (n if name == "start" else tokens * k):
-            raise ValueError(f"routes: {name} must be contiguous, int32 (weight fp32), a value a slot (start: experts + 1)")
-        setattr(c, name, t.data_ptr())
-    return c
+    return s[0], n - 1, s[1]
+
+
+def _routes_c(r):
+    """The bonsai_b1_routes of a Routes, all its arrays checked."""
+    tokens, experts, k = _routes_size(r)
+    i32, n = _torch.int32, tokens * k
+    return RoutesC(tokens, experts, k, _route_array(r.expert, i32, n, "expert"),
+                   _route_array(r.weight, _torch.float32, n, "weight"), _route_array(r.start, i32, experts + 1, "start"),
+                   _route_array(r.order, i32, n, "order"), _route_array(r.place, i32, n, "place"))
 
 
 def route(logits, top_k: int, score: str = "softmax", bias=None, renormalize: bool = True, scale: float = 1.0,
@@ -1118,15 +1124,18 @@ def linear_experts(packed_act, w_packed, routes, in_dim: int, out_dim: int, act:
         raise ValueError('rows is "tokens" or "routes"')
     dev = _on_current_device(packed_act, w_packed, routes.start, routes.order, out,
                              packed if packed is not True else None, nonfinite, bad)
-    c = _routes_c(routes, ("start", "order") if rows == "tokens" else ("start",))
-    n = c.tokens * c.top_k
+    tokens, experts, top_k = _routes_size(routes)
+    n = tokens * top_k
+    by_token = rows == "tokens"
+    c = RoutesC(tokens, experts, top_k, None, None, _route_array(routes.start, _torch.int32, experts + 1, "start"),
+                _route_array(routes.order, _torch.int32, n, "order") if by_token else None, None)
     if in_dim <= 0 or out_dim <= 0 or (in_dim | out_dim) >> 31:
         raise ValueError("in_dim and out_dim are positive")
     if not packed_act.is_contiguous() or packed_act.numel() * packed_act.element_size() < \
-            (c.tokens if rows == "tokens" else n) * in_dim * 2:
+            (tokens if by_token else n) * in_dim * 2:
         raise ValueError("packed_act must hold the rows' in_dim fp16 elements, contiguous")
     if w_packed.dtype is not _torch.uint8 or not w_packed.is_contiguous() or \
-            w_packed.numel() != c.experts * out_dim * (in_dim // BLOCK_SIZE) * BLOCK_BYTES:
+            w_packed.numel() != experts * out_dim * (in_dim // BLOCK_SIZE) * BLOCK_BYTES:
         raise ValueError("w_packed must be contiguous uint8 of experts * out_dim * in_dim/32 * 6 bytes")
     cols = out_dim // 2 if act == "swiglu" else out_dim
     p = o = None
@@ -1139,7 +1148,7 @@ def linear_experts(packed_act, w_packed, routes, in_dim: int, out_dim: int, act:
     else:
         y = out if out is not None else _empty(stream, (n, out_dim), _torch.float32, dev)
         o, ldo, ldp = y.data_ptr(), _f32_rows(y, n, out_dim, "out"), 0
-    args = ExpertsArgs(c, packed_act.data_ptr(), 1 if rows == "tokens" else 0, w_packed.data_ptr(), in_dim, out_dim,
+    args = ExpertsArgs(c, packed_act.data_ptr(), 1 if by_token else 0, w_packed.data_ptr(), in_dim, out_dim,
                        ACTS[act], p, ldp, o, ldo, _counter(nonfinite), _counter(bad))
     st = lib.bonsai_b1_linear_experts(ctypes.byref(args), _raw_stream(stream, dev))
     if st != OK:
@@ -1154,16 +1163,19 @@ def combine_experts(y, routes, residual=None, out=None, bad=None, stream=None):
     may be residual.  Returns out [tokens, H]."""
     lib = _lib or load()
     dev = _on_current_device(y, routes.weight, routes.place, residual, out, bad)
-    c = _routes_c(routes, ("weight", "place"))
+    tokens, experts, top_k = _routes_size(routes)
+    n = tokens * top_k
+    c = RoutesC(tokens, experts, top_k, None, _route_array(routes.weight, _torch.float32, n, "weight"), None, None,
+                _route_array(routes.place, _torch.int32, n, "place"))
     if y.dim() != 2:
         raise ValueError("y must be [tokens * top_k, H]")
     h = y.shape[1]
-    ldy = _f32_rows(y, c.tokens * c.top_k, h, "y")
-    r_p, ldr = (residual.data_ptr(), _f32_rows(residual, c.tokens, h, "residual")) if residual is not None else (None, 0)
+    ldy = _f32_rows(y, n, h, "y")
+    r_p, ldr = (residual.data_ptr(), _f32_rows(residual, tokens, h, "residual")) if residual is not None else (None, 0)
     if out is None:
-        out = _empty(stream, (c.tokens, h), _torch.float32, dev)
+        out = _empty(stream, (tokens, h), _torch.float32, dev)
     st = lib.bonsai_b1_combine_experts(ctypes.byref(c), y.data_ptr(), ldy, h, r_p, ldr, out.data_ptr(),
-                                       _f32_rows(out, c.tokens, h, "out"), _counter(bad), _raw_stream(stream, dev))
+                                       _f32_rows(out, tokens, h, "out"), _counter(bad), _raw_stream(stream, dev))
     if st != OK:
         raise B1Error(st, "bonsai_b1_combine_experts")
     return out

@@ -1243,9 +1243,9 @@ FewPlan plan_few(const ExpertArgs &a, int num_cus) {
     const int resident = (f.units == 1 ? 16 : f.units == 2 ? 12 : 8) / f.waves;
     const double groups = likely_groups(a, 16);
     double best = 1e30;
-    for (int p = 1; p <= steps; ++p) {
-        const int per = (steps + p - 1) / p;
-        if ((steps + per - 1) / per != p) continue; // fewer parts of as many steps
+    int per = steps;
+    for (int p = 1; p <= steps; p = per > 1 ? (steps + per - 2) / (per - 1) : steps + 1) { // the parts of each size
+        per = (steps + p - 1) / p;
         const double wgs = std::ceil(groups * p / num_cus), beside = std::min(wgs, (double)resident);
         const double rounds = std::ceil(wgs / resident), cost = rounds * (3.0 + per * (beside + 1.0));
         if (cost < best) {
