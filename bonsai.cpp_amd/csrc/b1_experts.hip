@@ -536,10 +536,11 @@ __device__ __forceinline__ void interleave() {
 // making fp16 of them and multiplying, 27 vector operations and four MFMAs a
 // block that overlap little: 512 rows over 128 experts, K = 2048, 1536 weight
 // rows (75 MB) 24.5 us, the same loads and sums without expansion or MFMAs
-// 16.5, the arithmetic without the loads 22.6.  Expanding a block
-// beside the MFMAs of the one before in a fixed order, two MFMA chains, two
-// steps of loads ahead: no gain.  The sums of each step by another wave first:
-// spread over all of them it took 1.4 us more.
+// 16.5, the arithmetic without the loads 22.6.  Expanding a block beside the
+// MFMAs of the one before in a fixed order, two MFMA chains, two steps of loads
+// ahead: no gain.  The sums of each step by another wave first: spread over all
+// of them it took 1.4 us more.
+//
 // MFMA 16x16x32 with 16 weight rows as the A operand and the rows of
 // activations as the B operand.  A wave takes U * 256 of K and lane (li, g)
 // two blocks (12 bytes) of weight row li for every 256: MFMA (b, c) of the 256
@@ -732,10 +733,10 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
 // PFLOP/s counting the rows they do not have (clock about 1.8 GHz at the
 // board's power limit, where a library product of 8192^3 runs at 1.29).  65536
 // rows over 128 experts, K = 2048, 1536 weight rows with SwiGLU: 361 to 381 us
-// by board = 1.08 to 1.14 PFLOP/s of rows there are; one work-group a tile with its
-// sums stored through LDS took 459.  Fp32 rows add their
-// bytes' time (K = 768, 2048 columns, 537 MB: 287 to 302 us): the stores
-// hold up the loads of the CU's other work-group, counted waits or not.
+// by board = 1.08 to 1.14 PFLOP/s of rows there are; one work-group a tile with
+// its sums stored through LDS took 459.  Fp32 rows add their bytes' time
+// (K = 768, 2048 columns, 537 MB: 287 to 302 us): the stores hold up the loads
+// of the CU's other work-group, counted waits or not.
 // Branches that skip the upper 64 rows of tiles without any saved what they
 // cost.  One loop over all stages, the reads behind the last one wasted: with
 // the last stages apart the compiler copied the sums between loops and spilled
@@ -876,8 +877,9 @@ __global__ __launch_bounds__(C::NT, C::OCC) void b1_experts_tile_kernel(ExpertAr
     uint8_t *const sw0 = smem + C::WBASE + wn * (C::RW * C::WGRP);
     int wfill;
     auto load_slice = [&](int at, int group) {
-        // (a group's stages past K: zeros past the buffer or the next row's, never used)
-        dma_buf_lds12s(wrs, sw0 + at, boff[0], (uint32_t)(min(group, last_group) * C::L * 12));
+        // (a group's stages past K are the next row's, or zeros past the buffer,
+        // whose end the lanes' offsets are checked against; never used)
+        dma_buf_lds12s(wrs, sw0 + at, boff[0] + (uint32_t)(min(group, last_group) * C::L * 12), 0);
         const uint32_t b0 = boff[0];
 #pragma unroll
         for (int i = 0; i + 1 < C::L; ++i) boff[i] = boff[i + 1];
