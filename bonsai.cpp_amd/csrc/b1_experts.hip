@@ -89,6 +89,9 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f); // -0 is 0
         return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
     };
+    auto value_of = [](uint32_t key) {
+        return __builtin_bit_cast(float, key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
+    };
 #pragma unroll
     for (int i = 0; i < EL; ++i) {
         const int e = lane * EL + i;
@@ -102,7 +105,7 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         top = max(top, hi[i]);
     }
     top = wave_max(top);
-    const float peak = __builtin_bit_cast(float, top ^ ((top >> 31) ? 0x80000000u : 0xffffffffu));
+    const float peak = value_of(top);
     float all = 0.f; // softmax over all experts
     if (!a.sigmoid && !a.renormalize) {
 #pragma unroll
@@ -210,7 +213,13 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         }
         weight = (float)(s * (double)a.scale);
     } else {
-        const float p = mine >= 0 ? expf(mine_x - peak) : 0.f;
+        // divided by their sum the chosen weights do not depend on what is
+        // subtracted: the largest chosen logit (without a bias the largest of
+        // all), so that none far above, left out by its bias, takes them to 0
+        float from = peak;
+        if constexpr (WIDE)
+            if (a.renormalize) from = value_of(wave_max(mine_x > -INFINITY ? key_of(mine_x) : 0u));
+        const float p = mine >= 0 ? expf(mine_x - from) : 0.f;
         weight = p / (a.renormalize ? wave_sum(p) : all) * a.scale;
     }
     if (any_nan) weight = __builtin_nanf("");

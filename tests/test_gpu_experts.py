@@ -108,6 +108,38 @@ def test_route_of_unusual_rows(torch, b1, score, with_bias, renormalize, tokens)
         check_routes(torch, r, x, k, score=score, bias=bias, renormalize=renormalize)
 
 
+@pytest.mark.parametrize("off", [-math.inf, -4.0])
+@pytest.mark.parametrize("experts", [6, 40, 100, 200, 400, 900])
+@pytest.mark.parametrize("tokens", [9, 90])
+def test_route_far_behind_a_logit_that_is_not_chosen(torch, b1, tokens, experts, off):
+    """Renormalized softmax weights depend on the chosen logits alone, however
+    far below the largest one they lie, which the bias turns off or puts
+    behind.  The bound: differences of at most `spread` to the largest chosen
+    logit, rounded (half a step each), an exponential (2 steps), a sum of four
+    (3 half steps), in numerator and denominator, and a division."""
+    say(f"route far behind {tokens} {experts} {off}")
+    k, peak = 4, experts // 3
+    far = torch.tensor([80.0, 87.5, 95.0, 103.0, 104.0, 120.0, 300.0, 1000.0, 3e38], device="cuda")
+    x = normal(torch, experts, tokens, experts)
+    x[:, peak] = far[torch.arange(tokens, device="cuda") % len(far)]
+    # steps of 2^-10 tell the others apart: their scores are below 1e-30
+    rank = torch.randperm(experts, generator=torch.Generator().manual_seed(experts))
+    bias = -rank.float() / 1024
+    bias[peak] = off
+    chosen = torch.argsort(bias, descending=True)[:k]
+    assert peak not in chosen.tolist()
+    r = b1.route(x, k, bias=bias.cuda())
+    expert = chosen.int().expand(tokens, k)
+    assert torch.equal(r.expert.cpu(), expert)
+    z = x.cpu().double()[:, chosen]
+    z = z - z.amax(1, keepdim=True)
+    want = z.exp() / z.exp().sum(1, keepdim=True)
+    spread = -z.amin(1, keepdim=True)
+    ref.check(r.weight, want, want * (2 * spread + 16) * ref.U32, torch.float32, "weights")
+    for got, at in zip((r.start, r.order, r.place), moe.layout(expert, experts)):
+        assert torch.equal(got.cpu(), at)
+
+
 def same_routes(torch, a, b):
     for name in ("expert", "start", "order", "place"):
         assert torch.equal(getattr(a, name), getattr(b, name)), name
