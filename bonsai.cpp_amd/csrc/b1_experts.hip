@@ -100,7 +100,7 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
     }
 #pragma unroll
     for (int i = 0; i < EL; ++i) {
-        nan |= x[i] != x[i];
+        nan |= x[i] != x[i] || (!a.sigmoid && x[i] == INFINITY);
         hi[i] = x[i] > -INFINITY ? key_of(x[i]) : x[i] != x[i] ? kNanKey : 0u;
         top = max(top, hi[i]);
     }
@@ -124,13 +124,16 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
             }
         }
         if (!a.sigmoid) sum = wave_sum(sum);
-        // an infinite logit: weights NaN, chosen by the logits
+        // an infinite logit: weights NaN, chosen by the logits of those not off
         const bool by_score = a.sigmoid || sum < (double)INFINITY;
 #pragma unroll
         for (int i = 0; i < EL; ++i) {
             lo[i] = 0;
-            if (!by_score || id[i] >= a.experts || hi[i] <= kNanKey) continue;
-            const double k = (a.sigmoid ? z[i] : z[i] / sum) + (double)a.bias[id[i]] + 0.0;
+            if (id[i] >= a.experts) continue;
+            const float bias = a.bias[id[i]];
+            if (bias == -INFINITY) hi[i] = 0; // off, whatever its logit
+            if (!by_score || hi[i] <= kNanKey) continue;
+            const double k = (a.sigmoid ? z[i] : z[i] / sum) + (double)bias + 0.0;
             const uint64_t b = __builtin_bit_cast(uint64_t, k);
             const uint64_t key = b ^ ((b >> 63) ? ~0ull : 1ull << 63);
             nan |= k != k;

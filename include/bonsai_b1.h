@@ -771,7 +771,8 @@ enum { BONSAI_B1_SCORE_SOFTMAX = 0, BONSAI_B1_SCORE_SIGMOID = 1 };
  * divided with `renormalize` by the sum of the token's chosen ones (0 where
  * that is 0), times `scale`.  The bias is no part of it.
  * A NaN among a token's logits or scores, or with softmax +inf, makes its
- * weights NaN (NaN is chosen behind every number).
+ * weights NaN (NaN is chosen behind every number; with softmax and +inf the
+ * choice goes by the logits of the experts that are not off).
  * Writes all arrays of `routes`, the same on every call with the same logits.
  * workspace: bonsai_b1_route_workspace_bytes(args) bytes (16-byte aligned),
  * or NULL for the library's per-stream workspace, with the rules of

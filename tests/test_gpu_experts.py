@@ -140,6 +140,35 @@ def test_route_far_behind_a_logit_that_is_not_chosen(torch, b1, tokens, experts,
         assert torch.equal(got.cpu(), at)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts", [6, 100, 200, 400, 900])
+@pytest.mark.parametrize("tokens", [7, 70])
+def test_route_never_chooses_what_a_bias_turns_off(torch, b1, tokens, experts, score):
+    """An expert whose bias is -inf has no rows, whatever the logits are: NaN
+    and infinities among them, its own or others'."""
+    say(f"route off by bias {tokens} {experts} {score}")
+    on = [1, experts // 2, experts - 1]
+    off = [e for e in range(experts) if e not in on]
+    bias = torch.full((experts,), -math.inf, device="cuda")
+    bias[on] = 0.0
+    x = normal(torch, 1, tokens, experts)
+    x[0, on[1]] = math.inf
+    x[1] = math.nan
+    x[2, off[0]] = math.nan
+    x[3, [on[0], off[1]]] = math.inf
+    x[4, off[-1]] = math.inf
+    x[5, off] = math.inf
+    r = b1.route(x, 4, score=score, bias=bias)
+    expert = r.expert.cpu()
+    assert bool((expert[:, 3] == -1).all()) and expert[:, :3].sort(1).values.tolist() == [on] * tokens
+    for got, at in zip((r.start, r.order, r.place), moe.layout(expert, experts)):
+        assert torch.equal(got.cpu(), at)
+    nan = torch.zeros(tokens, dtype=torch.bool)
+    nan[[1, 2] + ([0, 3, 4, 5] if score == "softmax" else [])] = True
+    weight = r.weight.cpu()
+    assert torch.equal(weight[:, :3].isnan(), nan[:, None].expand(tokens, 3)) and bool((weight[:, 3] == 0).all())
+
+
 def same_routes(torch, a, b):
     for name in ("expert", "start", "order", "place"):
         assert torch.equal(getattr(a, name), getattr(b, name)), name
