@@ -248,6 +248,14 @@ __device__ __forceinline__ uint32_t lds_prefix(uint32_t *v, int n) {
     return before;
 }
 
+// Orders the accesses of a wave's lanes to what they share, before it and
+// behind it (no instruction by itself: a wave's LDS accesses run in order).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Places of slots [s0, s1) of `expert` by a whole work-group: slot s of expert
 // e goes to row base[e] + the number of e's slots before s.  A wave takes a
 // contiguous part; counts[wave][expert] (LDS) become the parts' first rows.
@@ -283,13 +291,14 @@ __device__ __forceinline__ void route_place(const RouteArgs &a, int64_t s0, int6
             const uint64_t one = __ballot((e >> b) & 1);
             same &= (e >> b) & 1 ? one : ~one;
         }
-        int at = -1;
-        if (e >= 0) {
-            const int before = __popcll(same & ((1ull << lane) - 1));
-            at = (int)(mine[e] + (uint32_t)before);
-            if (before == 0) mine[e] = (uint32_t)at + (uint32_t)__popcll(same);
-            a.order[at] = (int)slot;
-        }
+        // all of them read the expert's next row before their first moves it on,
+        // and the next turn reads it behind that
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        const int at = e >= 0 ? (int)(mine[e] + (uint32_t)before) : -1;
+        wave_sync();
+        if (e >= 0 && before == 0) mine[e] = (uint32_t)at + (uint32_t)__popcll(same);
+        wave_sync();
+        if (e >= 0) a.order[at] = (int)slot;
         if (slot < p1) a.place[slot] = at;
     }
 }

@@ -169,6 +169,20 @@ def test_route_never_chooses_what_a_bias_turns_off(torch, b1, tokens, experts, s
     assert torch.equal(weight[:, :3].isnan(), nan[:, None].expand(tokens, 3)) and bool((weight[:, 3] == 0).all())
 
 
+@pytest.mark.parametrize("tokens", [1, 32, 33, 1000, 4099])
+@pytest.mark.parametrize("experts,k", [(1, 1), (2, 2), (3, 1), (8, 8)])
+def test_route_of_experts_that_all_tokens_want(torch, b1, tokens, experts, k):
+    """Every lane of a wave places a row of the same few experts, turn after
+    turn: in an expert's rows the slots still ascend."""
+    say(f"route all alike {tokens} {experts} {k}")
+    logits = torch.zeros(tokens, experts, device="cuda")
+    r = b1.route(logits, k)
+    expert = torch.arange(k, dtype=torch.int32).expand(tokens, k)
+    assert torch.equal(r.expert.cpu(), expert)
+    for got, at in zip((r.start, r.order, r.place), moe.layout(expert, experts)):
+        assert torch.equal(got.cpu(), at)
+
+
 def same_routes(torch, a, b):
     for name in ("expert", "start", "order", "place"):
         assert torch.equal(getattr(a, name), getattr(b, name)), name
