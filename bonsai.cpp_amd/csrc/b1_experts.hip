@@ -405,9 +405,10 @@ __global__ __launch_bounds__(kRouteThreads) void b1_route_place_kernel(RouteArgs
 // How many groups of up to BM rows of one expert there are, counting through
 // the experts in order, and lane l's share: experts l * each .. of them, the
 // first's rows from edge[0] on and its groups `before` the next lane's.  By a
-// whole wave.  Starts are brought into range and order first, so that any
-// contents of `start` give groups within the rows, apart from one another, and
-// no more of them than group_bound() says.  Up to 256 experts a lane keeps its
+// whole wave.  With starts out of order or range every row of the call is the
+// first expert's, so that any contents of `start` give groups within the rows,
+// apart from one another, no more of them than group_bound() says, and none of
+// the rows that become NaN is left out.  Up to 256 experts a lane keeps its
 // experts' edges (its loads all on their way at once), with more it reads them
 // again in find_group().
 constexpr int kEdges = 4;
@@ -422,50 +423,39 @@ __device__ __forceinline__ Groups count_groups(const int32_t *start, int experts
     Groups g;
     g.each = (experts + 63) / 64;
     const int e0 = min(lane * g.each, experts), e1 = min(e0 + g.each, experts);
-    auto within = [&](int v) { return (uint32_t)min(max(v, 0), routes); };
     auto groups = [&](uint32_t rows) { return (rows + BM - 1) / BM; };
     bool bad;
-    uint32_t top, n = 0;
+    uint32_t n = 0;
     if (g.each <= kEdges) {
         int v[kEdges + 1];
 #pragma unroll
         for (int i = 0; i <= kEdges; ++i) v[i] = start[min(e0 + i, e1)];
         bad = v[0] < 0 || v[kEdges] > routes;
+        g.edge[0] = (uint32_t)v[0];
 #pragma unroll
-        for (int i = 0; i < kEdges; ++i) bad |= v[i + 1] < v[i];
-        g.edge[0] = within(v[0]);
-#pragma unroll
-        for (int i = 1; i <= kEdges; ++i) g.edge[i] = max(g.edge[i - 1], within(v[i]));
-        top = g.edge[kEdges];
+        for (int i = 0; i < kEdges; ++i) {
+            bad |= v[i + 1] < v[i];
+            g.edge[i + 1] = (uint32_t)v[i + 1];
+            n += groups(g.edge[i + 1] - g.edge[i]);
+        }
     } else {
         int last = start[e0];
         bad = last < 0;
-        top = g.edge[0] = within(last);
+        g.edge[0] = (uint32_t)last;
         for (int e = e0; e < e1; ++e) {
             const int v = start[e + 1];
             bad |= v < last;
+            n += groups((uint32_t)v - (uint32_t)last);
             last = v;
-            top = max(top, within(v));
         }
         bad |= last > routes;
     }
     g.bad = __ballot(bad) != 0;
-    if (g.bad) { // no start before an earlier one
-        const uint32_t floor = __shfl_up(scan_max(top), 1);
-        if (lane) g.edge[0] = max(g.edge[0], floor);
+    if (g.bad) {
+        g.edge[0] = lane ? (uint32_t)routes : 0u;
 #pragma unroll
-        for (int i = 1; i <= kEdges; ++i) g.edge[i] = max(g.edge[i], g.edge[0]);
-    }
-    if (g.each <= kEdges) {
-#pragma unroll
-        for (int i = 0; i < kEdges; ++i) n += groups(g.edge[i + 1] - g.edge[i]);
-    } else {
-        uint32_t row = g.edge[0];
-        for (int e = e0; e < e1; ++e) {
-            const uint32_t end = max(row, within(start[e + 1]));
-            n += groups(end - row);
-            row = end;
-        }
+        for (int i = 1; i <= kEdges; ++i) g.edge[i] = (uint32_t)routes;
+        n = groups((uint32_t)routes - g.edge[0]);
     }
     g.before = scan_add(n);
     g.total = lane_value(g.before, 63);
@@ -498,7 +488,7 @@ __device__ __forceinline__ Group find_group(const Groups &g, const int32_t *star
         }
     } else {
         for (;; ++e) {
-            end = max(row, (uint32_t)min(max(start[e + 1], 0), routes));
+            end = (uint32_t)(g.bad ? routes : start[e + 1]);
             const uint32_t n = (end - row + BM - 1) / BM;
             if (left < n || e + 1 >= experts) break;
             left -= n;

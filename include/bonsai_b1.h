@@ -820,9 +820,9 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
  * bits.  SwiGLU's silu(x) uses the device's exponential and reciprocal
  * instructions, within 1.5 |x| + 7 half steps of fp32 before the rounding to
  * fp16 (other entries use its library exponential: not the same bits).
- * The non-finite counter counts y.  Starts out of order or range make every
- * row of the call NaN, an order entry out of range its row; `bad` grows by at
- * least 1 then, and nothing out of range is read or written.
+ * The non-finite counter counts y.  Starts out of order or range make all
+ * tokens * top_k rows NaN, an order entry out of range its row; `bad` grows by
+ * at least 1 then, and nothing out of range is read or written.
  */
 typedef struct bonsai_b1_experts_args {
     bonsai_b1_routes routes;

@@ -444,6 +444,50 @@ def test_bad_indices(torch, b1, tokens, experts, k):
         assert int(bad) >= 1 and bool(out[2].isnan().all()) and torch.equal(out[keep], want[keep])
 
 
+@pytest.mark.parametrize("act,packed", [("none", False), ("none", True), ("gelu_tanh", True), ("swiglu", True)])
+@pytest.mark.parametrize("tokens,experts,k,in_dim,out_dim", [
+    (40, 3, 2, 192, 256), (30, 900, 2, 128, 64), (200, 33, 6, 128, 576), (512, 20, 1, 1088, 2368),
+    (2721, 5, 3, 192, 128), (6000, 2, 1, 64, 2112), (3000, 300, 2, 192, 64)])
+def test_bad_indices_leave_no_row(torch, b1, tokens, experts, k, in_dim, out_dim, act, packed):
+    """Starts out of order or range make every row NaN, an order entry out of
+    range its row, in every kind of output; columns and rows around them stay
+    as they were."""
+    from bonsai_b1 import synth
+    good = routes_of(torch, b1, spread_out(torch, tokens, experts, k, 1), experts)
+    routes = tokens * k
+    a = b1.pack_act_f16(normal(torch, 1, tokens, in_dim))
+    w = synth.device_packed_weights(experts * out_dim, in_dim, 3)
+    cols = out_dim // 2 if act == "swiglu" else out_dim
+
+    def call(r):
+        bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+        dtype = torch.float16 if packed else torch.float32
+        guard = torch.full((routes + 16, cols + 8), 7.5, dtype=dtype, device="cuda")
+        inside = guard[8:8 + routes]
+        if packed:
+            b1.linear_experts(a, w, r, in_dim, out_dim, act=act, bad=bad,
+                              packed=inside.view(torch.uint8).flatten(), ldp=cols + 8)
+        else:
+            b1.linear_experts(a, w, r, in_dim, out_dim, bad=bad, out=inside[:, :cols])
+        assert bool((guard[:8] == 7.5).all()) and bool((guard[8 + routes:] == 7.5).all())
+        assert bool((inside[:, cols:] == 7.5).all())
+        return inside[:, :cols], int(bad)
+
+    fine, bad = call(good)
+    assert bad == 0 and bool(fine.isfinite().all())
+    for what, values in bad_starts(torch, routes, experts):
+        say(f"bad starts {what} {tokens} {experts} {act} {packed}")
+        y, bad = call(b1.Routes(good.expert, good.weight, torch.tensor(values, dtype=torch.int32, device="cuda"),
+                                good.order, good.place))
+        assert bad >= 1 and bool(y.isnan().all()), what
+    for value in (-1, routes, -(1 << 31)):
+        order = good.order.clone()
+        order[[0, routes - 1]] = value
+        y, bad = call(b1.Routes(good.expert, good.weight, good.start, order, good.place))
+        assert bad == 2 and bool(y[[0, routes - 1]].isnan().all())
+        assert torch.equal(y[1:-1], fine[1:-1])
+
+
 def test_no_rows(torch, b1):
     r = b1.route(torch.empty(0, 4, device="cuda"), 2)
     w = torch.zeros(4 * 64 * 2 * 6, dtype=torch.uint8, device="cuda")
