@@ -311,6 +311,42 @@ def test_linear_experts_by_each_kernel(torch, b1, unpack, shape, rows, act, pack
                packed)
 
 
+@pytest.mark.parametrize("rows", ["tokens", "routes"])
+@pytest.mark.parametrize("act,packed", [("none", False), ("none", True), ("gelu_tanh", True), ("swiglu", True)])
+@pytest.mark.parametrize("shape", list(moe.KERNELS) + [(1, 128, 8, 2048, 192), (300, 20, 3, 1344, 1408)])
+def test_linear_experts_lose_no_product(torch, b1, unpack, shape, rows, act, packed):
+    """Activations of +-1, 2, 3 and scales of 2^-5, 2^-4, 2^-3: every partial sum
+    is a multiple of 2^-5 below 2^13, exact in fp32 in any order, so that a
+    single product lost or taken twice shows at any width.  Rows are equal to
+    the definition's, plain packed rows to their rounding; behind an activation
+    only its own steps count."""
+    from bonsai_b1 import synth
+    tokens, experts, k, in_dim, out_dim = shape
+    say(f"linear_experts exact {shape} {rows} {act} {packed}")
+    r = routes_of(torch, b1, spread_out(torch, tokens, experts, k, tokens), experts)
+    n = tokens * k
+    have = tokens if rows == "tokens" else n
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens + in_dim)
+    a = torch.randint(1, 4, (have, in_dim), generator=g, device="cuda").float()
+    a *= torch.randint(0, 2, a.shape, generator=g, device="cuda") * 2 - 1
+    w = synth.device_packed_weights(experts * out_dim, in_dim, 12).view(-1, 6)
+    w[:, :2] = (2.0 ** torch.randint(-5, -2, (len(w), 1), generator=g, device="cuda")).half().view(torch.uint8)
+    w = w.flatten()
+    cols = out_dim // 2 if act == "swiglu" else out_dim
+    y = b1.linear_experts(b1.pack_act_f16(a), w, r, in_dim, out_dim, act=act, rows=rows, packed=packed or None)
+    got = ref.unpack(y, n, cols) if packed else y
+    order = r.order.cpu()
+    want, _ = moe.experts(a.cpu(), unpack(w, experts * out_dim, in_dim).cpu().view(experts, out_dim, in_dim),
+                          r.start.cpu(), order, k, rows == "tokens")
+    assert bool((want.abs() < 2 ** 13).all()) and torch.equal(want * 32, (want * 32).round())
+    if act == "none":
+        assert torch.equal(got.cpu(), want.to(torch.float16 if packed else torch.float32))
+        return
+    want, off = moe.activation(want, torch.zeros_like(want), act)
+    ref.check(got, want, off, torch.float16, "rows")
+
+
 @pytest.mark.parametrize("tokens,experts,k,in_dim,out_dim", [
     (20, 20, 2, 192, 2497), (100, 20, 3, 1088, 2303), (2721, 5, 3, 192, 131), (512, 20, 1, 1088, 2345),
     (2829, 3, 3, 320, 333), (6000, 2, 1, 64, 2111)])
