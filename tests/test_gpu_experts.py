@@ -778,3 +778,41 @@ def test_rows_past_32_bit_offsets(torch, b1, unpack):
     assert torch.equal(out, y)
     del a, y, out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens,experts,in_dim,out_dim", [
+    (262143, 1024, 8192, 64), (262143, 1000, 8192, 256), (32767, 1024, 65536, 64), (16384, 1024, 65536, 63)])
+def test_token_rows_past_31_bit_offsets(torch, b1, unpack, tokens, experts, in_dim, out_dim):
+    """Up projections over tokens whose rows take up to 2^32 bytes, the most
+    that is accepted: the same rows as from activations gathered beforehand,
+    and some of them against float64."""
+    from bonsai_b1 import synth
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of free device memory")
+    say(f"token rows past 31-bit offsets {tokens} {experts} {in_dim} {out_dim}")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens)
+    expert = torch.randint(0, experts, (tokens, 1), generator=g, device="cuda", dtype=torch.int32)
+    order = torch.argsort(expert.flatten(), stable=True)
+    place = torch.empty_like(order)
+    place[order] = torch.arange(tokens, device="cuda")
+    start = torch.bincount(expert.flatten(), minlength=experts).cumsum(0)
+    r = b1.Routes(expert, torch.ones(tokens, 1, device="cuda"), torch.cat([start.new_zeros(1), start]).int(),
+                  order.int(), place.int().view(tokens, 1))
+    a = torch.empty(tokens, in_dim, dtype=torch.float16, device="cuda").normal_(generator=g)
+    assert 1 << 31 <= 2 * a.numel() < 1 << 32
+    w = synth.device_packed_weights(experts * out_dim, in_dim, 2)
+    y = b1.linear_experts(a.view(torch.uint8), w, r, in_dim, out_dim)
+    gathered = torch.empty_like(a)
+    for at in torch.arange(tokens, device="cuda").split(1 << 15):
+        gathered[at] = a[order[at]]
+    assert torch.equal(y, b1.linear_experts(gathered.view(torch.uint8), w, r, in_dim, out_dim, rows="routes"))
+    for t in (0, 1, tokens // 2 - 1, tokens // 2, tokens // 2 + 1, tokens - 1):
+        e, row = int(expert[t]), int(place[t])
+        w64 = unpack(w.view(experts, -1)[e], out_dim, in_dim).cpu()
+        want, off = moe.linear(ref.unpack(a[t].view(torch.uint8), 1, in_dim), w64)
+        ref.check(y[row:row + 1], want, off, torch.float32, f"token {t}")
+    del a, gathered, y
+    torch.cuda.empty_cache()
