@@ -523,7 +523,10 @@ constexpr uint32_t kNowhere = 0x80000000u;
 // silu(x) = x / (1 + 2^(-x log2 e)) by the hardware's exponential and
 // reciprocal, which feed an fp16 rounding: the exponent is rounded once and so
 // is its factor, the instructions are off by a step each: within 1.5 |x| + 7
-// half steps of fp32.
+// half steps of fp32 from x = -87 on.  Below, the reciprocal leaves the normal
+// numbers and becomes 0 (as the exponential becomes infinite): off by less than
+// 87 e^-87 < 1.5e-36, which no finite value (below 2^49 from fp16 inputs, scales
+// and 2^16 products) brings near fp16's smallest 2^-24.
 __device__ __forceinline__ float silu_fast(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
 }

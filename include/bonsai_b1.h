@@ -818,8 +818,9 @@ int bonsai_b1_route(const bonsai_b1_route_args *args, void *workspace,
  * that depends on tokens, experts, top_k, the widths and the output's kind
  * (they choose the kernel), not on the routes: the same call gives the same
  * bits.  SwiGLU's silu(x) uses the device's exponential and reciprocal
- * instructions, within 1.5 |x| + 7 half steps of fp32 before the rounding to
- * fp16 (other entries use its library exponential: not the same bits).
+ * instructions, before the rounding to fp16 within 1.5 |x| + 7 half steps of
+ * fp32 from x = -87 on and within 1.5e-36 below, where it becomes 0 (other
+ * entries use its library exponential: not the same bits).
  * The non-finite counter counts y.  Starts out of order or range make all
  * tokens * top_k rows NaN, an order entry out of range its row; `bad` grows by
  * at least 1 then, and nothing out of range is read or written.

@@ -816,3 +816,28 @@ def test_token_rows_past_31_bit_offsets(torch, b1, unpack, tokens, experts, in_d
         ref.check(y[row:row + 1], want, off, torch.float32, f"token {t}")
     del a, gathered, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens,experts", [(41, 8), (41, 1), (2050, 2)])
+def test_swiglu_of_far_negative_gates(torch, b1, tokens, experts):
+    """Gates from -80 to -100, where the hardware's reciprocal passes through
+    its smallest numbers to 0: with values as large as inputs of fp16 make them
+    here (2^22) the result is a zero of the value's other sign."""
+    say(f"swiglu far gates {tokens} {experts}")
+    in_dim, f = 64, 64
+    a = torch.zeros(tokens, in_dim, device="cuda")
+    a[:, 0] = 80.0 + 0.5 * (torch.arange(tokens, device="cuda") % 41)
+    # gates -a[0], values +-2^15 a[0]
+    w = torch.zeros(experts, 2 * f, in_dim // 32, 6, dtype=torch.uint8, device="cuda")
+    scale = torch.ones(experts, 2 * f, in_dim // 32, 1, device="cuda")
+    scale[:, f:] = 2.0 ** 15
+    w[..., :2] = scale.half().view(torch.uint8)
+    w[:, f:, :, 2:] = 255
+    w[:, f + 1::2, :, 2:] = 0
+    expert = torch.arange(tokens, dtype=torch.int32).view(-1, 1) % experts
+    r = routes_of(torch, b1, expert, experts)
+    nf = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = b1.linear_experts(b1.pack_act_f16(a), w.flatten(), r, in_dim, 2 * f, act="swiglu", packed=True, nonfinite=nf)
+    got = ref.unpack(y, tokens, f)
+    assert bool((got == 0).all()) and int(nf) == 0
+    assert bool(got[:, ::2].signbit().all()) and not bool(got[:, 1::2].signbit().any())
