@@ -841,3 +841,65 @@ def test_swiglu_of_far_negative_gates(torch, b1, tokens, experts):
     got = ref.unpack(y, tokens, f)
     assert bool((got == 0).all()) and int(nf) == 0
     assert bool(got[:, ::2].signbit().all()) and not bool(got[:, 1::2].signbit().any())
+
+
+def test_the_most_routes(torch, b1):
+    """2^24 - 1 routes, the most that is accepted, nearly all of one expert:
+    the router's 16-bit counts of its work-groups full, and launches of close to
+    2^32 threads.  Whole activations and scales: rows are exact."""
+    tokens, in_dim, out_dim = (1 << 24) - 1, 64, 4
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of free device memory")
+    say("the most routes")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    logits = torch.zeros(tokens, 2, device="cuda")
+    other = torch.randint(0, tokens, (1000,), generator=g, device="cuda")
+    logits[other, 1] = 1.0
+    r = b1.route(logits, 1)
+    expert = (logits[:, 1] > 0).int()
+    assert torch.equal(r.expert.flatten(), expert) and bool((r.weight == 1).all())
+    order = torch.argsort(expert, stable=True)
+    first = tokens - int(expert.sum())
+    assert r.start.tolist() == [0, first, tokens] and torch.equal(r.order.long(), order)
+    assert torch.equal(r.place.flatten()[order], torch.arange(tokens, dtype=torch.int32, device="cuda"))
+    a = torch.randint(-3, 4, (tokens, in_dim), generator=g, device="cuda", dtype=torch.int8).half()
+    w = torch.randint(0, 256, (2, out_dim, in_dim // 32, 6), generator=g, device="cuda", dtype=torch.uint8)
+    w[..., :2] = torch.ones(2, out_dim, in_dim // 32, 1, device="cuda").half().view(torch.uint8)
+    y = b1.linear_experts(a.view(torch.uint8), w.flatten(), r, in_dim, out_dim)
+    bits = torch.arange(8, device="cuda", dtype=torch.uint8)
+    sign = 2.0 * ((w[..., 2:, None] >> bits) & 1).float().view(2, out_dim, in_dim) - 1.0
+    c = torch.arange(in_dim, device="cuda")  # column c of a row is stored here
+    stored = c // 32 * 32 + 2 * (c % 16) + c % 32 // 16
+    for e, (lo, hi) in enumerate(((0, first), (first, tokens))):
+        for at in torch.arange(lo, hi, device="cuda").split(1 << 21):
+            x = a[order[at]][:, stored].float()
+            want = torch.stack([(x * sign[e, n]).sum(1) for n in range(out_dim)], 1)
+            assert torch.equal(y[at], want)
+    x = normal(torch, 2, tokens, out_dim)
+    out = b1.combine_experts(y, r, residual=x)
+    assert torch.equal(out[order], y + x[order])
+    del a, y, x, out
+    torch.cuda.empty_cache()
+
+
+def test_combine_of_more_than_32_bits_of_threads(torch, b1):
+    """Tokens and columns whose work-groups have over 2^32 threads in all."""
+    tokens, h = (1 << 23) + 3, 1028
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    if free < 90 << 30:
+        pytest.skip("needs 90 GB of free device memory")
+    say("combine of more than 32 bits of threads")
+    place = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device="cuda").view(tokens, 1)
+    r = b1.Routes(torch.zeros_like(place), torch.ones(tokens, 1, device="cuda"),
+                  torch.tensor([0, tokens], dtype=torch.int32, device="cuda"), place.flatten(), place)
+    y = torch.empty(tokens, h, device="cuda").normal_()
+    out = torch.full((tokens, h), math.nan, device="cuda")
+    assert b1.combine_experts(y, r, out=out) is out
+    for at in torch.arange(tokens, device="cuda").split(1 << 20):
+        assert torch.equal(out[at], y[tokens - 1 - at])
+    del y, out
+    torch.cuda.empty_cache()
