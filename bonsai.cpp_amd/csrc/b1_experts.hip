@@ -100,7 +100,7 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
     }
 #pragma unroll
     for (int i = 0; i < EL; ++i) {
-        nan |= x[i] != x[i] || (!a.sigmoid && x[i] == INFINITY);
+        nan |= x[i] != x[i];
         hi[i] = x[i] > -INFINITY ? key_of(x[i]) : x[i] != x[i] ? kNanKey : 0u;
         top = max(top, hi[i]);
     }
@@ -125,6 +125,7 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, int token) {
         }
         if (!a.sigmoid) sum = wave_sum(sum);
         // an infinite logit: weights NaN, chosen by the logits of those not off
+        nan |= !a.sigmoid && peak == INFINITY;
         const bool by_score = a.sigmoid || sum < (double)INFINITY;
 #pragma unroll
         for (int i = 0; i < EL; ++i) {
