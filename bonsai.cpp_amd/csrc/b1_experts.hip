@@ -550,14 +550,17 @@ __device__ __forceinline__ void interleave() {
 
 // y = W a for up to 16 rows of one expert and `per` steps of 64 weight rows.
 //
-// The weights are read once a group (6 bytes a block of 32); what bounds it is
-// making fp16 of them and multiplying, 27 vector operations and four MFMAs a
-// block that overlap little: 512 rows over 128 experts, K = 2048, 1536 weight
-// rows (75 MB) 24.5 us, the same loads and sums without expansion or MFMAs
-// 16.5, the arithmetic without the loads 22.6.  Expanding a block beside the
-// MFMAs of the one before in a fixed order, two MFMA chains, two steps of loads
-// ahead: no gain.  The sums of each step by another wave first: spread over all
-// of them it took 1.4 us more.
+// The weights are read once a group (6 bytes a block of 32); 64 blocks, one a
+// lane, take 27 vector operations and four MFMAs.  512 rows over 128 experts,
+// K = 2048, 1536 weight rows (75 MB) 24.5 us, the same loads and sums without
+// expansion or MFMAs 16.5, the arithmetic without the loads 22.6.  What bounds
+// it is that little runs beside anything else: by its counters a SIMD's matrix
+// unit is busy 18 % of the time and its vector unit 38 %, with 2 waves on it
+// that wait for data 37 % of theirs and 37 % to issue.  Expanding a block
+// beside the MFMAs of the one before in a fixed order, two MFMA chains, two
+// steps of loads ahead: no gain.  The sums of each step by another wave first:
+// spread over all of them it took 1.4 us more.  Eight waves of four 256s and
+// fp32 rows spill 4 registers a step, nothing else does.
 //
 // MFMA 16x16x32 with 16 weight rows as the A operand and the rows of
 // activations as the B operand.  A wave takes U * 256 of K and lane (li, g)
@@ -749,16 +752,20 @@ __global__ __launch_bounds__(NW * 64, 2) void b1_experts_few_kernel(ExpertArgs a
 //
 // Bound by the matrix units: in the loop over K, 128-row tiles run at 1.4
 // PFLOP/s counting the rows they do not have (clock about 1.8 GHz at the
-// board's power limit, where a library product of 8192^3 runs at 1.29).  65536
-// rows over 128 experts, K = 2048, 1536 weight rows with SwiGLU: 361 to 381 us
-// by board = 1.08 to 1.14 PFLOP/s of rows there are; one work-group a tile with
-// its sums stored through LDS took 459.  Fp32 rows add their bytes' time
-// (K = 768, 2048 columns, 537 MB: 287 to 302 us): the stores hold up the loads
-// of the CU's other work-group, counted waits or not.
+// board's power limit, where a library product of 8192^3 runs at 1.29 to 1.35
+// by board); over the whole call the matrix units are busy 64 % of the time
+// and the vector units 26 %.  65536 rows over 128 experts, K = 2048, 1536
+// weight rows with SwiGLU: 361 to 381 us by board = 1.08 to 1.14 PFLOP/s of
+// rows there are; one work-group a tile with its sums stored through LDS took
+// 459.  Fp32 rows add their bytes' time (K = 768, 2048 columns, 537 MB: 287 to
+// 302 us): the stores hold up the loads of the CU's other work-group, counted
+// waits or not.
 // Branches that skip the upper 64 rows of tiles without any saved what they
 // cost.  One loop over all stages, the reads behind the last one wasted: with
 // the last stages apart the compiler copied the sums between loops and spilled
-// (405 us).
+// in them (405 us).  128-row tiles take all 256 registers: one value is stored
+// to memory once a work-group and read once a tile; the loop itself spills
+// none.
 //
 // MFMA, 16 weight rows as the A operand, rows of activations as the
 // B operand.  A stage is 64 of K: BM rows of 128 bytes, shared by the waves,

@@ -768,8 +768,9 @@ enum { BONSAI_B1_SCORE_SOFTMAX = 0, BONSAI_B1_SCORE_SIGMOID = 1 };
  * (or bias) is -inf is off: never chosen, so that a token may have fewer than
  * top_k routes, or none.  The score is the softmax over all the token's
  * experts or the sigmoid of the logit; the weight is the chosen one's score,
- * divided with `renormalize` by the sum of the token's chosen ones (0 where
- * that is 0), times `scale`.  The bias is no part of it.
+ * divided with `renormalize` by the sum of the token's chosen ones (with
+ * sigmoids 0 where that is 0 in 64 bits: logits below -709), times `scale`.
+ * The bias is no part of it.
  * A NaN among a token's logits or scores, or with softmax +inf, makes its
  * weights NaN (NaN is chosen behind every number; with softmax and +inf the
  * choice goes by the logits of the experts that are not off).
